@@ -251,6 +251,127 @@ int st_attention_static(int device, int mode, int heads, int head_dim, int windo
                         const float* q, const void* keys, const void* values, float* out, void* stream);
 const char* st_attention_static_error(void);
 
+/* ---- Window caches with sinks, and attention over them --------------------
+ *
+ * Operators on one layer's state for callers that run their own layers. No
+ * counterpart in the reference beyond its ring cache and split-window attention.
+ *
+ * A cache holds, for every stream and key/value head, `sinks` slots that the
+ * first positions keep for good, then a ring of `window` slots: position t
+ * lives in slot t when t < sinks and in slot sinks + (t - sinks) % window
+ * otherwise (sinks = 0 is the runtime's own ring). Keys are stored rotated, at
+ * their absolute positions. Rows are fp32, fp16, bf16 or 4 bits.
+ *
+ * 4-bit rows (ST_CACHE_INT4): every ST_CACHE_GROUP columns of a row share one
+ * bf16 scale and one bf16 lowest value, stored as the pair {scale, lowest}; a
+ * value stands for lowest + scale * code, code 0..15, two codes a byte, the
+ * even column in the low bits. Quantising takes lowest = bf16(min), scale =
+ * bf16((max - min) * (1/15)) and code = rint((x - lowest) / scale) clamped to
+ * 0..15 (0 where the scale is 0). A group with a non-finite value, or whose
+ * max - min or bf16(min) is not finite, reads back as NaN.
+ *
+ * All pointers are device memory of `device`, rows start on 16-byte
+ * boundaries, and work is queued on `stream` (a cudaStream_t) without waiting.
+ * Positions and starts are read on the device, so a captured graph replays
+ * with new ones. Each call returns ST_OK or an ST_ERR_* code with its message
+ * in st_cache_error() (one per thread). A CUDA error already pending on the
+ * calling thread is reported as ST_ERR_CUDA and left pending. */
+#define ST_CACHE_INT4 3
+#define ST_CACHE_GROUP 32
+#define ST_CACHE_MAX_HEAD_DIM 256
+
+typedef struct {
+  int device;
+  int type;                 /* st_mode of the rows, or ST_CACHE_INT4 */
+  int streams, heads;       /* streams and key/value heads, 1..65535 each */
+  int head_dim;             /* a multiple of 8 (INT4: of 32) up to 256 */
+  int sinks, window;        /* sinks >= 0, window >= 1, sum at most 2^30 */
+  int64_t stream_stride;    /* rows between streams: [stream][head][slot][head_dim] is heads * (sinks + window) */
+  int64_t head_stride;      /* rows between heads */
+  void *keys, *values;      /* rows of head_dim values of `type`, slots contiguous */
+  void *key_scales, *value_scales; /* INT4: [stream][head][slot][head_dim / 32][2] bf16, strides as the rows'; else NULL */
+} st_cache;
+
+/* Rows of queries, keys, values or outputs: [rows][heads][head_dim], the
+ * columns contiguous; strides in elements, multiples of 16 bytes. */
+typedef struct {
+  void* data;
+  int64_t row_stride, head_stride;
+} st_rows;
+
+/* Adds new rows to every stream's cache: per head, RMS norm of the query and
+ * key rows, rotation by their position, and the insert of keys and values.
+ *   norm      x * gain / sqrt(mean(x^2) + epsilon); a NULL gain skips the norm of that side
+ *   rotation  pair (2p, 2p + 1), p < rotary, by the angle position * frequencies[p]
+ *             (angle and its reduction in 64 bits; columns past 2 * rotary pass)
+ * Stream s owns rows starts[s] .. starts[s + 1] - 1 (starts NULL: row s alone,
+ * rows == streams) at positions positions[s], positions[s] + 1, ... A stream at
+ * a negative position is idle: its cache stays, and its rows of q_out and k_out
+ * become 0. Rows before starts[0] or behind the last stream's are left as they
+ * were. Of a stream's new rows only those still in the window, or at a sink
+ * position, are inserted. Sums and angles are fp32 or wider; each output is
+ * rounded once (4-bit rows are quantised from the fp32 values). */
+typedef struct {
+  int mode;                 /* st_mode of q, k, v, q_out, k_out: the cache's type, or fp16/bf16 for INT4 */
+  int heads;                /* query heads */
+  int64_t rows;             /* rows of q, k, v, up to 2^31 - 1 */
+  st_rows q, k, v;
+  st_rows q_out;            /* normed and rotated queries; may be q itself */
+  st_rows k_out;            /* the same of the keys, or data NULL; may be k itself */
+  const float *q_gain, *k_gain; /* [head_dim], or NULL */
+  float epsilon;            /* >= 0 */
+  int rotary;               /* rotated pairs, 0 .. head_dim / 2 */
+  const double* frequencies;    /* [rotary] radians per position */
+  const int64_t* positions; /* [streams] position of each stream's first new row */
+  const int32_t* starts;    /* [streams + 1] non-decreasing within 0 .. rows, or NULL */
+} st_append;
+int st_cache_append(const st_cache* cache, const st_append* args, void* stream);
+
+/* One query row per stream over its cache: out = softmax(scale q K^T) V over
+ * the slots 0 .. min(position + 1, sinks + window) - 1 of key head
+ * h / (heads / cache heads), position being that of the newest inserted row.
+ * Slots past those are not looked at, whatever they hold. A negative position
+ * gives a row of zeros.
+ * `workspace` holds the partial results of a split over the slots:
+ * st_cache_attention_workspace() bytes (0 for some shapes; then NULL will do),
+ * on a 256-byte boundary. Calls that may overlap need workspaces of their own. */
+typedef struct {
+  int mode;                 /* st_mode of q and out: the cache's type, or fp16/bf16 for INT4 */
+  int heads;                /* query heads, a multiple of the cache's */
+  float scale;              /* usually 1 / sqrt(head_dim) */
+  st_rows q, out;           /* [streams][heads][head_dim] */
+  const int64_t* positions; /* [streams] */
+  void* workspace;
+  size_t workspace_bytes;
+} st_attend;
+int st_cache_attention_workspace(const st_cache* cache, int heads, size_t* bytes);
+int st_cache_attention(const st_cache* cache, const st_attend* args, void* stream);
+
+/* What the rows of a 4-bit cache stand for, as `mode` rows
+ * [stream][head][slot][head_dim] (contiguous): every slot, written or not. */
+int st_cache_unpack(const st_cache* cache, int mode, void* keys, void* values, void* stream);
+
+/* Causal attention of whole sequences, packed one after another: row i of a
+ * sequence sees that sequence's rows j <= i with i - j < window or j < sinks.
+ * Sequence s is rows starts[s] .. starts[s + 1] - 1 (starts NULL: one
+ * sequence, all rows). Rows outside every sequence are not read into any
+ * result and their outputs are left as they were. */
+typedef struct {
+  int device;
+  int mode;                 /* st_mode of q, k, v and out */
+  int heads, kv_heads;      /* heads a multiple of kv_heads */
+  int head_dim;             /* a multiple of 8 up to 256 */
+  int sequences;
+  int64_t rows;             /* up to 2^31 - 1 */
+  int window, sinks;        /* window >= 1, sinks >= 0 */
+  float scale;
+  st_rows q, k, v, out;
+  const int32_t* starts;    /* [sequences + 1] non-decreasing within 0 .. rows, or NULL */
+} st_window;
+int st_window_attention(const st_window* args, void* stream);
+
+const char* st_cache_error(void);
+
 /* Scheduled-arrival replay (reference bench/Main.cpp:282-343, statistics
  * 416-447): event i of `inputs` ([count][features]) arrives at
  * i / rate seconds after the start (bursty: in groups of 16 arriving at the

@@ -1,0 +1,252 @@
+// st_append.cu -- per-head norm, rotation and cache insert in one pass
+// (st_cache_append), and the values 4-bit rows stand for (st_cache_unpack).
+//
+// One CTA takes one row (one position of one stream) with all its heads. The
+// angles depend on the position alone, so each pair's cosine and sine is found
+// once per row and shared by every head through shared memory: position *
+// frequency / (2 pi) in 64 bits, the whole turns dropped there, and only the
+// fraction goes to sincospi in fp32 (a position of 2^20 keeps an angle to
+// 2^-24 turns, where an fp32 product would lose it to 2^-4).
+// A head's row is a group of lanes with 8 columns each; the mean square is a
+// shuffle sum inside the group. Every row is read once and written once: the
+// bound is memory.
+#include "st_cache.cuh"
+#include "st_cache_host.h"
+
+namespace st {
+namespace {
+
+constexpr int kAppendThreads = 256;
+constexpr int kMaxPairs = ST_CACHE_MAX_HEAD_DIM / 2;
+
+struct AppendArgs {
+  void* q; void* k; void* v; void* q_out; void* k_out;
+  long long q_row, q_head, k_row, k_head, v_row, v_head, qo_row, qo_head, ko_row, ko_head;  // elements
+  void* keys; void* values;
+  unsigned* key_scales; unsigned* value_scales;
+  long long stream_stride, head_stride;  // cache rows
+  const float* q_gain; const float* k_gain;
+  const double* frequencies;
+  const long long* positions;
+  const int* starts;
+  int rows, streams, heads, kv_heads, head_dim, rotary, sinks, window;
+  float epsilon;
+};
+
+template <typename T, int LANES, bool INT4>
+__global__ void __launch_bounds__(kAppendThreads) k_cache_append(const AppendArgs a) {
+  __shared__ float2 turn[kMaxPairs];
+  __shared__ int sh_slot;
+  __shared__ int sh_stream;
+  const int row = blockIdx.x, tid = threadIdx.x;
+  // the stream that owns this row: the number of streams that end at or before it
+  int stream = row, first = row, last = row + 1;
+  if (a.starts) {
+    int ended = 0;
+    for (int base = 0; base < a.streams; base += kAppendThreads) {
+      const int s = base + tid;
+      ended += __syncthreads_count(s < a.streams && a.starts[s + 1] <= row);
+    }
+    stream = ended;
+    if (stream >= a.streams) return;  // behind the last stream
+    first = clamp_row(a.starts[stream], a.rows);
+    last = clamp_row(a.starts[stream + 1], a.rows);
+    if (row < first || row >= last) return;  // before the first stream
+  }
+  const long long p0 = a.positions[stream];
+  const bool idle = p0 < 0;
+  const long long position = p0 + (row - first);
+  for (int p = tid; p < a.rotary; p += kAppendThreads) {
+    const double t = (double)position * a.frequencies[p] * 0.15915494309189533577;  // 1 / (2 pi)
+    float s, c;
+    sincospif(2.f * (float)(t - rint(t)), &s, &c);
+    turn[p] = make_float2(c, s);
+  }
+  if (tid == 0) {
+    // inserted: sink positions, and those the stream's last `window` rows hold
+    const long long newest = p0 + (last - 1 - first);
+    int slot = -1;
+    if (!idle) {
+      if (position < a.sinks) slot = (int)position;
+      else if (position > newest - a.window) slot = a.sinks + (int)((position - a.sinks) % a.window);
+    }
+    sh_slot = slot;
+    sh_stream = stream;
+  }
+  __syncthreads();
+  const int slot = sh_slot;
+  const int lane = tid % LANES, col = lane * 8;
+  const unsigned mask = LANES == 32 ? 0xffffffffu : ((1u << LANES) - 1u) << ((tid & 31) / LANES * LANES);
+  const bool on = col < a.head_dim;
+  const int tasks = a.heads + 2 * a.kv_heads;
+  for (int task = tid / LANES; task < tasks; task += kAppendThreads / LANES) {
+    const bool is_q = task < a.heads, is_v = task >= a.heads + a.kv_heads;
+    const int head = is_q ? task : is_v ? task - a.heads - a.kv_heads : task - a.heads;
+    if (!is_q && slot < 0 && (is_v || !a.k_out)) continue;
+    const T* in = is_q ? static_cast<const T*>(a.q) + row * a.q_row + head * a.q_head
+                : is_v ? static_cast<const T*>(a.v) + row * a.v_row + head * a.v_head
+                       : static_cast<const T*>(a.k) + row * a.k_row + head * a.k_head;
+    float f[8] = {};
+    if (on && !idle) load8(in + col, f);
+    if (!is_v && !idle) {
+      const float* gain = is_q ? a.q_gain : a.k_gain;
+      if (gain) {
+        float sum = 0.f;
+#pragma unroll
+        for (int i = 0; i < 8; ++i) sum = fmaf(f[i], f[i], sum);
+#pragma unroll
+        for (int o = 1; o < LANES; o *= 2) sum += __shfl_xor_sync(mask, sum, o);
+        const float scale = 1.0f / sqrtf(sum / (float)a.head_dim + a.epsilon);
+        if (on) {
+          float g[8];
+          load8(gain + col, g);
+#pragma unroll
+          for (int i = 0; i < 8; ++i) f[i] = f[i] * scale * g[i];
+        }
+      }
+#pragma unroll
+      for (int i = 0; i < 4; ++i) {
+        if (col / 2 + i < a.rotary) {
+          const float2 t = turn[col / 2 + i];
+          const float x = f[2 * i], y = f[2 * i + 1];
+          f[2 * i] = x * t.x - y * t.y;
+          f[2 * i + 1] = x * t.y + y * t.x;
+        }
+      }
+    }
+    if (is_q) {
+      if (on) store8(static_cast<T*>(a.q_out) + row * a.qo_row + head * a.qo_head + col, f);
+      continue;
+    }
+    if (!is_v && a.k_out && on) store8(static_cast<T*>(a.k_out) + row * a.ko_row + head * a.ko_head + col, f);
+    if (slot < 0) continue;
+    const long long at = stream * a.stream_stride + head * a.head_stride + slot;
+    if (INT4) {
+      unsigned pair;
+      const unsigned codes = encode8(f, mask, &pair);
+      if (on) {
+        static_cast<unsigned*>(is_v ? a.values : a.keys)[at * (a.head_dim / 8) + lane] = codes;
+        if (lane % 4 == 0) (is_v ? a.value_scales : a.key_scales)[at * (a.head_dim / 32) + lane / 4] = pair;
+      }
+    } else if (on) {
+      store8(static_cast<T*>(is_v ? a.values : a.keys) + at * a.head_dim + col, f);
+    }
+  }
+}
+
+template <typename T, bool INT4>
+void launch_append(const AppendArgs& a, cudaStream_t s) {
+  switch (lanes_per_row(a.head_dim)) {
+    case 1: if constexpr (!INT4) k_cache_append<T, 1, INT4><<<a.rows, kAppendThreads, 0, s>>>(a); break;
+    case 2: if constexpr (!INT4) k_cache_append<T, 2, INT4><<<a.rows, kAppendThreads, 0, s>>>(a); break;
+    case 4: k_cache_append<T, 4, INT4><<<a.rows, kAppendThreads, 0, s>>>(a); break;
+    case 8: k_cache_append<T, 8, INT4><<<a.rows, kAppendThreads, 0, s>>>(a); break;
+    case 16: k_cache_append<T, 16, INT4><<<a.rows, kAppendThreads, 0, s>>>(a); break;
+    default: k_cache_append<T, 32, INT4><<<a.rows, kAppendThreads, 0, s>>>(a); break;
+  }
+}
+
+struct UnpackArgs {
+  const unsigned* codes[2];
+  const unsigned* scales[2];
+  void* out[2];
+  long long stream_stride, head_stride, total;  // total: 8-column pieces of one side
+  int heads, slots, pieces;                     // pieces per row
+};
+
+template <typename T>
+__global__ void __launch_bounds__(256) k_cache_unpack(const UnpackArgs a) {
+  const int side = blockIdx.y;
+  for (long long i = blockIdx.x * 256ll + threadIdx.x; i < a.total; i += gridDim.x * 256ll) {
+    const long long r = i / a.pieces;
+    const int piece = (int)(i - r * a.pieces);
+    const long long sh = r / a.slots, stream = sh / a.heads;
+    const long long at = stream * a.stream_stride + (sh - stream * a.heads) * a.head_stride + (r - sh * a.slots);
+    float f[8];
+    decode8(a.codes[side][at * a.pieces + piece], a.scales[side][at * (a.pieces / 4) + piece / 4], f);
+    store8(static_cast<T*>(a.out[side]) + i * 8, f);
+  }
+}
+
+}  // namespace
+}  // namespace st
+
+using namespace st;
+
+extern "C" {
+
+int st_cache_append(const st_cache* c, const st_append* p, void* stream) {
+  int rc = check_cache(c, true);
+  if (rc != ST_OK) return rc;
+  if (!p) return cache_fail(ST_ERR_INVALID, "null arguments");
+  if (p->mode < ST_MODE_FP32 || p->mode > ST_MODE_BF16) return cache_fail(ST_ERR_INVALID, "unknown row mode");
+  if (c->type == ST_CACHE_INT4 ? p->mode == ST_MODE_FP32 : p->mode != c->type)
+    return cache_fail(ST_ERR_INVALID, "rows are of the cache's type, or fp16 or bf16 for a 4-bit cache");
+  if (p->heads < 1 || p->heads > 65535) return cache_fail(ST_ERR_INVALID, "query heads are 1 to 65535");
+  if (p->rows < 0 || p->rows > INT32_MAX) return cache_fail(ST_ERR_INVALID, "rows are 0 to 2^31 - 1");
+  if (!p->starts && p->rows != c->streams)
+    return cache_fail(ST_ERR_INVALID, "without starts there is one row for each stream");
+  if (p->rows == 0) return ST_OK;
+  if ((rc = check_rows(p->q, "q", p->mode, p->rows, p->heads, c->head_dim, false)) != ST_OK ||
+      (rc = check_rows(p->k, "k", p->mode, p->rows, c->heads, c->head_dim, false)) != ST_OK ||
+      (rc = check_rows(p->v, "v", p->mode, p->rows, c->heads, c->head_dim, false)) != ST_OK ||
+      (rc = check_rows(p->q_out, "q_out", p->mode, p->rows, p->heads, c->head_dim, true)) != ST_OK ||
+      (p->k_out.data && (rc = check_rows(p->k_out, "k_out", p->mode, p->rows, c->heads, c->head_dim, true)) != ST_OK))
+    return rc;
+  if (!p->positions) return cache_fail(ST_ERR_INVALID, "null positions");
+  if (!(p->epsilon >= 0.f) || p->epsilon > 3.0e38f) return cache_fail(ST_ERR_INVALID, "epsilon must be finite and >= 0");
+  if (p->rotary < 0 || p->rotary > c->head_dim / 2 || (p->rotary && !p->frequencies))
+    return cache_fail(ST_ERR_INVALID, "rotary is 0 to head_dim / 2, with a frequency for each");
+  for (const float* g : {p->q_gain, p->k_gain})
+    if (reinterpret_cast<uintptr_t>(g) % 16) return cache_fail(ST_ERR_INVALID, "gains must start on a 16-byte boundary");
+  DeviceScope scope(c->device);
+  if (scope.status() != ST_OK) return scope.status();
+  AppendArgs a{};
+  a.q = p->q.data; a.k = p->k.data; a.v = p->v.data; a.q_out = p->q_out.data; a.k_out = p->k_out.data;
+  a.q_row = p->q.row_stride; a.q_head = p->q.head_stride;
+  a.k_row = p->k.row_stride; a.k_head = p->k.head_stride;
+  a.v_row = p->v.row_stride; a.v_head = p->v.head_stride;
+  a.qo_row = p->q_out.row_stride; a.qo_head = p->q_out.head_stride;
+  a.ko_row = p->k_out.row_stride; a.ko_head = p->k_out.head_stride;
+  a.keys = c->keys; a.values = c->values;
+  a.key_scales = static_cast<unsigned*>(c->key_scales); a.value_scales = static_cast<unsigned*>(c->value_scales);
+  a.stream_stride = c->stream_stride; a.head_stride = c->head_stride;
+  a.q_gain = p->q_gain; a.k_gain = p->k_gain; a.frequencies = p->frequencies;
+  a.positions = reinterpret_cast<const long long*>(p->positions); a.starts = p->starts;
+  a.rows = (int)p->rows; a.streams = c->streams; a.heads = p->heads; a.kv_heads = c->heads;
+  a.head_dim = c->head_dim; a.rotary = p->rotary; a.sinks = c->sinks; a.window = c->window; a.epsilon = p->epsilon;
+  cudaStream_t s = static_cast<cudaStream_t>(stream);
+  const bool four = c->type == ST_CACHE_INT4;
+  if (p->mode == ST_MODE_FP32) launch_append<float, false>(a, s);
+  else if (p->mode == ST_MODE_FP16) four ? launch_append<__half, true>(a, s) : launch_append<__half, false>(a, s);
+  else four ? launch_append<__nv_bfloat16, true>(a, s) : launch_append<__nv_bfloat16, false>(a, s);
+  return cache_cuda(cudaGetLastError(), "append launch: ");
+}
+
+int st_cache_unpack(const st_cache* c, int mode, void* keys, void* values, void* stream) {
+  int rc = check_cache(c, false);
+  if (rc != ST_OK) return rc;
+  if (c->type != ST_CACHE_INT4) return cache_fail(ST_ERR_INVALID, "only a 4-bit cache is unpacked");
+  if (mode < ST_MODE_FP32 || mode > ST_MODE_BF16) return cache_fail(ST_ERR_INVALID, "unknown row mode");
+  if (!keys || !values) return cache_fail(ST_ERR_INVALID, "null pointer");
+  if (reinterpret_cast<uintptr_t>(keys) % 16 || reinterpret_cast<uintptr_t>(values) % 16)
+    return cache_fail(ST_ERR_INVALID, "outputs must start on a 16-byte boundary");
+  DeviceScope scope(c->device);
+  if (scope.status() != ST_OK) return scope.status();
+  UnpackArgs a{};
+  a.codes[0] = static_cast<const unsigned*>(c->keys); a.codes[1] = static_cast<const unsigned*>(c->values);
+  a.scales[0] = static_cast<const unsigned*>(c->key_scales); a.scales[1] = static_cast<const unsigned*>(c->value_scales);
+  a.out[0] = keys; a.out[1] = values;
+  a.stream_stride = c->stream_stride; a.head_stride = c->head_stride;
+  a.heads = c->heads; a.slots = c->sinks + c->window; a.pieces = c->head_dim / 8;
+  a.total = (long long)c->streams * c->heads * a.slots * a.pieces;
+  const long long need = (a.total + 255) / 256, most = 16ll * sm_count(c->device);
+  const dim3 grid((unsigned)(need < most ? need : most), 2);
+  cudaStream_t s = static_cast<cudaStream_t>(stream);
+  if (mode == ST_MODE_FP32) k_cache_unpack<float><<<grid, 256, 0, s>>>(a);
+  else if (mode == ST_MODE_FP16) k_cache_unpack<__half><<<grid, 256, 0, s>>>(a);
+  else k_cache_unpack<__nv_bfloat16><<<grid, 256, 0, s>>>(a);
+  return cache_cuda(cudaGetLastError(), "unpack launch: ");
+}
+
+}  // extern "C"
