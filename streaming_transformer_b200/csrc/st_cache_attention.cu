@@ -145,8 +145,9 @@ __device__ __forceinline__ void let_next_kernel_start() { asm volatile("griddepc
 __device__ __forceinline__ void wait_for_previous_kernel() { asm volatile("griddepcontrol.wait;" ::: "memory"); }
 
 // ---------------------------------------------------------------- 16-bit and 4-bit rows
-// DB: blocks of 64 columns; NT: blocks of 8 query heads.
-template <typename T, int DB, int NT, bool INT4>
+// DB: blocks of 64 columns; NT: blocks of 8 query heads; FULL: head_dim is 64 DB, so that row offsets are constants
+// and no column is checked.
+template <typename T, int DB, int NT, bool INT4, bool FULL>
 __global__ void __launch_bounds__(kAttendThreads) k_attend_mma(const AttendArgs a) {
   constexpr int J = 2 * DB;   // pieces of 32 columns
   constexpr float kLift = std::is_same<T, __half>::value && !INT4 ? 10.f : 0.f;
@@ -201,74 +202,96 @@ __global__ void __launch_bounds__(kAttendThreads) k_attend_mma(const AttendArgs 
   for (int n = 0; n < NT; ++n) m[n][0] = m[n][1] = -INFINITY, l[n][0] = l[n][1] = 0.f;
 
   const long long row0 = stream * a.stream_stride + kv * a.head_stride;
-  const int row_bytes = INT4 ? a.head_dim / 2 : a.head_dim * 2, groups = a.head_dim / 32;
-  const char* kbase = static_cast<const char*>(a.keys) + row0 * row_bytes;
-  const char* vbase = static_cast<const char*>(a.values) + row0 * row_bytes;
+  const int dim = FULL ? DB * 64 : a.head_dim, groups = dim / 32, row_bytes = INT4 ? dim / 2 : dim * 2;
+  const int step = 16 * kAttendWarps;
+  int slot0 = first + warp * 16;
+  // this lane's first addresses of the tile to load next
+  const char* kp = static_cast<const char*>(a.keys) + (row0 + slot0 + g) * row_bytes + t * (INT4 ? 8 : 16);
+  const char* vp = static_cast<const char*>(a.values) + (row0 + slot0 + 2 * t) * row_bytes + g * (INT4 ? 4 : 16);
+  const unsigned* ksp = a.key_scales + (row0 + slot0 + g) * groups;
+  const unsigned* vsp = a.value_scales + (row0 + slot0 + g) * groups;
 
   // one tile in registers: loaded a step ahead of its use
   constexpr int KW = INT4 ? DB * 2 : J * 4, VW = INT4 ? DB : DB * 4;
   unsigned kf[2][KW], vf[4][VW], ks[2][INT4 ? J : 1], vs[2][INT4 ? J : 1];
 
-  // Slots past `last` load nothing and count as zeros, so that no value there matters.
-  auto load_k = [&](int slot0) {
+  auto load_scales = [&](unsigned(&f)[2][INT4 ? J : 1], const unsigned* sp, int at, bool whole) {
 #pragma unroll
     for (int r = 0; r < 2; ++r) {
-      const int slot = slot0 + g + 8 * r;
-      const char* p = kbase + (long long)slot * row_bytes;
+      const bool in = whole || at + g + 8 * r < last;
+      const unsigned* p = sp + 8 * r * groups;
+      if constexpr (FULL && J % 4 == 0) {
+#pragma unroll
+        for (int j = 0; j < J; j += 4) {
+          const uint4 u = in ? ld_row16(p + j) : make_uint4(0, 0, 0, 0);
+          f[r][j] = u.x; f[r][j + 1] = u.y; f[r][j + 2] = u.z; f[r][j + 3] = u.w;
+        }
+      } else if constexpr (FULL) {
+        const uint2 u = in ? ld_row8(p) : make_uint2(0, 0);
+        f[r][0] = u.x; f[r][1] = u.y;
+      } else {
+#pragma unroll
+        for (int j = 0; j < J; ++j) f[r][j] = in && j < groups ? ld_row4(p + j) : 0u;
+      }
+    }
+  };
+  // Slots past `last` load nothing and count as zeros, so that no value there matters; `whole`: the tile has none.
+  auto load_k = [&](int at, bool whole) {
+#pragma unroll
+    for (int r = 0; r < 2; ++r) {
+      const bool in = whole || at + g + 8 * r < last;
+      const char* p = kp + 8 * r * row_bytes;
       if constexpr (INT4) {
 #pragma unroll
         for (int i = 0; i < DB; ++i) {  // 16 columns: 64 i + 16 t
-          uint2 u = make_uint2(0, 0);
-          if (slot < last && i * 64 + t * 16 < a.head_dim) u = ld_row8(p + i * 32 + t * 8);
-          kf[r][2 * i] = u.x;
-          kf[r][2 * i + 1] = u.y;
+          const uint2 u = in && (FULL || i * 64 + t * 16 < dim) ? ld_row8(p + i * 32) : make_uint2(0, 0);
+          kf[r][2 * i] = u.x; kf[r][2 * i + 1] = u.y;
         }
-        const unsigned* sp = a.key_scales + (row0 + slot) * groups;
-#pragma unroll
-        for (int j = 0; j < J; ++j) ks[r][j] = slot < last && j < groups ? ld_row4(sp + j) : 0u;
       } else {
 #pragma unroll
         for (int j = 0; j < J; ++j) {
-          uint4 u = make_uint4(0, 0, 0, 0);
-          if (slot < last && j * 32 + t * 8 < a.head_dim) u = ld_row16(p + j * 64 + t * 16);
+          const uint4 u = in && (FULL || j * 32 + t * 8 < dim) ? ld_row16(p + j * 64) : make_uint4(0, 0, 0, 0);
           kf[r][4 * j] = u.x; kf[r][4 * j + 1] = u.y; kf[r][4 * j + 2] = u.z; kf[r][4 * j + 3] = u.w;
         }
       }
     }
+    if constexpr (INT4) load_scales(ks, ksp, at, whole);
   };
-  auto load_v = [&](int slot0) {
+  auto load_v = [&](int at, bool whole) {
 #pragma unroll
     for (int r = 0; r < 4; ++r) {
-      const int slot = slot0 + 2 * t + (r & 1) + 8 * (r >> 1);
-      const char* p = vbase + (long long)slot * row_bytes;
+      const int ahead = (r & 1) + 8 * (r >> 1);
+      const bool in = whole || at + 2 * t + ahead < last;
+      const char* p = vp + ahead * row_bytes;
 #pragma unroll
       for (int i = 0; i < DB; ++i) {
-        const bool on = slot < last && i * 64 + g * 8 < a.head_dim;
+        const bool on = in && (FULL || i * 64 + g * 8 < dim);
         if constexpr (INT4) {
-          vf[r][i] = on ? ld_row4(p + i * 32 + g * 4) : 0u;
+          vf[r][i] = on ? ld_row4(p + i * 32) : 0u;
         } else {
-          uint4 u = make_uint4(0, 0, 0, 0);
-          if (on) u = ld_row16(p + i * 128 + g * 16);
+          const uint4 u = on ? ld_row16(p + i * 128) : make_uint4(0, 0, 0, 0);
           vf[r][4 * i] = u.x; vf[r][4 * i + 1] = u.y; vf[r][4 * i + 2] = u.z; vf[r][4 * i + 3] = u.w;
         }
       }
     }
-    if constexpr (INT4) {
-#pragma unroll
-      for (int r = 0; r < 2; ++r) {
-        const int slot = slot0 + g + 8 * r;
-        const unsigned* sp = a.value_scales + (row0 + slot) * groups;
-#pragma unroll
-        for (int j = 0; j < J; ++j) vs[r][j] = slot < last && j < groups ? ld_row4(sp + j) : 0u;
-      }
-    }
+    if constexpr (INT4) load_scales(vs, vsp, at, whole);
+  };
+  auto fetch_k = [&](int at) {
+    if (at + 16 <= last) load_k(at, true);
+    else load_k(at, false);
+    kp += (long long)step * row_bytes;
+    if (INT4) ksp += step * groups;
+  };
+  auto fetch_v = [&](int at) {
+    if (at + 16 <= last) load_v(at, true);
+    else load_v(at, false);
+    vp += (long long)step * row_bytes;
+    if (INT4) vsp += step * groups;
   };
 
-  const int step = 16 * kAttendWarps;
-  int slot0 = first + warp * 16;
   if (slot0 < last) {
-    load_k(slot0);
-    load_v(slot0);
+    fetch_k(slot0);
+    fetch_v(slot0);
   }
   for (; slot0 < last; slot0 += step) {
     // S^T: slots g (c0, c1) and g + 8 (c2, c3), heads 8 n + 2 t, + 1
@@ -322,7 +345,7 @@ __global__ void __launch_bounds__(kAttendThreads) k_attend_mma(const AttendArgs 
       }
     }
     const int next = slot0 + step;
-    load_k(next);
+    if (next < last) fetch_k(next);
 
     const bool in0 = slot0 + g < last, in1 = slot0 + g + 8 < last;
     unsigned pf[NT][INT4 ? J : 1][2];
@@ -417,7 +440,7 @@ __global__ void __launch_bounds__(kAttendThreads) k_attend_mma(const AttendArgs 
         }
       }
     }
-    load_v(next);
+    if (next < last) fetch_v(next);
   }
 
   // this warp's part into shared memory, columns in their own order
@@ -615,17 +638,22 @@ int splits_of(const st_cache* c, int heads) {
   return n < 1 ? 1 : n > 1024 ? 1024 : (int)n;
 }
 
-template <typename T, bool INT4>
+template <typename T, bool INT4, bool FULL>
 void launch_mma(const AttendArgs& a, int per, dim3 grid, cudaStream_t s) {
   if (a.head_dim <= 64) {
-    if (per == 8) k_attend_mma<T, 1, 1, INT4><<<grid, kAttendThreads, 0, s>>>(a);
-    else k_attend_mma<T, 1, 2, INT4><<<grid, kAttendThreads, 0, s>>>(a);
+    if (per == 8) k_attend_mma<T, 1, 1, INT4, FULL><<<grid, kAttendThreads, 0, s>>>(a);
+    else k_attend_mma<T, 1, 2, INT4, FULL><<<grid, kAttendThreads, 0, s>>>(a);
   } else if (a.head_dim <= 128) {
-    if (per == 8) k_attend_mma<T, 2, 1, INT4><<<grid, kAttendThreads, 0, s>>>(a);
-    else k_attend_mma<T, 2, 2, INT4><<<grid, kAttendThreads, 0, s>>>(a);
+    if (per == 8) k_attend_mma<T, 2, 1, INT4, FULL><<<grid, kAttendThreads, 0, s>>>(a);
+    else k_attend_mma<T, 2, 2, INT4, FULL><<<grid, kAttendThreads, 0, s>>>(a);
   } else {
-    k_attend_mma<T, 4, 1, INT4><<<grid, kAttendThreads, 0, s>>>(a);
+    k_attend_mma<T, 4, 1, INT4, FULL><<<grid, kAttendThreads, 0, s>>>(a);
   }
+}
+template <typename T, bool INT4>
+void launch_mma(const AttendArgs& a, int per, dim3 grid, cudaStream_t s) {
+  if (a.head_dim == 64 || a.head_dim == 128 || a.head_dim == 256) launch_mma<T, INT4, true>(a, per, grid, s);
+  else launch_mma<T, INT4, false>(a, per, grid, s);
 }
 
 template <int LANES>
