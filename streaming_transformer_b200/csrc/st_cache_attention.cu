@@ -23,12 +23,14 @@
 // S^T leaves slots in rows and heads in columns; movmatrix turns each 8 x 8
 // piece of P into the B operand of the second product.
 //
-// 4-bit rows: codes 0..15 are exact 16-bit operands. Within a group of 32
-// columns sum q k = scale * sum q code + lowest * sum q, so the product runs on
-// the codes and the group's scale and lowest value enter in fp32 once per slot
-// and head. For values the scale is folded into the weight before its one
-// rounding (to bf16: its range holds any scale), and sum p * lowest is kept in
-// fp32 beside the product.
+// 4-bit rows become the 16-bit operands that a 16-bit cache would hold: a lane's
+// columns lie in one group, codes turn into exact 16-bit numbers two at a time,
+// and one packed multiply-add with the group's scale and lowest value rounds
+// once, to 2^-9 of the value (keys of fp16 rows: 2^-12), where the code itself
+// is off by up to half a scale, a thirtieth of the group's range. Values become
+// bf16 whatever the rows are: its range holds any scale. Folding the scales into
+// fp32 sums instead, without that rounding, took 1.5 to 2 times the instructions
+// and the kernel is bound by those (256 Large streams: 77 us).
 //
 // Softmax statistics are fp32: a running maximum per head (in units of log2),
 // the sum of unrounded weights, and output sums. Weights are rounded to the 16
@@ -103,24 +105,6 @@ __device__ __forceinline__ unsigned ld_row4(const void* p) {
   return r;
 }
 
-// Nibbles i and i + 4 of `w` as a pair of exact 16-bit numbers: the nibble in
-// the low mantissa bits of 2^10 (fp16) or 2^7 (bf16), which is taken off again.
-template <typename T>
-__device__ __forceinline__ unsigned code_pair(unsigned w, int i) {
-  if constexpr (std::is_same<T, __half>::value) {
-    unsigned x = ((w >> (4 * i)) & 0x000f000fu) | 0x64006400u;
-    const unsigned base = 0x64006400u;
-    const __half2 y = __hsub2(*reinterpret_cast<const __half2*>(&x), *reinterpret_cast<const __half2*>(&base));
-    return *reinterpret_cast<const unsigned*>(&y);
-  } else {
-    unsigned x = ((w >> (4 * i)) & 0x000f000fu) | 0x43004300u;
-    const unsigned base = 0x43004300u;
-    const __nv_bfloat162 y =
-        __hsub2(*reinterpret_cast<const __nv_bfloat162*>(&x), *reinterpret_cast<const __nv_bfloat162*>(&base));
-    return *reinterpret_cast<const unsigned*>(&y);
-  }
-}
-
 // Part of this CTA's split in tiles of `tile` slots: [first, last).
 __device__ __forceinline__ void split_slots(int seen, int tile, int split, int splits, int& first, int& last) {
   const int tiles = (seen + tile - 1) / tile, per = (tiles + splits - 1) / splits;
@@ -145,13 +129,41 @@ __device__ __forceinline__ void let_next_kernel_start() { asm volatile("griddepc
 __device__ __forceinline__ void wait_for_previous_kernel() { asm volatile("griddepcontrol.wait;" ::: "memory"); }
 
 // ---------------------------------------------------------------- 16-bit and 4-bit rows
-// DB: blocks of 64 columns; NT: blocks of 8 query heads; FULL: head_dim is 64 DB, so that row offsets are constants
-// and no column is checked.
-template <typename T, int DB, int NT, bool INT4, bool FULL>
+// {scale, lowest} twice over, as packed operands of T.
+template <typename T>
+__device__ __forceinline__ void group_operands(unsigned pair_a, unsigned pair_b, unsigned& scale, unsigned& lowest) {
+  if constexpr (std::is_same<T, __half>::value) {
+    scale = pack2((__half*)nullptr, group_scale(pair_a), group_scale(pair_b));
+    lowest = pack2((__half*)nullptr, group_lowest(pair_a), group_lowest(pair_b));
+  } else {
+    scale = __byte_perm(pair_a, pair_b, 0x5410);
+    lowest = __byte_perm(pair_a, pair_b, 0x7632);
+  }
+}
+// Nibble i of both halves of `w` as lowest + scale * code, rounded once. The
+// nibble in the low mantissa bits of 2^10 (fp16) or 2^7 (bf16) is an exact
+// number, from which the power is taken off again.
+template <typename T>
+__device__ __forceinline__ unsigned decode_pair(unsigned w, int i, unsigned scale, unsigned lowest) {
+  using T2 = typename std::conditional<std::is_same<T, __half>::value, __half2, __nv_bfloat162>::type;
+  const unsigned base = std::is_same<T, __half>::value ? 0x64006400u : 0x43004300u;
+  const unsigned x = ((w >> (4 * i)) & 0x000f000fu) | base;
+  const T2 c = __hsub2(*reinterpret_cast<const T2*>(&x), *reinterpret_cast<const T2*>(&base));
+  const T2 y = __hfma2(c, *reinterpret_cast<const T2*>(&scale), *reinterpret_cast<const T2*>(&lowest));
+  return *reinterpret_cast<const unsigned*>(&y);
+}
+
+// DB: blocks of 64 columns; NT: blocks of 8 query heads; FULL: head_dim is
+// 64 DB, so that row offsets are constants and no column is checked; ONE: one
+// query head a key head, so that the odd columns of S^T are not computed on.
+// A step takes TS tiles of 16 slots.
+template <typename T, int DB, int NT, bool INT4, bool FULL, bool ONE>
 __global__ void __launch_bounds__(kAttendThreads) k_attend_mma(const AttendArgs a) {
-  constexpr int J = 2 * DB;   // pieces of 32 columns
-  constexpr float kLift = std::is_same<T, __half>::value && !INT4 ? 10.f : 0.f;
-  using PT = typename std::conditional<INT4, __nv_bfloat16, T>::type;  // type of the second product
+  constexpr int J = 2 * DB;   // 16-bit: 16-byte pieces of a key row a lane holds
+  constexpr int TS = INT4 && DB * NT <= 2 ? 2 : 1;
+  constexpr int X = ONE ? 1 : 2;  // query heads a lane has of each block: 8 n + 2 t + x
+  using PT = typename std::conditional<INT4, __nv_bfloat16, T>::type;  // operands of the second product
+  constexpr float kLift = std::is_same<PT, __half>::value ? 10.f : 0.f;
   __shared__ float sh_o[kAttendWarps][NT * 8][DB * 64 + 4];
   __shared__ float sh_m[kAttendWarps][NT * 8], sh_l[kAttendWarps][NT * 8];
   const int split = blockIdx.x, kv = blockIdx.y / a.blocks, block = blockIdx.y % a.blocks, stream = blockIdx.z;
@@ -159,36 +171,118 @@ __global__ void __launch_bounds__(kAttendThreads) k_attend_mma(const AttendArgs 
   if (a.splits > 1) let_next_kernel_start();
   const int seen = slots_seen(a.positions[stream], a.slots);
   int first, last;
-  split_slots(seen, 16 * kAttendWarps, split, a.splits, first, last);
+  split_slots(seen, 16 * TS * kAttendWarps, split, a.splits, first, last);
   const int head0 = kv * a.group + block * NT * 8;                          // first query head of the block
   const int nheads = min(NT * 8, a.group - block * NT * 8);
 
-  // query fragments: columns 32 j + 8 t of head 8 n + g (4-bit: pairs (i, i + 4) of the 8 columns)
+  const long long row0 = stream * a.stream_stride + kv * a.head_stride;
+  const int dim = FULL ? DB * 64 : a.head_dim, groups = dim / 32, row_bytes = INT4 ? dim / 2 : dim * 2;
+  constexpr int kStep = 16 * TS * kAttendWarps;
+  int slot0 = first + warp * 16 * TS;
+  // this lane's first addresses of the tile to load next
+  const char* kp = static_cast<const char*>(a.keys) + (row0 + slot0 + g) * row_bytes + t * (INT4 ? 8 * DB : 16);
+  const char* vp = static_cast<const char*>(a.values) + (row0 + slot0 + 2 * t) * row_bytes + g * (INT4 ? 4 * DB : 16);
+  const unsigned* ksp = INT4 ? a.key_scales + (row0 + slot0 + g) * groups + t * DB / 2 : nullptr;
+  const unsigned* vsp = INT4 ? a.value_scales + (row0 + slot0 + 2 * t) * groups + g * DB / 4 : nullptr;
+
+  // one step's rows in registers, loaded a step ahead of their use
+  constexpr int KW = INT4 ? DB * 2 : J * 4, VW = INT4 ? DB : DB * 4, KG = INT4 ? (DB + 1) / 2 : 1;
+  unsigned kf[TS][2][KW], vf[TS][4][VW], ks[TS][2][KG], vs[TS][4];
+
+  // Slots past `last` load nothing and count as zeros, so that no value there matters; `whole`: the step has none.
+  auto load_k = [&](int at, bool whole) {
+#pragma unroll
+    for (int u = 0; u < TS; ++u)
+#pragma unroll
+      for (int r = 0; r < 2; ++r) {
+        const int ahead = 16 * u + 8 * r;
+        const bool in = whole || at + g + ahead < last;
+        const char* p = kp + ahead * row_bytes;
+        if constexpr (INT4) {  // columns 16 DB t .. + 16 DB - 1
+          if constexpr (DB == 1) {
+            const uint2 w = in && (FULL || t * 16 < dim) ? ld_row8(p) : make_uint2(0, 0);
+            kf[u][r][0] = w.x; kf[u][r][1] = w.y;
+          } else {
+#pragma unroll
+            for (int i = 0; i < DB / 2; ++i) {
+              const uint4 w = in && (FULL || t * 16 * DB + 32 * i < dim) ? ld_row16(p + 16 * i) : make_uint4(0, 0, 0, 0);
+              kf[u][r][4 * i] = w.x; kf[u][r][4 * i + 1] = w.y; kf[u][r][4 * i + 2] = w.z; kf[u][r][4 * i + 3] = w.w;
+            }
+          }
+#pragma unroll
+          for (int i = 0; i < KG; ++i)
+            ks[u][r][i] = in && (FULL || t * 16 * DB + 32 * i < dim) ? ld_row4(ksp + ahead * groups + i) : 0u;
+        } else {
+#pragma unroll
+          for (int j = 0; j < J; ++j) {
+            const uint4 w = in && (FULL || j * 32 + t * 8 < dim) ? ld_row16(p + j * 64) : make_uint4(0, 0, 0, 0);
+            kf[u][r][4 * j] = w.x; kf[u][r][4 * j + 1] = w.y; kf[u][r][4 * j + 2] = w.z; kf[u][r][4 * j + 3] = w.w;
+          }
+        }
+      }
+  };
+  auto load_v = [&](int at, bool whole) {
+#pragma unroll
+    for (int u = 0; u < TS; ++u)
+#pragma unroll
+      for (int r = 0; r < 4; ++r) {
+        const int ahead = 16 * u + (r & 1) + 8 * (r >> 1);
+        const bool in = whole || at + 2 * t + ahead < last;
+        const char* p = vp + ahead * row_bytes;
+        if constexpr (INT4) {  // columns 8 DB g .. + 8 DB - 1
+          const bool on = in && (FULL || g * 8 * DB < dim);
+          if constexpr (DB == 1) {
+            vf[u][r][0] = on ? ld_row4(p) : 0u;
+          } else if constexpr (DB == 2) {
+            const uint2 w = on ? ld_row8(p) : make_uint2(0, 0);
+            vf[u][r][0] = w.x; vf[u][r][1] = w.y;
+          } else {
+            const uint4 w = on ? ld_row16(p) : make_uint4(0, 0, 0, 0);
+            vf[u][r][0] = w.x; vf[u][r][1] = w.y; vf[u][r][2] = w.z; vf[u][r][3] = w.w;
+          }
+          vs[u][r] = on ? ld_row4(vsp + ahead * groups) : 0u;
+        } else {
+#pragma unroll
+          for (int i = 0; i < DB; ++i) {
+            const uint4 w = in && (FULL || i * 64 + g * 8 < dim) ? ld_row16(p + i * 128) : make_uint4(0, 0, 0, 0);
+            vf[u][r][4 * i] = w.x; vf[u][r][4 * i + 1] = w.y; vf[u][r][4 * i + 2] = w.z; vf[u][r][4 * i + 3] = w.w;
+          }
+        }
+      }
+  };
+  auto fetch_k = [&](int at) {
+    if (at + 16 * TS <= last) load_k(at, true);
+    else load_k(at, false);
+    kp += (long long)kStep * row_bytes;
+    if (INT4) ksp += kStep * groups;
+  };
+  auto fetch_v = [&](int at) {
+    if (at + 16 * TS <= last) load_v(at, true);
+    else load_v(at, false);
+    vp += (long long)kStep * row_bytes;
+    if (INT4) vsp += kStep * groups;
+  };
+  if (slot0 < last) {
+    fetch_k(slot0);
+    fetch_v(slot0);
+  }
+
+  // query fragments: the columns of this lane's key words, head 8 n + g (4-bit: pairs (i, i + 4) of each 8 columns)
   unsigned qf[NT][J][4];
-  float qsum[NT][J][2];  // 4-bit: sum of the group's columns for heads 8 n + 2 t, + 1
 #pragma unroll
   for (int n = 0; n < NT; ++n) {
     const bool head_on = n * 8 + g < nheads;
     const T* qp = static_cast<const T*>(a.q) + stream * a.q_row + (long long)(head0 + n * 8 + g) * a.q_head;
 #pragma unroll
     for (int j = 0; j < J; ++j) {
+      const int col = INT4 ? t * 16 * DB + 8 * j : j * 32 + t * 8;
       uint4 u = make_uint4(0, 0, 0, 0);
-      // 4-bit: the group's 8-column words reach lanes 0 .. 3 in the order 0, 2, 1, 3 (see the exchange below)
-      const int col = j * 32 + (INT4 ? (t & 1) * 16 + (t >> 1) * 8 : t * 8);
-      if (head_on && col < a.head_dim) u = *reinterpret_cast<const uint4*>(qp + col);
+      if (head_on && col < dim) u = *reinterpret_cast<const uint4*>(qp + col);
       if (INT4) {
         qf[n][j][0] = __byte_perm(u.x, u.z, 0x5410);  // columns 0, 4
         qf[n][j][1] = __byte_perm(u.x, u.z, 0x7632);  // 1, 5
         qf[n][j][2] = __byte_perm(u.y, u.w, 0x5410);  // 2, 6
         qf[n][j][3] = __byte_perm(u.y, u.w, 0x7632);  // 3, 7
-        float f[8], s = 0.f;
-        load8(reinterpret_cast<const T*>(&u), f);
-#pragma unroll
-        for (int i = 0; i < 8; ++i) s += f[i];
-        s += __shfl_xor_sync(0xffffffffu, s, 1);
-        s += __shfl_xor_sync(0xffffffffu, s, 2);
-        qsum[n][j][0] = __shfl_sync(0xffffffffu, s, (2 * t) * 4);
-        qsum[n][j][1] = __shfl_sync(0xffffffffu, s, (2 * t + 1) * 4);
       } else {
         qf[n][j][0] = u.x; qf[n][j][1] = u.y; qf[n][j][2] = u.z; qf[n][j][3] = u.w;
       }
@@ -196,173 +290,64 @@ __global__ void __launch_bounds__(kAttendThreads) k_attend_mma(const AttendArgs 
   }
 
   float o[NT][DB][4][4] = {};        // [head block][column block][m-tile]
-  float olow[NT][J][2] = {};         // 4-bit: sum of weight * lowest, this lane's slots
-  float m[NT][2], l[NT][2];
+  float m[NT][X], l[NT][X];
 #pragma unroll
-  for (int n = 0; n < NT; ++n) m[n][0] = m[n][1] = -INFINITY, l[n][0] = l[n][1] = 0.f;
+  for (int n = 0; n < NT; ++n)
+#pragma unroll
+    for (int x = 0; x < X; ++x) m[n][x] = -INFINITY, l[n][x] = 0.f;
 
-  const long long row0 = stream * a.stream_stride + kv * a.head_stride;
-  const int dim = FULL ? DB * 64 : a.head_dim, groups = dim / 32, row_bytes = INT4 ? dim / 2 : dim * 2;
-  const int step = 16 * kAttendWarps;
-  int slot0 = first + warp * 16;
-  // this lane's first addresses of the tile to load next
-  const char* kp = static_cast<const char*>(a.keys) + (row0 + slot0 + g) * row_bytes + t * (INT4 ? 8 : 16);
-  const char* vp = static_cast<const char*>(a.values) + (row0 + slot0 + 2 * t) * row_bytes + g * (INT4 ? 4 : 16);
-  const unsigned* ksp = a.key_scales + (row0 + slot0 + g) * groups;
-  const unsigned* vsp = a.value_scales + (row0 + slot0 + g) * groups;
-
-  // one tile in registers: loaded a step ahead of its use
-  constexpr int KW = INT4 ? DB * 2 : J * 4, VW = INT4 ? DB : DB * 4;
-  unsigned kf[2][KW], vf[4][VW], ks[2][INT4 ? J : 1], vs[2][INT4 ? J : 1];
-
-  auto load_scales = [&](unsigned(&f)[2][INT4 ? J : 1], const unsigned* sp, int at, bool whole) {
+  for (; slot0 < last; slot0 += kStep) {
+    // S^T: slots g (c0, c1) and g + 8 (c2, c3) of each tile, heads 8 n + 2 t, + 1
+    float s[TS][NT][4] = {};
 #pragma unroll
-    for (int r = 0; r < 2; ++r) {
-      const bool in = whole || at + g + 8 * r < last;
-      const unsigned* p = sp + 8 * r * groups;
-      if constexpr (FULL && J % 4 == 0) {
+    for (int u = 0; u < TS; ++u)
 #pragma unroll
-        for (int j = 0; j < J; j += 4) {
-          const uint4 u = in ? ld_row16(p + j) : make_uint4(0, 0, 0, 0);
-          f[r][j] = u.x; f[r][j + 1] = u.y; f[r][j + 2] = u.z; f[r][j + 3] = u.w;
-        }
-      } else if constexpr (FULL) {
-        const uint2 u = in ? ld_row8(p) : make_uint2(0, 0);
-        f[r][0] = u.x; f[r][1] = u.y;
-      } else {
-#pragma unroll
-        for (int j = 0; j < J; ++j) f[r][j] = in && j < groups ? ld_row4(p + j) : 0u;
-      }
-    }
-  };
-  // Slots past `last` load nothing and count as zeros, so that no value there matters; `whole`: the tile has none.
-  auto load_k = [&](int at, bool whole) {
-#pragma unroll
-    for (int r = 0; r < 2; ++r) {
-      const bool in = whole || at + g + 8 * r < last;
-      const char* p = kp + 8 * r * row_bytes;
-      if constexpr (INT4) {
-#pragma unroll
-        for (int i = 0; i < DB; ++i) {  // 16 columns: 64 i + 16 t
-          const uint2 u = in && (FULL || i * 64 + t * 16 < dim) ? ld_row8(p + i * 32) : make_uint2(0, 0);
-          kf[r][2 * i] = u.x; kf[r][2 * i + 1] = u.y;
-        }
-      } else {
-#pragma unroll
-        for (int j = 0; j < J; ++j) {
-          const uint4 u = in && (FULL || j * 32 + t * 8 < dim) ? ld_row16(p + j * 64) : make_uint4(0, 0, 0, 0);
-          kf[r][4 * j] = u.x; kf[r][4 * j + 1] = u.y; kf[r][4 * j + 2] = u.z; kf[r][4 * j + 3] = u.w;
-        }
-      }
-    }
-    if constexpr (INT4) load_scales(ks, ksp, at, whole);
-  };
-  auto load_v = [&](int at, bool whole) {
-#pragma unroll
-    for (int r = 0; r < 4; ++r) {
-      const int ahead = (r & 1) + 8 * (r >> 1);
-      const bool in = whole || at + 2 * t + ahead < last;
-      const char* p = vp + ahead * row_bytes;
-#pragma unroll
-      for (int i = 0; i < DB; ++i) {
-        const bool on = in && (FULL || i * 64 + g * 8 < dim);
+      for (int j = 0; j < J; ++j) {
+        unsigned c[2][4];
         if constexpr (INT4) {
-          vf[r][i] = on ? ld_row4(p + i * 32) : 0u;
+#pragma unroll
+          for (int r = 0; r < 2; ++r) {
+            unsigned scale, lowest;
+            const unsigned pair = ks[u][r][j / 4];
+            group_operands<T>(pair, pair, scale, lowest);
+#pragma unroll
+            for (int x = 0; x < 4; ++x) c[r][x] = decode_pair<T>(kf[u][r][j], x, scale, lowest);
+          }
         } else {
-          const uint4 u = on ? ld_row16(p + i * 128) : make_uint4(0, 0, 0, 0);
-          vf[r][4 * i] = u.x; vf[r][4 * i + 1] = u.y; vf[r][4 * i + 2] = u.z; vf[r][4 * i + 3] = u.w;
-        }
-      }
-    }
-    if constexpr (INT4) load_scales(vs, vsp, at, whole);
-  };
-  auto fetch_k = [&](int at) {
-    if (at + 16 <= last) load_k(at, true);
-    else load_k(at, false);
-    kp += (long long)step * row_bytes;
-    if (INT4) ksp += step * groups;
-  };
-  auto fetch_v = [&](int at) {
-    if (at + 16 <= last) load_v(at, true);
-    else load_v(at, false);
-    vp += (long long)step * row_bytes;
-    if (INT4) vsp += step * groups;
-  };
-
-  if (slot0 < last) {
-    fetch_k(slot0);
-    fetch_v(slot0);
-  }
-  for (; slot0 < last; slot0 += step) {
-    // S^T: slots g (c0, c1) and g + 8 (c2, c3), heads 8 n + 2 t, + 1
-    float s[NT][4];
-    if constexpr (INT4) {
-#pragma unroll
-      for (int n = 0; n < NT; ++n) s[n][0] = s[n][1] = s[n][2] = s[n][3] = 0.f;
-#pragma unroll
-      for (int i = 0; i < DB; ++i) {
-        // lanes t = 0, 1 hold 16 columns of group 2 i, lanes 2, 3 of group 2 i + 1: swap one word, so that every
-        // lane has 8 columns of each; the group's 4 words come in the order of lanes 0, 2, 1, 3
-        unsigned w[2][2];
-#pragma unroll
-        for (int r = 0; r < 2; ++r) {
-          const unsigned give = t < 2 ? kf[r][2 * i + 1] : kf[r][2 * i], keep = t < 2 ? kf[r][2 * i] : kf[r][2 * i + 1];
-          const unsigned got = __shfl_xor_sync(0xffffffffu, give, 2);
-          w[r][0] = t < 2 ? keep : got;
-          w[r][1] = t < 2 ? got : keep;
-        }
-#pragma unroll
-        for (int e = 0; e < 2; ++e) {
-          const int j = 2 * i + e;
-          unsigned c[2][4];
 #pragma unroll
           for (int r = 0; r < 2; ++r)
 #pragma unroll
-            for (int x = 0; x < 4; ++x) c[r][x] = code_pair<T>(w[r][e], x);
-          const float s0 = group_scale(ks[0][j]), l0 = group_lowest(ks[0][j]);
-          const float s1 = group_scale(ks[1][j]), l1 = group_lowest(ks[1][j]);
+            for (int x = 0; x < 4; ++x) c[r][x] = kf[u][r][4 * j + x];
+        }
 #pragma unroll
-          for (int n = 0; n < NT; ++n) {
-            float acc[4] = {0.f, 0.f, 0.f, 0.f};
-            mma<T>(acc, c[0][0], c[1][0], c[0][1], c[1][1], qf[n][j][0], qf[n][j][1]);
-            mma<T>(acc, c[0][2], c[1][2], c[0][3], c[1][3], qf[n][j][2], qf[n][j][3]);
-            s[n][0] = fmaf(acc[0], s0, fmaf(l0, qsum[n][j][0], s[n][0]));
-            s[n][1] = fmaf(acc[1], s0, fmaf(l0, qsum[n][j][1], s[n][1]));
-            s[n][2] = fmaf(acc[2], s1, fmaf(l1, qsum[n][j][0], s[n][2]));
-            s[n][3] = fmaf(acc[3], s1, fmaf(l1, qsum[n][j][1], s[n][3]));
-          }
+        for (int n = 0; n < NT; ++n) {
+          mma<T>(s[u][n], c[0][0], c[1][0], c[0][1], c[1][1], qf[n][j][0], qf[n][j][1]);
+          mma<T>(s[u][n], c[0][2], c[1][2], c[0][3], c[1][3], qf[n][j][2], qf[n][j][3]);
         }
       }
-    } else {
-#pragma unroll
-      for (int n = 0; n < NT; ++n) {
-        s[n][0] = s[n][1] = s[n][2] = s[n][3] = 0.f;
-#pragma unroll
-        for (int j = 0; j < J; ++j) {
-          mma<T>(s[n], kf[0][4 * j], kf[1][4 * j], kf[0][4 * j + 1], kf[1][4 * j + 1], qf[n][j][0], qf[n][j][1]);
-          mma<T>(s[n], kf[0][4 * j + 2], kf[1][4 * j + 2], kf[0][4 * j + 3], kf[1][4 * j + 3], qf[n][j][2], qf[n][j][3]);
-        }
-      }
-    }
-    const int next = slot0 + step;
+    const int next = slot0 + kStep;
     if (next < last) fetch_k(next);
 
-    const bool in0 = slot0 + g < last, in1 = slot0 + g + 8 < last;
-    unsigned pf[NT][INT4 ? J : 1][2];
+    unsigned pf[TS][NT][2];
 #pragma unroll
     for (int n = 0; n < NT; ++n) {
-      float p[4], top[2];
+      float p[TS][2][X], top[X];
 #pragma unroll
-      for (int x = 0; x < 4; ++x) p[x] = (x < 2 ? in0 : in1) ? s[n][x] * a.scale2 : -INFINITY;
+      for (int x = 0; x < X; ++x) {
+        top[x] = -INFINITY;
 #pragma unroll
-      for (int x = 0; x < 2; ++x) {
-        top[x] = fmaxf(p[x], p[2 + x]);
+        for (int u = 0; u < TS; ++u)
+#pragma unroll
+          for (int r = 0; r < 2; ++r) {
+            p[u][r][x] = slot0 + g + 16 * u + 8 * r < last ? s[u][n][2 * r + x] * a.scale2 : -INFINITY;
+            top[x] = fmaxf(top[x], p[u][r][x]);
+          }
 #pragma unroll
         for (int d = 4; d < 32; d *= 2) top[x] = fmaxf(top[x], __shfl_xor_sync(0xffffffffu, top[x], d));
       }
-      if (__any_sync(0xffffffffu, top[0] > m[n][0] || top[1] > m[n][1])) {
+      if (__any_sync(0xffffffffu, top[0] > m[n][0] || top[X - 1] > m[n][X - 1])) {
 #pragma unroll
-        for (int x = 0; x < 2; ++x) {
+        for (int x = 0; x < X; ++x) {
           top[x] = fmaxf(top[x], m[n][x]);
           const float keep = top[x] == -INFINITY ? 1.f : exp2_fast(m[n][x] - top[x]);
           m[n][x] = top[x];
@@ -374,71 +359,53 @@ __global__ void __launch_bounds__(kAttendThreads) k_attend_mma(const AttendArgs 
               o[n][i][w][x] *= keep;
               o[n][i][w][2 + x] *= keep;
             }
-          if (INT4)
-#pragma unroll
-            for (int j = 0; j < J; ++j) olow[n][j][x] *= keep;
         }
       }
 #pragma unroll
-      for (int x = 0; x < 4; ++x) {
-        const float ref = m[n][x & 1] == -INFINITY ? 0.f : m[n][x & 1] - kLift;
-        p[x] = exp2_fast(p[x] - ref);
-        l[n][x & 1] += p[x];
-      }
-      if constexpr (INT4) {
+      for (int u = 0; u < TS; ++u)
 #pragma unroll
-        for (int j = 0; j < J; ++j) {
-          const float s0 = group_scale(vs[0][j]), l0 = group_lowest(vs[0][j]);
-          const float s1 = group_scale(vs[1][j]), l1 = group_lowest(vs[1][j]);
-          olow[n][j][0] = fmaf(p[0], l0, fmaf(p[2], l1, olow[n][j][0]));
-          olow[n][j][1] = fmaf(p[1], l0, fmaf(p[3], l1, olow[n][j][1]));
-          pf[n][j][0] = transpose8x8(pack2((PT*)nullptr, p[0] * s0, p[1] * s0));
-          pf[n][j][1] = transpose8x8(pack2((PT*)nullptr, p[2] * s1, p[3] * s1));
+        for (int r = 0; r < 2; ++r) {
+#pragma unroll
+          for (int x = 0; x < X; ++x) {
+            const float ref = m[n][x] == -INFINITY ? 0.f : m[n][x] - kLift;
+            p[u][r][x] = exp2_fast(p[u][r][x] - ref);
+            l[n][x] += p[u][r][x];
+          }
+          pf[u][n][r] = transpose8x8(pack2((PT*)nullptr, p[u][r][0], ONE ? 0.f : p[u][r][X - 1]));
         }
-      } else {
-        pf[n][0][0] = transpose8x8(pack2((PT*)nullptr, p[0], p[1]));
-        pf[n][0][1] = transpose8x8(pack2((PT*)nullptr, p[2], p[3]));
-      }
     }
 
     // O^T += V^T P^T
 #pragma unroll
-    for (int i = 0; i < DB; ++i) {
+    for (int u = 0; u < TS; ++u) {
+      unsigned scale[2], lowest[2];
       if constexpr (INT4) {
-        // lanes g < 4 hold 8 columns of group 2 i, g >= 4 of group 2 i + 1: swap halves with lane g ^ 4, so that
-        // every lane has 4 columns of each (low half: group 2 i)
-        unsigned w[4];
+        group_operands<PT>(vs[u][0], vs[u][1], scale[0], lowest[0]);
+        group_operands<PT>(vs[u][2], vs[u][3], scale[1], lowest[1]);
+      }
 #pragma unroll
-        for (int r = 0; r < 4; ++r) {
-          const unsigned got = __shfl_xor_sync(0xffffffffu, vf[r][i], 16);
-          w[r] = __byte_perm(vf[r][i], got, g < 4 ? 0x5410 : 0x3276);
-        }
-#pragma unroll
-        for (int e = 0; e < 2; ++e) {
-          // slots (2 t, 2 t + 1) and (2 t + 8, 2 t + 9) side by side: nibble c of both halves is column c's pair
-          const unsigned x0 = __byte_perm(w[0], w[1], e ? 0x7632 : 0x5410);
-          const unsigned x1 = __byte_perm(w[2], w[3], e ? 0x7632 : 0x5410);
-          unsigned c0[4], c1[4];
-#pragma unroll
-          for (int c = 0; c < 4; ++c) c0[c] = code_pair<PT>(x0, c), c1[c] = code_pair<PT>(x1, c);
-#pragma unroll
-          for (int n = 0; n < NT; ++n)
-#pragma unroll
-            for (int c = 0; c < 2; ++c)
-              mma<PT>(o[n][i][2 * e + c], c0[2 * c], c0[2 * c + 1], c1[2 * c], c1[2 * c + 1], pf[n][2 * i + e][0],
-                      pf[n][2 * i + e][1]);
-        }
-      } else {
+      for (int i = 0; i < DB; ++i)
 #pragma unroll
         for (int w = 0; w < 4; ++w) {
-          const unsigned a0 = __byte_perm(vf[0][4 * i + w], vf[1][4 * i + w], 0x5410);
-          const unsigned a1 = __byte_perm(vf[0][4 * i + w], vf[1][4 * i + w], 0x7632);
-          const unsigned a2 = __byte_perm(vf[2][4 * i + w], vf[3][4 * i + w], 0x5410);
-          const unsigned a3 = __byte_perm(vf[2][4 * i + w], vf[3][4 * i + w], 0x7632);
+          unsigned c[4];
+          if constexpr (INT4) {
+            // slots (2 t, 2 t + 1) and (2 t + 8, 2 t + 9) side by side: a nibble of both halves is one column's pair
 #pragma unroll
-          for (int n = 0; n < NT; ++n) mma<PT>(o[n][i][w], a0, a1, a2, a3, pf[n][0][0], pf[n][0][1]);
+            for (int r = 0; r < 2; ++r) {
+              const unsigned y = __byte_perm(vf[u][2 * r][i], vf[u][2 * r + 1][i], w < 2 ? 0x5410 : 0x7632);
+              c[2 * r] = decode_pair<PT>(y, 2 * (w & 1), scale[r], lowest[r]);
+              c[2 * r + 1] = decode_pair<PT>(y, 2 * (w & 1) + 1, scale[r], lowest[r]);
+            }
+          } else {
+#pragma unroll
+            for (int r = 0; r < 2; ++r) {
+              c[2 * r] = __byte_perm(vf[u][2 * r][4 * i + w], vf[u][2 * r + 1][4 * i + w], 0x5410);
+              c[2 * r + 1] = __byte_perm(vf[u][2 * r][4 * i + w], vf[u][2 * r + 1][4 * i + w], 0x7632);
+            }
+          }
+#pragma unroll
+          for (int n = 0; n < NT; ++n) mma<PT>(o[n][i][w], c[0], c[1], c[2], c[3], pf[u][n][0], pf[u][n][1]);
         }
-      }
     }
     if (next < last) fetch_v(next);
   }
@@ -447,38 +414,26 @@ __global__ void __launch_bounds__(kAttendThreads) k_attend_mma(const AttendArgs 
 #pragma unroll
   for (int n = 0; n < NT; ++n)
 #pragma unroll
-    for (int x = 0; x < 2; ++x) {
+    for (int x = 0; x < X; ++x) {
       const int h = n * 8 + 2 * t + x;
       float sum = l[n][x];
 #pragma unroll
       for (int d = 4; d < 32; d *= 2) sum += __shfl_xor_sync(0xffffffffu, sum, d);
+      if (h >= nheads) continue;
       if (g == 0) {
         sh_m[warp][h] = m[n][x];
         sh_l[warp][h] = sum;
       }
-      if (INT4)
 #pragma unroll
-        for (int j = 0; j < J; ++j)
+      for (int i = 0; i < DB; ++i) {
+        float* to = &sh_o[warp][h][INT4 ? g * 8 * DB + 8 * i : i * 64 + g * 8];
 #pragma unroll
-          for (int d = 4; d < 32; d *= 2) olow[n][j][x] += __shfl_xor_sync(0xffffffffu, olow[n][j][x], d);
-#pragma unroll
-      for (int i = 0; i < DB; ++i)
-#pragma unroll
-        for (int w = 0; w < 4; ++w)
-#pragma unroll
-          for (int r = 0; r < 2; ++r) {
-            if (INT4) {
-              // m-tile w: group 2 i + w / 2; this lane's 4 columns of it are 8 (g % 4) + (g < 4 ? 0 : 4)
-              const int c = i * 64 + (w / 2) * 32 + (g & 3) * 8 + (g < 4 ? 0 : 4) + (w & 1) * 2 + r;
-              sh_o[warp][h][c] = o[n][i][w][2 * r + x] + olow[n][2 * i + w / 2][x];
-            } else {
-              sh_o[warp][h][i * 64 + g * 8 + w * 2 + r] = o[n][i][w][2 * r + x];
-            }
-          }
+        for (int w = 0; w < 4; ++w) *reinterpret_cast<float2*>(to + 2 * w) = make_float2(o[n][i][w][x], o[n][i][w][2 + x]);
+      }
     }
   __syncthreads();
-  for (int e = threadIdx.x; e < nheads * a.head_dim; e += kAttendThreads) {
-    const int h = e / a.head_dim, d = e - h * a.head_dim;
+  for (int e = threadIdx.x; e < nheads * dim; e += kAttendThreads) {
+    const int h = e / dim, d = e - h * dim;
     float top = -INFINITY, sum = 0.f, out = 0.f;
 #pragma unroll
     for (int w = 0; w < kAttendWarps; ++w) top = fmaxf(top, sh_m[w][h]);
@@ -638,22 +593,20 @@ int splits_of(const st_cache* c, int heads) {
   return n < 1 ? 1 : n > 1024 ? 1024 : (int)n;
 }
 
-template <typename T, bool INT4, bool FULL>
+template <typename T, int DB, bool INT4, bool FULL>
 void launch_mma(const AttendArgs& a, int per, dim3 grid, cudaStream_t s) {
-  if (a.head_dim <= 64) {
-    if (per == 8) k_attend_mma<T, 1, 1, INT4, FULL><<<grid, kAttendThreads, 0, s>>>(a);
-    else k_attend_mma<T, 1, 2, INT4, FULL><<<grid, kAttendThreads, 0, s>>>(a);
-  } else if (a.head_dim <= 128) {
-    if (per == 8) k_attend_mma<T, 2, 1, INT4, FULL><<<grid, kAttendThreads, 0, s>>>(a);
-    else k_attend_mma<T, 2, 2, INT4, FULL><<<grid, kAttendThreads, 0, s>>>(a);
-  } else {
-    k_attend_mma<T, 4, 1, INT4, FULL><<<grid, kAttendThreads, 0, s>>>(a);
-  }
+  if (a.group == 1) k_attend_mma<T, DB, 1, INT4, FULL, true><<<grid, kAttendThreads, 0, s>>>(a);
+  else if (per == 8) k_attend_mma<T, DB, 1, INT4, FULL, false><<<grid, kAttendThreads, 0, s>>>(a);
+  else if constexpr (DB < 4) k_attend_mma<T, DB, 2, INT4, FULL, false><<<grid, kAttendThreads, 0, s>>>(a);
 }
 template <typename T, bool INT4>
 void launch_mma(const AttendArgs& a, int per, dim3 grid, cudaStream_t s) {
-  if (a.head_dim == 64 || a.head_dim == 128 || a.head_dim == 256) launch_mma<T, INT4, true>(a, per, grid, s);
-  else launch_mma<T, INT4, false>(a, per, grid, s);
+  if (a.head_dim == 64) launch_mma<T, 1, INT4, true>(a, per, grid, s);
+  else if (a.head_dim < 64) launch_mma<T, 1, INT4, false>(a, per, grid, s);
+  else if (a.head_dim == 128) launch_mma<T, 2, INT4, true>(a, per, grid, s);
+  else if (a.head_dim < 128) launch_mma<T, 2, INT4, false>(a, per, grid, s);
+  else if (a.head_dim == 256) launch_mma<T, 4, INT4, true>(a, per, grid, s);
+  else launch_mma<T, 4, INT4, false>(a, per, grid, s);
 }
 
 template <int LANES>
