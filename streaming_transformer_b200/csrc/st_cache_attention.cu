@@ -44,6 +44,7 @@
 // knows; the number of splits follows the cache's size.
 #include "st_cache.cuh"
 #include "st_cache_host.h"
+#include <cstdlib>
 
 namespace st {
 namespace {
@@ -537,40 +538,59 @@ __global__ void __launch_bounds__(kAttendThreads) k_attend_fp32(const AttendArgs
 }
 
 // ---------------------------------------------------------------- parts of several CTAs
+// One CTA joins one head of one stream: 8 warps take every eighth part, 4
+// columns a lane, and meet in shared memory in warp order.
+constexpr int kMergeWarps = 8;
+constexpr int kMaxSplits = 1024;
+
 template <typename T>
-__global__ void __launch_bounds__(kAttendThreads) k_merge(const AttendArgs a) {
-  __shared__ float sh_f[kAttendThreads];
-  const int h = blockIdx.x, stream = blockIdx.y;
+__global__ void __launch_bounds__(32 * kMergeWarps) k_merge(const AttendArgs a) {
+  __shared__ float sh_f[kMaxSplits], sh_w[2][kMergeWarps];
+  __shared__ float4 sh_o[kMergeWarps][ST_CACHE_MAX_HEAD_DIM / 4];
+  const int h = blockIdx.x, stream = blockIdx.y, warp = threadIdx.x >> 5, lane = threadIdx.x & 31;
   const int seen = slots_seen(a.positions[stream], a.slots);
   const long long at = ((long long)stream * a.heads + h) * a.splits;
   const float2* ml = reinterpret_cast<const float2*>(a.parts) + at;
-  const float* part = a.parts + (long long)a.streams * a.heads * a.splits * 2 + at * a.head_dim;
+  const float4* part = reinterpret_cast<const float4*>(a.parts + (long long)a.streams * a.heads * a.splits * 2 + at * a.head_dim);
+  const int quads = a.head_dim / 4;
   wait_for_previous_kernel();
-  float top = -INFINITY;
-  for (int s = 0; s < a.splits; ++s) top = fmaxf(top, ml[s].x);
-  float sum = 0.f, o[2] = {};
-  for (int base = 0; base < a.splits; base += kAttendThreads) {
-    const int n = min(kAttendThreads, a.splits - base);
-    __syncthreads();
-    if ((int)threadIdx.x < n) {
-      const float m = ml[base + threadIdx.x].x;
-      sh_f[threadIdx.x] = m == -INFINITY ? 1.f : exp2_fast(m - top);
-    }
-    __syncthreads();
-    for (int s = 0; s < n; ++s) {
-      sum = fmaf(ml[base + s].y, sh_f[s], sum);
+  float top = -INFINITY, sum = 0.f;
+  for (int s = threadIdx.x; s < a.splits; s += 32 * kMergeWarps) top = fmaxf(top, ml[s].x);
 #pragma unroll
-      for (int r = 0; r < 2; ++r) {
-        const int d = threadIdx.x + r * kAttendThreads;
-        if (d < a.head_dim) o[r] = fmaf(part[(long long)(base + s) * a.head_dim + d], sh_f[s], o[r]);
-      }
-    }
+  for (int d = 1; d < 32; d *= 2) top = fmaxf(top, __shfl_xor_sync(0xffffffffu, top, d));
+  if (lane == 0) sh_w[0][warp] = top;
+  __syncthreads();
+#pragma unroll
+  for (int w = 0; w < kMergeWarps; ++w) top = fmaxf(top, sh_w[0][w]);
+  for (int s = threadIdx.x; s < a.splits; s += 32 * kMergeWarps) {
+    const float2 p = ml[s];
+    const float f = p.x == -INFINITY ? 1.f : exp2_fast(p.x - top);  // an empty part is all zeros, or NaN
+    sh_f[s] = f;
+    sum = fmaf(p.y, f, sum);
   }
 #pragma unroll
-  for (int r = 0; r < 2; ++r) {
-    const int d = threadIdx.x + r * kAttendThreads;
-    if (d < a.head_dim)
-      static_cast<T*>(a.out)[stream * a.o_row + h * a.o_head + d] = static_cast<T>(seen ? o[r] / sum : 0.f);
+  for (int d = 1; d < 32; d *= 2) sum += __shfl_xor_sync(0xffffffffu, sum, d);
+  if (lane == 0) sh_w[1][warp] = sum;
+  __syncthreads();
+  for (int c = lane; c < quads; c += 32) {
+    float4 o = make_float4(0.f, 0.f, 0.f, 0.f);
+#pragma unroll 4
+    for (int s = warp; s < a.splits; s += kMergeWarps) {
+      const float4 v = __ldcg(part + (long long)s * quads + c);
+      const float f = sh_f[s];
+      o.x = fmaf(v.x, f, o.x); o.y = fmaf(v.y, f, o.y); o.z = fmaf(v.z, f, o.z); o.w = fmaf(v.w, f, o.w);
+    }
+    sh_o[warp][c] = o;
+  }
+  __syncthreads();
+  for (int d = threadIdx.x; d < a.head_dim; d += 32 * kMergeWarps) {
+    float l = 0.f, o = 0.f;
+#pragma unroll
+    for (int w = 0; w < kMergeWarps; ++w) {
+      l += sh_w[1][w];
+      o += reinterpret_cast<const float*>(sh_o[w])[d];
+    }
+    static_cast<T*>(a.out)[stream * a.o_row + h * a.o_head + d] = static_cast<T>(seen ? o / l : 0.f);
   }
 }
 
@@ -587,10 +607,12 @@ int splits_of(const st_cache* c, int heads) {
   const int per = heads_per_block(c, heads), group = heads / c->heads;
   const long long ctas = (long long)c->streams * c->heads * ((group + per - 1) / per);
   const int slots = c->sinks + c->window;
-  const long long want = (8ll * sm_count(c->device) + ctas - 1) / ctas;  // 4 resident CTAs an SM, twice over
-  const long long most = (slots + 255) / 256;                             // at least 256 slots each
+  static const int per_sm = getenv("X_PER") ? atoi(getenv("X_PER")) : 6;
+  static const int least = getenv("X_LEAST") ? atoi(getenv("X_LEAST")) : 256;
+  const long long want = ((long long)per_sm * sm_count(c->device) + ctas / 2) / ctas;
+  const long long most = (slots + least - 1) / least;
   const long long n = want < most ? want : most;
-  return n < 1 ? 1 : n > 1024 ? 1024 : (int)n;
+  return n < 1 ? 1 : n > kMaxSplits ? kMaxSplits : (int)n;
 }
 
 template <typename T, int DB, bool INT4, bool FULL>
@@ -620,7 +642,7 @@ template <typename T>
 cudaError_t launch_merge(const AttendArgs& a, cudaStream_t s) {
   cudaLaunchConfig_t cfg{};
   cfg.gridDim = dim3(a.heads, a.streams);
-  cfg.blockDim = dim3(kAttendThreads);
+  cfg.blockDim = dim3(32 * kMergeWarps);
   cfg.stream = s;
   cudaLaunchAttribute attr{};
   attr.id = cudaLaunchAttributeProgrammaticStreamSerialization;  // its launch overlaps the parts' kernel
