@@ -44,7 +44,8 @@
 // knows; the number of splits follows the cache's size.
 #include "st_cache.cuh"
 #include "st_cache_host.h"
-#include <cstdlib>
+
+#include <algorithm>
 
 namespace st {
 namespace {
@@ -159,7 +160,7 @@ __device__ __forceinline__ unsigned decode_pair(unsigned w, int i, unsigned scal
 // query head a key head, so that the odd columns of S^T are not computed on.
 // A step takes TS tiles of 16 slots.
 template <typename T, int DB, int NT, bool INT4, bool FULL, bool ONE>
-__global__ void __launch_bounds__(kAttendThreads) k_attend_mma(const AttendArgs a) {
+__global__ void __launch_bounds__(kAttendThreads, DB * NT == 1 ? 6 : 1) k_attend_mma(const AttendArgs a) {
   constexpr int J = 2 * DB;   // 16-bit: 16-byte pieces of a key row a lane holds
   constexpr int TS = INT4 && DB * NT <= 2 ? 2 : 1;
   constexpr int X = ONE ? 1 : 2;  // query heads a lane has of each block: 8 n + 2 t + x
@@ -602,17 +603,15 @@ int heads_per_block(const st_cache* c, int heads) {
   return group <= 8 || c->head_dim > 128 ? 8 : 16;
 }
 
-// CTAs that share the slots of one key head.
+// CTAs that share the slots of one key head: one for each SM while each still
+// has 64 slots (a tile a warp), and up to 12 for each SM while each has 512, so
+// that streams of uneven lengths even out. Measured (us): see the launch below.
 int splits_of(const st_cache* c, int heads) {
-  const int per = heads_per_block(c, heads), group = heads / c->heads;
-  const long long ctas = (long long)c->streams * c->heads * ((group + per - 1) / per);
-  const int slots = c->sinks + c->window;
-  static const int per_sm = getenv("X_PER") ? atoi(getenv("X_PER")) : 6;
-  static const int least = getenv("X_LEAST") ? atoi(getenv("X_LEAST")) : 256;
-  const long long want = ((long long)per_sm * sm_count(c->device) + ctas / 2) / ctas;
-  const long long most = (slots + least - 1) / least;
-  const long long n = want < most ? want : most;
-  return n < 1 ? 1 : n > kMaxSplits ? kMaxSplits : (int)n;
+  const int per = heads_per_block(c, heads), group = heads / c->heads, slots = c->sinks + c->window;
+  const long long ctas = (long long)c->streams * c->heads * ((group + per - 1) / per), sms = sm_count(c->device);
+  const long long fill = std::min<long long>(sms / ctas, slots / 64);
+  const long long even = std::min<long long>(12 * sms / ctas, slots / 512);
+  return (int)std::min<long long>(std::max<long long>({fill, even, 1}), kMaxSplits);
 }
 
 template <typename T, int DB, bool INT4, bool FULL>
