@@ -1,11 +1,37 @@
 // st_window.cu -- causal attention of packed sequences with a sliding window
 // and sinks (st_window_attention).
 //
-// A group of lanes takes one query row of one head and walks the keys it sees:
-// the sinks before the window, then the window. One pass, with a running
-// maximum and sum in fp32.
-#include "st_cache.cuh"
+// Two kernels. k_window_tiles: 16-bit rows of up to 128 columns, on tcgen05.
+// k_window_rows: a few lanes walk the keys that one query row of one head sees,
+// in fp32; it serves fp32 rows (there is no fp32 tensor product), wider rows,
+// and scales that are not positive.
+//
+// k_window_tiles. A CTA takes 128 consecutive rows of the packed input, one TMEM
+// lane each, and one head. Rows may belong to several sequences: the keys that
+// the tile needs are those from its first row's window on, which covers every
+// sequence that begins inside the tile, and the sinks of the first row's
+// sequence. They are walked in blocks of 32 rows (sinks first, then the window
+// from exactly its first key), several blocks to a key tile:
+//   S = Q K^T          one MMA per 16 columns, both operands in shared memory, S in TMEM
+//   P = 2^(c S - m)    one thread a row; m, and the sum l, in fp32
+//   O += P V           P from TMEM (written over S), V as it lies in memory (N contiguous)
+// O is rescaled only when a row's maximum has grown by more than 2^8 since the
+// last time; P then stays below 2^8, which both 16-bit types hold, and l and O
+// share the reference, so the quotient is exact.
+//
+// Only tiles at an edge of somebody's window are masked. A masked weight is 0,
+// but 0 times an infinite or NaN value is not: in masked tiles the rows of V are
+// looked at, and if any is not finite (only then) the CTA does its rows again
+// with the row kernel's code, which never reads what a row does not see.
+//
+// Every wait has a time limit; a CTA that ran into one writes NaN.
+#include <cuda.h>
+
+#include <atomic>
+
 #include "st_cache_host.h"
+#include "st_umma.cuh"
+#include "st_cache.cuh"
 
 namespace st {
 namespace {
@@ -34,14 +60,10 @@ __device__ int sequence_start(const WindowArgs& a, int row) {
   return first <= row ? first : -1;
 }
 
+// One query row of one head by a group of LANES lanes (`mask`: those lanes of the warp).
 template <typename T, int LANES>
-__global__ void __launch_bounds__(kWindowThreads) k_window_rows(const WindowArgs a) {
-  const int lane = threadIdx.x % LANES, h = blockIdx.y, kv = h / (a.heads / a.kv_heads);
-  const unsigned mask = LANES == 32 ? 0xffffffffu : ((1u << LANES) - 1u) << ((threadIdx.x & 31) / LANES * LANES);
-  const long long row = (long long)blockIdx.x * (kWindowThreads / LANES) + threadIdx.x / LANES;
-  if (row >= a.rows) return;
-  const int start = sequence_start(a, (int)row);
-  if (start < 0) return;
+__device__ __forceinline__ void window_row(const WindowArgs& a, int row, int start, int h, int lane, unsigned mask) {
+  const int kv = h / (a.heads / a.kv_heads);
   const bool on = lane * 8 < a.head_dim;
   float q[8] = {}, acc[8] = {}, m = -INFINITY, l = 0.f;
   if (on) load8(static_cast<const T*>(a.q) + row * a.q_row + h * a.q_head + lane * 8, q);
@@ -49,7 +71,8 @@ __global__ void __launch_bounds__(kWindowThreads) k_window_rows(const WindowArgs
   for (int i = 0; i < 8; ++i) q[i] *= a.scale;
   const T* kp = static_cast<const T*>(a.k) + kv * a.k_head + lane * 8;
   const T* vp = static_cast<const T*>(a.v) + kv * a.v_head + lane * 8;
-  const int low = (int)max((long long)start, row - a.window + 1);  // first row of the window
+  const int low = (int)max((long long)start, (long long)row - a.window + 1);  // first row of the window
+  const long long sinks = (long long)start + a.sinks;                         // first row behind the sinks
   int j = start < low && a.sinks > 0 ? start : low;
   while (j <= row) {
     float k[8] = {}, v[8] = {}, dot = 0.f;
@@ -68,12 +91,379 @@ __global__ void __launch_bounds__(kWindowThreads) k_window_rows(const WindowArgs
 #pragma unroll
     for (int i = 0; i < 8; ++i) acc[i] = fmaf(acc[i], keep, p * v[i]);
     ++j;
-    if (j < low && j - start >= a.sinks) j = low;
+    if (j < low && j >= sinks) j = low;
   }
-  const float inv = l > 0.f ? 1.f / l : NAN;
 #pragma unroll
-  for (int i = 0; i < 8; ++i) acc[i] *= inv;
+  for (int i = 0; i < 8; ++i) acc[i] /= l;
   if (on) store8(static_cast<T*>(a.out) + row * a.o_row + h * a.o_head + lane * 8, acc);
+}
+
+template <int LANES>
+__device__ __forceinline__ unsigned row_mask() {
+  return LANES == 32 ? 0xffffffffu : ((1u << LANES) - 1u) << ((threadIdx.x & 31) / LANES * LANES);
+}
+
+template <typename T, int LANES>
+__global__ void __launch_bounds__(kWindowThreads) k_window_rows(const WindowArgs a) {
+  const long long row = (long long)blockIdx.x * (kWindowThreads / LANES) + threadIdx.x / LANES;
+  if (row >= a.rows) return;
+  const int start = sequence_start(a, (int)row);
+  if (start < 0) return;
+  window_row<T, LANES>(a, (int)row, start, blockIdx.y, threadIdx.x % LANES, row_mask<LANES>());
+}
+
+// ---------------------------------------------------------------- tcgen05
+constexpr int kTileRows = 128;      // query rows of a CTA: TMEM lanes
+constexpr int kBlockRows = 32;      // key rows of one copy
+constexpr int kTileThreads = 192;   // 4 warps of rows, one that copies, one that issues products
+constexpr unsigned long long kWaitNs = 2000000000ull;
+
+// DP: columns, padded to 64 or 128 with zeros by the copies. Key tiles are DP rows: S takes DP TMEM columns beside
+// O's DP, so that 2 (DP 128) or 3 (DP 64) CTAs share an SM and one's products run under another's softmax.
+template <int DP>
+struct Tiles {
+  static constexpr int kKeys = DP, kBlocks = kKeys / kBlockRows, kPanels = DP / 64, kStages = DP == 64 ? 2 : 1;
+  static constexpr int kQBytes = kPanels * kTileRows * 128, kKvBytes = kPanels * kKeys * 128;
+  static constexpr int kSmem = kQBytes + 2 * kStages * kKvBytes + 1024;
+};
+
+struct TileMaps {
+  CUtensorMap q, k, v;
+};
+
+// Shared-memory matrix descriptors, 128-byte swizzle (layout type 2), version 1. K-major (Q, K): 8-row groups 1024
+// bytes apart. MN-major (V): the same groups along K, 64-column panels `panel` bytes apart.
+__device__ __forceinline__ unsigned long long swizzled_desc(const void* smem, unsigned panel) {
+  return (unsigned long long)((smem_addr(smem) & 0x3FFFFu) >> 4) | ((unsigned long long)(panel >> 4) << 16) |
+         ((unsigned long long)(1024 >> 4) << 32) | (1ull << 46) | (2ull << 61);
+}
+
+// Box at (column, head, row) of a row tensor.
+__device__ __forceinline__ void copy_box(void* dst, const CUtensorMap* map, int col, int head, int row,
+                                         unsigned long long* bar) {
+  asm volatile(
+      "cp.async.bulk.tensor.3d.shared::cta.global.tile.mbarrier::complete_tx::bytes [%0], [%1, {%2, %3, %4}], [%5];"
+      :: "r"(smem_addr(dst)), "l"(map), "r"(col), "r"(head), "r"(row), "r"(smem_addr(bar)) : "memory");
+}
+
+// A from TMEM, B by descriptor.
+__device__ __forceinline__ void umma_f16_ts(unsigned d, unsigned at, unsigned long long bdesc, unsigned idesc,
+                                            unsigned accumulate) {
+  asm volatile(
+      "{\n\t.reg .pred p;\n\t"
+      "setp.ne.b32 p, %4, 0;\n\t"
+      "tcgen05.mma.cta_group::1.kind::f16 [%0], [%1], %2, %3, p;\n\t}" ::"r"(d), "r"(at), "l"(bdesc), "r"(idesc),
+      "r"(accumulate)
+      : "memory");
+}
+
+// 32 lanes x 32 columns between registers and TMEM.
+__device__ __forceinline__ void tmem_ld32(unsigned addr, float (&v)[32]) {
+  unsigned r[32];
+  asm volatile(
+      "tcgen05.ld.sync.aligned.32x32b.x32.b32 "
+      "{%0,%1,%2,%3,%4,%5,%6,%7,%8,%9,%10,%11,%12,%13,%14,%15,%16,%17,%18,%19,%20,%21,%22,%23,%24,%25,%26,%27,%28,%29,"
+      "%30,%31}, [%32];"
+      : "=r"(r[0]), "=r"(r[1]), "=r"(r[2]), "=r"(r[3]), "=r"(r[4]), "=r"(r[5]), "=r"(r[6]), "=r"(r[7]), "=r"(r[8]),
+        "=r"(r[9]), "=r"(r[10]), "=r"(r[11]), "=r"(r[12]), "=r"(r[13]), "=r"(r[14]), "=r"(r[15]), "=r"(r[16]),
+        "=r"(r[17]), "=r"(r[18]), "=r"(r[19]), "=r"(r[20]), "=r"(r[21]), "=r"(r[22]), "=r"(r[23]), "=r"(r[24]),
+        "=r"(r[25]), "=r"(r[26]), "=r"(r[27]), "=r"(r[28]), "=r"(r[29]), "=r"(r[30]), "=r"(r[31])
+      : "r"(addr)
+      : "memory");
+  asm volatile("tcgen05.wait::ld.sync.aligned;" ::: "memory");
+#pragma unroll
+  for (int i = 0; i < 32; ++i) v[i] = __uint_as_float(r[i]);
+}
+__device__ __forceinline__ void tmem_st32(unsigned addr, const float (&v)[32]) {
+  unsigned r[32];
+#pragma unroll
+  for (int i = 0; i < 32; ++i) r[i] = __float_as_uint(v[i]);
+  asm volatile(
+      "tcgen05.st.sync.aligned.32x32b.x32.b32 [%32], "
+      "{%0,%1,%2,%3,%4,%5,%6,%7,%8,%9,%10,%11,%12,%13,%14,%15,%16,%17,%18,%19,%20,%21,%22,%23,%24,%25,%26,%27,%28,%29,"
+      "%30,%31};" ::"r"(r[0]), "r"(r[1]), "r"(r[2]), "r"(r[3]), "r"(r[4]), "r"(r[5]), "r"(r[6]), "r"(r[7]), "r"(r[8]),
+      "r"(r[9]), "r"(r[10]), "r"(r[11]), "r"(r[12]), "r"(r[13]), "r"(r[14]), "r"(r[15]), "r"(r[16]), "r"(r[17]),
+      "r"(r[18]), "r"(r[19]), "r"(r[20]), "r"(r[21]), "r"(r[22]), "r"(r[23]), "r"(r[24]), "r"(r[25]), "r"(r[26]),
+      "r"(r[27]), "r"(r[28]), "r"(r[29]), "r"(r[30]), "r"(r[31]), "r"(addr)
+      : "memory");
+}
+__device__ __forceinline__ void tmem_st16(unsigned addr, const unsigned (&r)[16]) {
+  asm volatile(
+      "tcgen05.st.sync.aligned.32x32b.x16.b32 [%16], {%0,%1,%2,%3,%4,%5,%6,%7,%8,%9,%10,%11,%12,%13,%14,%15};" ::"r"(r[0]),
+      "r"(r[1]), "r"(r[2]), "r"(r[3]), "r"(r[4]), "r"(r[5]), "r"(r[6]), "r"(r[7]), "r"(r[8]), "r"(r[9]), "r"(r[10]),
+      "r"(r[11]), "r"(r[12]), "r"(r[13]), "r"(r[14]), "r"(r[15]), "r"(addr)
+      : "memory");
+}
+__device__ __forceinline__ void tmem_st_wait() { asm volatile("tcgen05.wait::st.sync.aligned;" ::: "memory"); }
+
+__device__ __forceinline__ float exp2_fast(float x) {
+  float y;
+  asm("ex2.approx.ftz.f32 %0, %1;" : "=f"(y) : "f"(x));
+  return y;
+}
+
+// Bits lo .. hi of a 32-bit word (either end may lie outside it).
+__device__ __forceinline__ unsigned bit_range(int lo, int hi) {
+  lo = max(lo, 0);
+  hi = min(hi, 31);
+  return lo > hi ? 0u : (0xffffffffu >> (31 - hi)) & (0xffffffffu << lo);
+}
+
+// What a CTA's tile of rows needs: its rows inside sequences, and its key blocks.
+struct TileKeys {
+  int r0, r1;              // first and last row inside a sequence
+  int start;               // first row of r0's sequence
+  int sink_end;            // sinks walked apart: rows start .. sink_end - 1
+  int low;                 // first row of the window blocks
+  int sink_blocks, blocks;
+  __device__ int base(int block) const {  // first row of a block
+    return block < sink_blocks ? start + block * kBlockRows : low + (block - sink_blocks) * kBlockRows;
+  }
+};
+__device__ __forceinline__ bool tile_keys(const WindowArgs& a, int tile, TileKeys& t) {
+  t.r0 = tile * kTileRows;
+  t.r1 = (int)min((long long)a.rows, (long long)t.r0 + kTileRows) - 1;
+  if (a.starts) {
+    t.r0 = max(t.r0, clamp_row(a.starts[0], a.rows));
+    t.r1 = min(t.r1, clamp_row(a.starts[a.sequences], a.rows) - 1);
+  }
+  if (t.r0 > t.r1) return false;
+  t.start = sequence_start(a, t.r0);
+  if (t.start < 0) t.start = t.r0;  // only with starts that decrease
+  t.low = (int)max((long long)t.start, (long long)t.r0 - a.window + 1);
+  t.sink_end = (int)min((long long)t.low, (long long)t.start + a.sinks);
+  t.sink_blocks = (t.sink_end - t.start + kBlockRows - 1) / kBlockRows;
+  t.blocks = t.sink_blocks + (t.r1 - t.low + kBlockRows) / kBlockRows;
+  return true;
+}
+
+template <typename T, int DP>
+__global__ void __launch_bounds__(kTileThreads, DP == 64 ? 3 : 2)
+    k_window_tiles(const WindowArgs a, const __grid_constant__ TileMaps maps) {
+  using G = Tiles<DP>;
+  extern __shared__ unsigned char raw[];
+  __shared__ unsigned long long q_full, k_full[G::kStages], k_free[G::kStages], v_full[G::kStages], v_free[G::kStages],
+      s_full, p_full, o_full;
+  __shared__ unsigned tmem_base;
+  __shared__ int sh_slow, sh_dead;
+  const int warp = threadIdx.x >> 5;
+  const int h = blockIdx.x % a.heads, tile = gridDim.x / a.heads - 1 - blockIdx.x / a.heads;  // most keys first
+  TileKeys keys;
+  if (!tile_keys(a, tile, keys)) return;
+  unsigned char* smem = raw + ((1024u - (smem_addr(raw) & 1023u)) & 1023u);
+  unsigned char *sq = smem, *sk = sq + G::kQBytes, *sv = sk + G::kStages * G::kKvBytes;
+  if (threadIdx.x == 0) {
+    mbar_init(&q_full, 1);
+    for (int s = 0; s < G::kStages; ++s) {
+      mbar_init(&k_full[s], 1);
+      mbar_init(&k_free[s], 1);
+      mbar_init(&v_full[s], 1);
+      mbar_init(&v_free[s], 1);
+    }
+    mbar_init(&s_full, 1);
+    mbar_init(&p_full, 4);
+    mbar_init(&o_full, 1);
+    fence_mbar_init();
+    sh_slow = sh_dead = 0;
+  }
+  if (warp == 5) {
+    tmem_alloc(&tmem_base, 2 * DP);
+    tmem_relinquish();
+  }
+  tc_fence_before();
+  __syncthreads();
+  tc_fence_after();
+  const unsigned tm_s = tmem_base, tm_o = tmem_base + DP;
+  const int tiles = (keys.blocks + G::kBlocks - 1) / G::kBlocks;
+  // A wait that runs out ends its role; the others' waits then run out as well.
+  auto wait = [&](unsigned long long* bar, int use) -> bool {
+    if (mbar_wait_bounded(bar, use & 1, kWaitNs)) return true;
+    *(volatile int*)&sh_dead = 1;
+    return false;
+  };
+
+  if (warp == 4) {
+    if ((threadIdx.x & 31) == 0) {
+      const int kv = h / (a.heads / a.kv_heads);
+      mbar_expect_tx(&q_full, G::kQBytes);
+      for (int p = 0; p < G::kPanels; ++p)
+        copy_box(sq + p * kTileRows * 128, &maps.q, p * 64, h, tile * kTileRows, &q_full);
+      int issued = 0;
+      for (; issued < tiles; ++issued) {
+        const int s = issued % G::kStages, use = issued / G::kStages, b0 = issued * G::kBlocks;
+        const int nb = min(G::kBlocks, keys.blocks - b0);
+        bool ok = true;
+        for (int side = 0; side < 2 && ok; ++side) {
+          unsigned long long *full = side ? &v_full[s] : &k_full[s], *free = side ? &v_free[s] : &k_free[s];
+          if (use > 0 && !(ok = wait(free, use - 1))) break;
+          unsigned char* dst = (side ? sv : sk) + s * G::kKvBytes;
+          mbar_expect_tx(full, nb * G::kPanels * kBlockRows * 128);
+          for (int b = 0; b < nb; ++b)
+            for (int p = 0; p < G::kPanels; ++p)
+              copy_box(dst + p * G::kKeys * 128 + b * kBlockRows * 128, side ? &maps.v : &maps.k, p * 64, kv,
+                       keys.base(b0 + b), full);
+        }
+        if (!ok) break;
+      }
+      if (*(volatile int*)&sh_dead) {  // no copy may land after the CTA has left
+        wait(&q_full, 0);
+        for (int i = max(0, issued - G::kStages); i < min(tiles, issued + 1); ++i) {
+          mbar_wait_bounded(&k_full[i % G::kStages], (i / G::kStages) & 1, kWaitNs);
+          mbar_wait_bounded(&v_full[i % G::kStages], (i / G::kStages) & 1, kWaitNs);
+        }
+      }
+    }
+  } else if (warp == 5) {
+    if ((threadIdx.x & 31) == 0 && wait(&q_full, 0)) {
+      const int ksteps = (a.head_dim + 15) / 16, n_o = ksteps * 16;
+      const unsigned idesc_o = umma_idesc<T>(kTileRows, n_o) | (1u << 16);  // V: N contiguous
+      for (int i = 0; i < tiles; ++i) {
+        const int s = i % G::kStages, use = i / G::kStages, nb = min(G::kBlocks, keys.blocks - i * G::kBlocks);
+        if (!wait(&k_full[s], use)) break;
+        if (i > 0 && !wait(&o_full, i - 1)) break;  // P(i - 1), under S, has been read
+        tc_fence_after();
+        const unsigned idesc_s = umma_idesc<T>(kTileRows, nb * kBlockRows);
+        for (int k = 0; k < ksteps; ++k)
+          umma_f16(tm_s, swizzled_desc(sq + (k / 4) * kTileRows * 128 + (k % 4) * 32, 0),
+                   swizzled_desc(sk + s * G::kKvBytes + (k / 4) * G::kKeys * 128 + (k % 4) * 32, 0), idesc_s, k > 0);
+        umma_commit(&k_free[s]);
+        umma_commit(&s_full);
+        if (!wait(&v_full[s], use) || !wait(&p_full, i)) break;
+        tc_fence_after();
+        for (int k = 0; k < nb * 2; ++k)
+          umma_f16_ts(tm_o, tm_s + k * 8, swizzled_desc(sv + s * G::kKvBytes + k * 2048, G::kKeys * 128), idesc_o,
+                      i > 0 || k > 0);
+        umma_commit(&v_free[s]);
+        umma_commit(&o_full);
+      }
+    }
+  } else {
+    const int row = tile * kTileRows + threadIdx.x, lane = threadIdx.x & 31;
+    const unsigned my_s = tm_s + ((unsigned)(warp * 32) << 16), my_o = tm_o + ((unsigned)(warp * 32) << 16);
+    const bool inside = row >= keys.r0 && row <= keys.r1;
+    const int start = inside ? sequence_start(a, row) : -1;
+    const int low = (int)max((long long)start, (long long)row - a.window + 1);
+    const int sink_last = (int)min((long long)row, (long long)start + a.sinks - 1);
+    // the tile's common part: keys every row sees lie in [all_low, r0]
+    const int start_last = sequence_start(a, keys.r1);
+    const int all_low = (int)max((long long)start_last, (long long)keys.r1 - a.window + 1);
+    const float c = a.scale * 1.4426950408889634f;
+    float m = -INFINITY, l = 0.f;  // m: reference of the weights, in units of S
+    bool ok = true;
+    for (int i = 0; i < tiles && ok; ++i) {
+      const int b0 = i * G::kBlocks, nb = min(G::kBlocks, keys.blocks - b0);
+      const bool plain = b0 >= keys.sink_blocks && keys.base(b0) >= all_low &&
+                         keys.base(b0 + nb - 1) + kBlockRows - 1 <= keys.r0;
+      if (!(ok = wait(&s_full, i))) break;
+      tc_fence_after();
+      auto masked = [&](int b, float (&x)[32]) {
+        if (plain) return;
+        const int base = keys.base(b0 + b);
+        unsigned bits = 0;
+        if (start >= 0) {
+          if (b0 + b < keys.sink_blocks)
+            bits = start == keys.start ? bit_range(0, min(sink_last, keys.sink_end - 1) - base) : 0u;
+          else
+            bits = bit_range(low - base, row - base) | bit_range(start - base, sink_last - base);
+        }
+#pragma unroll
+        for (int e = 0; e < 32; ++e) x[e] = (bits >> e) & 1u ? x[e] : -INFINITY;
+      };
+      float x[32], top = -INFINITY;
+      for (int b = 0; b < nb; ++b) {
+        tmem_ld32(my_s + b * 32, x);
+        masked(b, x);
+#pragma unroll
+        for (int e = 0; e < 32; ++e) top = fmaxf(top, x[e]);
+      }
+      // a new reference only when the old one is too low; exp2(8) is the most a weight can be
+      const bool grow = top > m && !((top - m) * c <= 8.f);
+      if (__any_sync(0xffffffffu, grow)) {
+        const float next = grow ? top : m;
+        const float keep = next == -INFINITY ? 1.f : exp2_fast((m - next) * c);
+        m = next;
+        l *= keep;
+        if (i > 0) {
+#pragma unroll
+          for (int d = 0; d < DP; d += 32) {
+            float o[32];
+            tmem_ld32(my_o + d, o);
+#pragma unroll
+            for (int e = 0; e < 32; ++e) o[e] *= keep;
+            tmem_st32(my_o + d, o);
+          }
+        }
+      }
+      // fp16 weights 2^7 higher, up to 2^15, away from its denormals
+      const float ref = m == -INFINITY ? 0.f : m * c - (std::is_same<T, __half>::value ? 7.f : 0.f);
+      for (int b = 0; b < nb; ++b) {
+        tmem_ld32(my_s + b * 32, x);
+        masked(b, x);
+        unsigned p[16];
+#pragma unroll
+        for (int e = 0; e < 32; ++e) {
+          x[e] = exp2_fast(fmaf(x[e], c, -ref));
+          l += x[e];
+        }
+#pragma unroll
+        for (int e = 0; e < 16; ++e) p[e] = pack2((T*)nullptr, x[2 * e], x[2 * e + 1]);
+        tmem_st16(my_s + b * 16, p);
+      }
+      if (!plain) {
+        // a value that is not finite would reach rows that do not see it
+        const int s = i % G::kStages;
+        if (!(ok = wait(&v_full[s], i / G::kStages))) break;
+        const unsigned top_bits = std::is_same<T, __half>::value ? 0x7c007c00u : 0x7f807f80u;
+        const unsigned one = std::is_same<T, __half>::value ? 0x04000400u : 0x00800080u;  // carries into bit 15 or 31
+        unsigned bad = 0;
+        for (int p = 0; p < G::kPanels; ++p) {
+          const uint4* v = reinterpret_cast<const uint4*>(sv + s * G::kKvBytes + p * G::kKeys * 128);
+          for (int e = threadIdx.x; e < nb * kBlockRows * 8; e += 128) {
+            const uint4 u = v[e];
+            bad |= ((u.x & top_bits) + one) | ((u.y & top_bits) + one) | ((u.z & top_bits) + one) | ((u.w & top_bits) + one);
+          }
+        }
+        if (bad & 0x80008000u) sh_slow = 1;
+      }
+      tmem_st_wait();
+      tc_fence_before();
+      __syncwarp();
+      if (lane == 0) mbar_arrive(&p_full);
+    }
+    if (ok) ok = wait(&o_full, tiles - 1);
+    tc_fence_after();
+    const bool good = __all_sync(0xffffffffu, ok);
+    if (good || inside) {
+      T* to = static_cast<T*>(a.out) + (long long)row * a.o_row + h * a.o_head;
+#pragma unroll
+      for (int d = 0; d < DP; d += 32) {
+        float o[32];
+        if (good) tmem_ld32(my_o + d, o);
+        const float inv = good ? 1.f / l : NAN;
+        if (inside && start >= 0)
+#pragma unroll
+          for (int e = 0; e < 32; e += 8) {
+            if (d + e < a.head_dim) {
+              float r[8];
+#pragma unroll
+              for (int w = 0; w < 8; ++w) r[w] = good ? o[e + w] * inv : NAN;
+              store8(to + d + e, r);
+            }
+          }
+      }
+    }
+    tc_fence_before();
+  }
+  __syncthreads();
+  tc_fence_after();
+  if (warp == 5) tmem_dealloc(tmem_base, 2 * DP);
+  if (sh_slow && !sh_dead && warp < 4) {
+    constexpr int kLanes = DP / 8;
+    for (int r = keys.r0 + threadIdx.x / kLanes; r <= keys.r1; r += 128 / kLanes) {
+      const int start = sequence_start(a, r);
+      if (start >= 0) window_row<T, kLanes>(a, r, start, h, threadIdx.x % kLanes, row_mask<kLanes>());
+    }
+  }
 }
 
 template <typename T, int LANES>
@@ -92,6 +482,46 @@ void launch_window(const WindowArgs& a, cudaStream_t s) {
     case 16: launch_rows<T, 16>(a, s); break;
     default: launch_rows<T, 32>(a, s); break;
   }
+}
+
+using EncodeTiled = CUresult (*)(CUtensorMap*, CUtensorMapDataType, cuuint32_t, void*, const cuuint64_t*,
+                                 const cuuint64_t*, const cuuint32_t*, const cuuint32_t*, CUtensorMapInterleave,
+                                 CUtensorMapSwizzle, CUtensorMapL2promotion, CUtensorMapFloatOOBfill);
+EncodeTiled encode_tiled() {
+  static std::atomic<EncodeTiled> fn{nullptr};
+  EncodeTiled f = fn.load(std::memory_order_acquire);
+  if (!f) {
+    void* p = nullptr;
+    cudaDriverEntryPointQueryResult found{};
+    if (cudaGetDriverEntryPointByVersion("cuTensorMapEncodeTiled", &p, 12000, cudaEnableDefault, &found) != cudaSuccess ||
+        found != cudaDriverEntryPointSuccess)
+      return nullptr;
+    f = reinterpret_cast<EncodeTiled>(p);
+    fn.store(f, std::memory_order_release);
+  }
+  return f;
+}
+
+// [rows][heads][head_dim] as a tensor whose boxes are 64 columns of `box_rows` rows of one head. Columns past
+// head_dim and rows past `rows` read as zeros. A stride along a dimension of one element, or of 0, is never used.
+bool encode_rows(CUtensorMap* map, const st_rows& r, int mode, long long rows, int heads, int head_dim, int box_rows) {
+  const cuuint64_t dims[3] = {(cuuint64_t)head_dim, (cuuint64_t)heads, (cuuint64_t)rows};
+  const cuuint64_t strides[2] = {(cuuint64_t)r.head_stride * 2, (cuuint64_t)r.row_stride * 2};
+  const cuuint32_t box[3] = {64, 1, (cuuint32_t)box_rows}, step[3] = {1, 1, 1};
+  const EncodeTiled encode = encode_tiled();
+  return encode && encode(map, mode == ST_MODE_FP16 ? CU_TENSOR_MAP_DATA_TYPE_FLOAT16 : CU_TENSOR_MAP_DATA_TYPE_BFLOAT16, 3,
+                          r.data, dims, strides, box, step, CU_TENSOR_MAP_INTERLEAVE_NONE, CU_TENSOR_MAP_SWIZZLE_128B,
+                          CU_TENSOR_MAP_L2_PROMOTION_L2_256B, CU_TENSOR_MAP_FLOAT_OOB_FILL_NONE) == CUDA_SUCCESS;
+}
+
+template <typename T, int DP>
+cudaError_t launch_tiles(const WindowArgs& a, const TileMaps& maps, cudaStream_t s) {
+  const cudaError_t e =
+      cudaFuncSetAttribute(k_window_tiles<T, DP>, cudaFuncAttributeMaxDynamicSharedMemorySize, Tiles<DP>::kSmem);
+  if (e != cudaSuccess) return e;
+  const unsigned tiles = (unsigned)((a.rows + kTileRows - 1ll) / kTileRows);
+  k_window_tiles<T, DP><<<tiles * a.heads, kTileThreads, Tiles<DP>::kSmem, s>>>(a, maps);
+  return cudaSuccess;
 }
 
 }  // namespace
@@ -131,8 +561,27 @@ extern "C" int st_window_attention(const st_window* p, void* stream) {
   a.heads = p->heads; a.kv_heads = p->kv_heads; a.head_dim = p->head_dim;
   a.window = p->window; a.sinks = p->sinks; a.scale = p->scale;
   cudaStream_t s = static_cast<cudaStream_t>(stream);
-  if (p->mode == ST_MODE_FP32) launch_window<float>(a, s);
-  else if (p->mode == ST_MODE_FP16) launch_window<__half>(a, s);
-  else launch_window<__nv_bfloat16>(a, s);
+  TileMaps maps;
+  const long long ctas = (p->rows + kTileRows - 1) / kTileRows * p->heads;
+  const bool tiles = p->mode != ST_MODE_FP32 && p->head_dim <= 128 && p->scale > 0.f && ctas <= INT32_MAX &&
+                     encode_rows(&maps.q, p->q, p->mode, p->rows, p->heads, p->head_dim, kTileRows) &&
+                     encode_rows(&maps.k, p->k, p->mode, p->rows, p->kv_heads, p->head_dim, kBlockRows) &&
+                     encode_rows(&maps.v, p->v, p->mode, p->rows, p->kv_heads, p->head_dim, kBlockRows);
+  if (tiles) {
+    const bool half = p->mode == ST_MODE_FP16, small = p->head_dim <= 64;
+    const cudaError_t e = half ? (small ? launch_tiles<__half, 64>(a, maps, s) : launch_tiles<__half, 128>(a, maps, s))
+                               : (small ? launch_tiles<__nv_bfloat16, 64>(a, maps, s)
+                                        : launch_tiles<__nv_bfloat16, 128>(a, maps, s));
+    if (e != cudaSuccess) {
+      cudaGetLastError();  // reported here, so not left pending
+      return cache_cuda(e, "window attention: ");
+    }
+  } else if (p->mode == ST_MODE_FP32) {
+    launch_window<float>(a, s);
+  } else if (p->mode == ST_MODE_FP16) {
+    launch_window<__half>(a, s);
+  } else {
+    launch_window<__nv_bfloat16>(a, s);
+  }
   return cache_cuda(cudaGetLastError(), "window attention launch: ");
 }

@@ -10,13 +10,13 @@ Attention: o = sum_j p_j v_j / sum_j p_j.
     exponential: 2 F |logit - max| more; the fast exponential adds 2^-21.
     A weight is therefore off by w = 2 max_j(logit error) + 2^-20 relative.
   * kernels that multiply weights and values as 16-bit operands round each weight
-    once: u(T), or in fp16 2^-35 of the largest weight where that is more (they
-    are held 2^10 times larger, and fp16 steps by 2^-24 at its low end).
+    once: u(T), or in fp16 2^-32 of the largest weight where that is more (they
+    are held at least 2^7 times larger, and fp16 steps by 2^-24 at its low end).
   * 4-bit rows are rounded to 16-bit operands: a key to T, which moves a logit by
     u(T) scale sum|q k| more, a value and its weight to bf16, u(bf16) each.
   * sums of n terms in up to n / 8 + 64 steps a chain: (n / 8 + 64) F.
   * the result is rounded to T.
-  |got - o| <= u(T) |o| + (1 + u(T)) (2 w + u(P) + u(V) + 2 (n / 8 + 64) F) sum p |v| / sum p + tiny(T) (+ n 2^-35 max|v|)
+  |got - o| <= u(T) |o| + (1 + u(T)) (2 w + u(P) + u(V) + 2 (n / 8 + 64) F) sum p |v| / sum p + tiny(T) (+ n 2^-32 max|v|)
 """
 from __future__ import annotations
 
@@ -54,7 +54,7 @@ def attention(q, k, v, see, scale, dtype, four=False):
     up = 2 * half if four else u
     bound = u * out.abs() + (1 + u) * (2 * w + up + 2 * (n / 8 + 64) * F) * size + TINY[dtype]
     if dtype == torch.float16 and not four:
-        bound = bound + n * 2.0 ** -35 * clean.abs().amax()
+        bound = bound + n * 2.0 ** -32 * clean.abs().amax()
     return out, torch.where(seen_any, bound, 0.0)
 
 
