@@ -6,21 +6,26 @@ Outputs (git-ignored, but shipped with the source tree to the GPU box):
     streaming_transformer_b200/lib/libstreaming_b200.so   CUDA kernels + C ABI
     streaming_transformer_b200/lib/libstream_runtime.so   C++ Stream::Runtime / Stream::Model
                                                           API over the C ABI
+    streaming_transformer_b200/lib/attention_binding.so   torch tensors to the window-cache entry
+                                                          points (skipped where torch is missing)
 A target is rebuilt only when one of its sources is newer than it.
 """
 from __future__ import annotations
 
 import argparse
+import importlib.util
 import os
 import shutil
 import subprocess
 import sys
+import sysconfig
 from pathlib import Path
 
 PKG = Path(__file__).resolve().parent
 ROOT = PKG.parent
 CSRC = PKG / "csrc"
 HOST = PKG / "host"
+BINDING = PKG / "binding"
 LIB = PKG / "lib"
 INCLUDE = ROOT / "include"
 CUDA_HOME = Path(os.environ.get("CUDA_HOME", "/usr/local/cuda"))
@@ -35,6 +40,7 @@ NVCC_FLAGS = ["-O3", "-lineinfo", "-std=c++17", "-Xcompiler", "-fPIC", "-Xptxas"
 
 CUDA_LIB = LIB / "libstreaming_b200.so"
 CPP_LIB = LIB / "libstream_runtime.so"
+TORCH_LIB = LIB / "attention_binding.so"
 
 
 def _stale(target: Path, sources: list[Path]) -> bool:
@@ -90,9 +96,26 @@ def build_cpp(force: bool = False) -> Path | None:
     return CPP_LIB
 
 
+def build_binding(force: bool = False) -> Path | None:
+    spec = importlib.util.find_spec("torch")
+    if spec is None:
+        return None
+    torch = Path(spec.origin).parent
+    deps = [*BINDING.glob("*.cpp"), INCLUDE / "streaming_b200.h", CUDA_LIB, torch / "version.py"]
+    if force or _stale(TORCH_LIB, deps):
+        includes = [INCLUDE, torch / "include", torch / "include" / "torch" / "csrc" / "api" / "include",
+                    sysconfig.get_paths()["include"], CUDA_HOME / "include"]
+        _run([CXX, "-O2", "-std=c++17", "-fPIC", "-shared", *[f"-I{d}" for d in includes], "-o", str(TORCH_LIB),
+              *[str(s) for s in sorted(BINDING.glob("*.cpp"))], "-L", str(LIB), "-lstreaming_b200",
+              "-L", str(torch / "lib"), "-ltorch_python", "-ltorch", "-ltorch_cpu", "-lc10", "-lc10_cuda",
+              "-Wl,-rpath,$ORIGIN", f"-Wl,-rpath,{torch / 'lib'}"])
+    return TORCH_LIB
+
+
 def build(force: bool = False) -> None:
     build_cuda(force)
     build_cpp(force)
+    build_binding(force)
 
 
 if __name__ == "__main__":
