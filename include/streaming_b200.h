@@ -268,7 +268,8 @@ const char* st_attention_static_error(void);
  * even column in the low bits. Quantising takes lowest = bf16(min), scale =
  * bf16((max - min) * (1/15)) and code = rint((x - lowest) / scale) clamped to
  * 0..15 (0 where the scale is 0). A group with a non-finite value, or whose
- * max - min or bf16(min) is not finite, reads back as NaN.
+ * max - min or bf16(min) is not finite, reads back as NaN. Attention takes
+ * value scales from 2^-56 to 2^56 (or 0).
  *
  * All pointers are device memory of `device`, rows start on 16-byte
  * boundaries, and work is queued on `stream` (a cudaStream_t) without waiting.

@@ -23,14 +23,26 @@
 // S^T leaves slots in rows and heads in columns; movmatrix turns each 8 x 8
 // piece of P into the B operand of the second product.
 //
-// 4-bit rows become the 16-bit operands that a 16-bit cache would hold: a lane's
-// columns lie in one group, codes turn into exact 16-bit numbers two at a time,
-// and one packed multiply-add with the group's scale and lowest value rounds
-// once, to 2^-9 of the value (keys of fp16 rows: 2^-12), where the code itself
-// is off by up to half a scale, a thirtieth of the group's range. Values become
-// bf16 whatever the rows are: its range holds any scale. Folding the scales into
-// fp32 sums instead, without that rounding, took 1.5 to 2 times the instructions
-// and the kernel is bound by those (256 Large streams: 77 us).
+// That holds 4 (head_dim 128) to 2 (64) KB in flight a warp, in registers. 4-bit
+// rows are too short for it: they go through a ring in shared memory, a few
+// stages of 16 or 32 slots for each warp, filled by 16-byte cp.async (zeros past
+// the last slot). Rows there are an odd number of 16-byte units apart, so that
+// neither product's reads meet in a bank.
+//
+// 4-bit rows: the codes enter the products as they are. A nibble in the low
+// byte of a 16-bit word is that many of the type's smallest steps (c 2^-24 in
+// fp16, c 2^-133 in bf16; 16 c for the byte's high nibble), which the
+// instruction takes exactly, so a word of 8 codes costs four masks and a shift.
+// Queries are scaled by a power of two per head beforehand so that sums come out
+// as normal numbers (and by 1/16 where they meet a high nibble). A product stays
+// within one group of 32 columns, whose scale and lowest value then enter in
+// fp32: sum q k = scale * sum q c + lowest * sum q. For values the scale is
+// folded into the weight before its one rounding, to bf16 (times 2^70: its range
+// takes scales from 2^-56 to 2^56). Codes are 0..15 where the values lie about
+// 0, so that rounding would count double; the fp32 sum beside the product takes
+// p * (lowest + 7.5 scale) - 7.5 * (the rounded weight), which leaves the error
+// with the code's distance from 7.5. Turning codes into 16-bit values first took 1.7 times the
+// instructions, which bound the kernel, and rounded each value once more.
 //
 // Softmax statistics are fp32: a running maximum per head (in units of log2),
 // the sum of unrounded weights, and output sums. Weights are rounded to the 16
@@ -96,16 +108,18 @@ __device__ __forceinline__ uint4 ld_row16(const void* p) {
                : "=r"(r.x), "=r"(r.y), "=r"(r.z), "=r"(r.w) : "l"(p));
   return r;
 }
-__device__ __forceinline__ uint2 ld_row8(const void* p) {
-  uint2 r;
-  asm volatile("ld.global.nc.v2.u32 {%0,%1}, [%2];" : "=r"(r.x), "=r"(r.y) : "l"(p));
-  return r;
+// 16, 8 or 4 bytes to shared memory, zeros unless `in`.
+template <int N>
+__device__ __forceinline__ void copy_async(void* dst, const void* src, bool in) {
+  const unsigned to = (unsigned)__cvta_generic_to_shared(dst);
+  if constexpr (N == 16)
+    asm volatile("cp.async.cg.shared.global [%0], [%1], 16, %2;" ::"r"(to), "l"(src), "r"(in ? 16 : 0) : "memory");
+  else
+    asm volatile("cp.async.ca.shared.global [%0], [%1], %2, %3;" ::"r"(to), "l"(src), "n"(N), "r"(in ? N : 0) : "memory");
 }
-__device__ __forceinline__ unsigned ld_row4(const void* p) {
-  unsigned r;
-  asm volatile("ld.global.nc.u32 %0, [%1];" : "=r"(r) : "l"(p));
-  return r;
-}
+__device__ __forceinline__ void copy_commit() { asm volatile("cp.async.commit_group;" ::: "memory"); }
+template <int N>
+__device__ __forceinline__ void copy_wait() { asm volatile("cp.async.wait_group %0;" ::"n"(N) : "memory"); }
 
 // Part of this CTA's split in tiles of `tile` slots: [first, last).
 __device__ __forceinline__ void split_slots(int seen, int tile, int split, int splits, int& first, int& last) {
@@ -131,42 +145,41 @@ __device__ __forceinline__ void let_next_kernel_start() { asm volatile("griddepc
 __device__ __forceinline__ void wait_for_previous_kernel() { asm volatile("griddepcontrol.wait;" ::: "memory"); }
 
 // ---------------------------------------------------------------- 16-bit and 4-bit rows
-// {scale, lowest} twice over, as packed operands of T.
-template <typename T>
-__device__ __forceinline__ void group_operands(unsigned pair_a, unsigned pair_b, unsigned& scale, unsigned& lowest) {
-  if constexpr (std::is_same<T, __half>::value) {
-    scale = pack2((__half*)nullptr, group_scale(pair_a), group_scale(pair_b));
-    lowest = pack2((__half*)nullptr, group_lowest(pair_a), group_lowest(pair_b));
-  } else {
-    scale = __byte_perm(pair_a, pair_b, 0x5410);
-    lowest = __byte_perm(pair_a, pair_b, 0x7632);
-  }
+// Nibbles 0 .. 3 of each half of `w`: as low-byte steps, the odd ones times 16.
+__device__ __forceinline__ void code_steps(unsigned w, unsigned (&c)[4]) {
+  const unsigned z = w >> 8;
+  c[0] = w & 0x000f000fu; c[1] = w & 0x00f000f0u; c[2] = z & 0x000f000fu; c[3] = z & 0x00f000f0u;
 }
-// Nibble i of both halves of `w` as lowest + scale * code, rounded once. The
-// nibble in the low mantissa bits of 2^10 (fp16) or 2^7 (bf16) is an exact
-// number, from which the power is taken off again.
-template <typename T>
-__device__ __forceinline__ unsigned decode_pair(unsigned w, int i, unsigned scale, unsigned lowest) {
-  using T2 = typename std::conditional<std::is_same<T, __half>::value, __half2, __nv_bfloat162>::type;
-  const unsigned base = std::is_same<T, __half>::value ? 0x64006400u : 0x43004300u;
-  const unsigned x = ((w >> (4 * i)) & 0x000f000fu) | base;
-  const T2 c = __hsub2(*reinterpret_cast<const T2*>(&x), *reinterpret_cast<const T2*>(&base));
-  const T2 y = __hfma2(c, *reinterpret_cast<const T2*>(&scale), *reinterpret_cast<const T2*>(&lowest));
-  return *reinterpret_cast<const unsigned*>(&y);
-}
+constexpr float kValueLift = 0x1p70f, kValueDrop = 0x1p63f;  // 2^70 on the weights, 2^-133 on the codes
+
+// Shared memory of a CTA: the warps' rings (4-bit rows), and after the loop their parts of the result.
+template <int DB, int NT, bool INT4>
+struct AttendSmem {
+  static constexpr int kTiles = INT4 && DB * NT <= 2 ? 2 : 1;         // tiles of 16 slots in a step (or stage)
+  static constexpr int kStages = 2;  // 3 and 4 stages leave room for fewer warps: 1 % and 12 % slower
+  static constexpr int kRowBytes = DB * 32 + 16;                       // largest distance of 4-bit rows
+  static constexpr int kScaleBytes = DB * 8;                           // largest scales of a slot
+  static constexpr int kStageBytes = 16 * kTiles * 2 * (kRowBytes + kScaleBytes);
+  static constexpr int kRing = INT4 ? kAttendWarps * kStages * kStageBytes : 0;
+  static constexpr int kPartRow = DB * 64 + 4;                         // floats
+  static constexpr int kParts = kAttendWarps * NT * 8 * kPartRow * 4;
+  static constexpr int kBytes = kRing > kParts ? kRing : kParts;
+};
 
 // DB: blocks of 64 columns; NT: blocks of 8 query heads; FULL: head_dim is
 // 64 DB, so that row offsets are constants and no column is checked; ONE: one
 // query head a key head, so that the odd columns of S^T are not computed on.
-// A step takes TS tiles of 16 slots.
 template <typename T, int DB, int NT, bool INT4, bool FULL, bool ONE>
-__global__ void __launch_bounds__(kAttendThreads, DB * NT == 1 ? 6 : 1) k_attend_mma(const AttendArgs a) {
+__global__ void __launch_bounds__(kAttendThreads, DB * NT == 1 ? (INT4 ? 5 : 6) : INT4 && DB == 2 && NT == 1 ? 3 : 1)
+    k_attend_mma(const AttendArgs a) {
   constexpr int J = 2 * DB;   // 16-bit: 16-byte pieces of a key row a lane holds
-  constexpr int TS = INT4 && DB * NT <= 2 ? 2 : 1;
+  using Smem = AttendSmem<DB, NT, INT4>;
+  constexpr int TS = Smem::kTiles;
   constexpr int X = ONE ? 1 : 2;  // query heads a lane has of each block: 8 n + 2 t + x
   using PT = typename std::conditional<INT4, __nv_bfloat16, T>::type;  // operands of the second product
   constexpr float kLift = std::is_same<PT, __half>::value ? 10.f : 0.f;
-  __shared__ float sh_o[kAttendWarps][NT * 8][DB * 64 + 4];
+  extern __shared__ uint4 dynamic[];
+  float(*sh_o)[NT * 8][Smem::kPartRow] = reinterpret_cast<float(*)[NT * 8][Smem::kPartRow]>(dynamic);
   __shared__ float sh_m[kAttendWarps][NT * 8], sh_l[kAttendWarps][NT * 8];
   const int split = blockIdx.x, kv = blockIdx.y / a.blocks, block = blockIdx.y % a.blocks, stream = blockIdx.z;
   const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31, g = lane >> 2, t = lane & 3;
@@ -181,156 +194,232 @@ __global__ void __launch_bounds__(kAttendThreads, DB * NT == 1 ? 6 : 1) k_attend
   const int dim = FULL ? DB * 64 : a.head_dim, groups = dim / 32, row_bytes = INT4 ? dim / 2 : dim * 2;
   constexpr int kStep = 16 * TS * kAttendWarps;
   int slot0 = first + warp * 16 * TS;
-  // this lane's first addresses of the tile to load next
-  const char* kp = static_cast<const char*>(a.keys) + (row0 + slot0 + g) * row_bytes + t * (INT4 ? 8 * DB : 16);
-  const char* vp = static_cast<const char*>(a.values) + (row0 + slot0 + 2 * t) * row_bytes + g * (INT4 ? 4 * DB : 16);
-  const unsigned* ksp = INT4 ? a.key_scales + (row0 + slot0 + g) * groups + t * DB / 2 : nullptr;
-  const unsigned* vsp = INT4 ? a.value_scales + (row0 + slot0 + 2 * t) * groups + g * DB / 4 : nullptr;
+  constexpr int SW = INT4 ? J : 1;
 
-  // one step's rows in registers, loaded a step ahead of their use
-  constexpr int KW = INT4 ? DB * 2 : J * 4, VW = INT4 ? DB : DB * 4, KG = INT4 ? (DB + 1) / 2 : 1;
-  unsigned kf[TS][2][KW], vf[TS][4][VW], ks[TS][2][KG], vs[TS][4];
+  // 4-bit rows: this warp's ring. A stage: key rows, value rows, key scales, value scales of kSlots slots.
+  constexpr int kSlots = 16 * TS;
+  const int row_apart = row_bytes + (row_bytes / 16 % 2 ? 0 : 16), scale_bytes = groups * 4;
+  char* const ring = reinterpret_cast<char*>(dynamic) + warp * Smem::kStages * Smem::kStageBytes;
+  const char* const k4 = static_cast<const char*>(a.keys) + row0 * row_bytes;
+  const char* const v4 = static_cast<const char*>(a.values) + row0 * row_bytes;
+  const char* const ks4 = reinterpret_cast<const char*>(a.key_scales) + row0 * scale_bytes;
+  const char* const vs4 = reinterpret_cast<const char*>(a.value_scales) + row0 * scale_bytes;
+  auto fill = [&](int stage, int at) {
+    if (at < last) {
+      char* to = ring + stage * Smem::kStageBytes;
+      const int chunks = row_bytes / 16;
+      const long long off = (long long)at * row_bytes;
+      auto rows = [&](int c) {
+        const int row = FULL ? c / (2 * DB) : c / chunks, col = FULL ? c % (2 * DB) : c - row * chunks;
+        const bool in = at + row < last;
+        copy_async<16>(to + row * row_apart + col * 16, k4 + (in ? off + c * 16 : 0), in);
+        copy_async<16>(to + (kSlots + row) * row_apart + col * 16, v4 + (in ? off + c * 16 : 0), in);
+      };
+      if constexpr (FULL) {
+#pragma unroll
+        for (int c = 0; c < kSlots * 2 * DB; c += 32) rows(c + lane);
+      } else {
+        for (int c = lane; c < kSlots * chunks; c += 32) rows(c);
+      }
+      to += 2 * kSlots * row_apart;
+      const long long soff = (long long)at * scale_bytes;
+      // lanes take slots: 32 of each side, or 16 of both
+      const int slot = TS == 2 ? lane : lane & 15;
+      const bool in = at + slot < last;
+#pragma unroll
+      for (int side = 0; side < TS; ++side) {
+        const bool value = TS == 2 ? side == 1 : lane >= 16;
+        const char* from = (value ? vs4 : ks4) + (in ? soff + slot * scale_bytes : 0);
+        char* dst = to + (value ? kSlots * scale_bytes : 0) + slot * scale_bytes;
+        if constexpr (FULL) {
+          constexpr int N = DB == 1 ? 8 : 16;
+#pragma unroll
+          for (int i = 0; i < 8 * DB; i += N) copy_async<N>(dst + i, from + i, in);
+        } else {
+          for (int i = 0; i < scale_bytes; i += 4) copy_async<4>(dst + i, from + i, in);
+        }
+      }
+    }
+    copy_commit();
+  };
+  // scales of slot `slot` of a stage's side
+  auto read_scales = [&](const char* p, int slot, unsigned(&f)[SW]) {
+    p += slot * scale_bytes;
+    if constexpr (FULL && J == 2) {
+      const uint2 w = *reinterpret_cast<const uint2*>(p);
+      f[0] = w.x; f[1] = w.y;
+    } else if constexpr (FULL && INT4) {
+#pragma unroll
+      for (int j = 0; j < J; j += 4) {
+        const uint4 w = *reinterpret_cast<const uint4*>(p + 4 * j);
+        f[j] = w.x; f[j + 1] = w.y; f[j + 2] = w.z; f[j + 3] = w.w;
+      }
+    } else {
+#pragma unroll
+      for (int j = 0; j < SW; ++j) f[j] = j < groups ? *reinterpret_cast<const unsigned*>(p + 4 * j) : 0u;
+    }
+  };
 
+  // 16-bit rows: one tile in registers, loaded a step ahead of its use. This lane's first addresses:
+  const char* kp = static_cast<const char*>(a.keys) + (row0 + slot0 + g) * row_bytes + t * 16;
+  const char* vp = static_cast<const char*>(a.values) + (row0 + slot0 + 2 * t) * row_bytes + g * 16;
+  unsigned kf[2][J * 4], vf[4][DB * 4];
   // Slots past `last` load nothing and count as zeros, so that no value there matters; `whole`: the step has none.
   auto load_k = [&](int at, bool whole) {
 #pragma unroll
-    for (int u = 0; u < TS; ++u)
+    for (int r = 0; r < 2; ++r) {
+      const bool in = whole || at + g + 8 * r < last;
+      const char* p = kp + 8 * r * row_bytes;
 #pragma unroll
-      for (int r = 0; r < 2; ++r) {
-        const int ahead = 16 * u + 8 * r;
-        const bool in = whole || at + g + ahead < last;
-        const char* p = kp + ahead * row_bytes;
-        if constexpr (INT4) {  // columns 16 DB t .. + 16 DB - 1
-          if constexpr (DB == 1) {
-            const uint2 w = in && (FULL || t * 16 < dim) ? ld_row8(p) : make_uint2(0, 0);
-            kf[u][r][0] = w.x; kf[u][r][1] = w.y;
-          } else {
-#pragma unroll
-            for (int i = 0; i < DB / 2; ++i) {
-              const uint4 w = in && (FULL || t * 16 * DB + 32 * i < dim) ? ld_row16(p + 16 * i) : make_uint4(0, 0, 0, 0);
-              kf[u][r][4 * i] = w.x; kf[u][r][4 * i + 1] = w.y; kf[u][r][4 * i + 2] = w.z; kf[u][r][4 * i + 3] = w.w;
-            }
-          }
-#pragma unroll
-          for (int i = 0; i < KG; ++i)
-            ks[u][r][i] = in && (FULL || t * 16 * DB + 32 * i < dim) ? ld_row4(ksp + ahead * groups + i) : 0u;
-        } else {
-#pragma unroll
-          for (int j = 0; j < J; ++j) {
-            const uint4 w = in && (FULL || j * 32 + t * 8 < dim) ? ld_row16(p + j * 64) : make_uint4(0, 0, 0, 0);
-            kf[u][r][4 * j] = w.x; kf[u][r][4 * j + 1] = w.y; kf[u][r][4 * j + 2] = w.z; kf[u][r][4 * j + 3] = w.w;
-          }
-        }
+      for (int j = 0; j < J; ++j) {
+        const uint4 w = in && (FULL || j * 32 + t * 8 < dim) ? ld_row16(p + j * 64) : make_uint4(0, 0, 0, 0);
+        kf[r][4 * j] = w.x; kf[r][4 * j + 1] = w.y; kf[r][4 * j + 2] = w.z; kf[r][4 * j + 3] = w.w;
       }
+    }
   };
   auto load_v = [&](int at, bool whole) {
 #pragma unroll
-    for (int u = 0; u < TS; ++u)
+    for (int r = 0; r < 4; ++r) {
+      const int ahead = (r & 1) + 8 * (r >> 1);
+      const bool in = whole || at + 2 * t + ahead < last;
+      const char* p = vp + ahead * row_bytes;
 #pragma unroll
-      for (int r = 0; r < 4; ++r) {
-        const int ahead = 16 * u + (r & 1) + 8 * (r >> 1);
-        const bool in = whole || at + 2 * t + ahead < last;
-        const char* p = vp + ahead * row_bytes;
-        if constexpr (INT4) {  // columns 8 DB g .. + 8 DB - 1
-          const bool on = in && (FULL || g * 8 * DB < dim);
-          if constexpr (DB == 1) {
-            vf[u][r][0] = on ? ld_row4(p) : 0u;
-          } else if constexpr (DB == 2) {
-            const uint2 w = on ? ld_row8(p) : make_uint2(0, 0);
-            vf[u][r][0] = w.x; vf[u][r][1] = w.y;
-          } else {
-            const uint4 w = on ? ld_row16(p) : make_uint4(0, 0, 0, 0);
-            vf[u][r][0] = w.x; vf[u][r][1] = w.y; vf[u][r][2] = w.z; vf[u][r][3] = w.w;
-          }
-          vs[u][r] = on ? ld_row4(vsp + ahead * groups) : 0u;
-        } else {
-#pragma unroll
-          for (int i = 0; i < DB; ++i) {
-            const uint4 w = in && (FULL || i * 64 + g * 8 < dim) ? ld_row16(p + i * 128) : make_uint4(0, 0, 0, 0);
-            vf[u][r][4 * i] = w.x; vf[u][r][4 * i + 1] = w.y; vf[u][r][4 * i + 2] = w.z; vf[u][r][4 * i + 3] = w.w;
-          }
-        }
+      for (int i = 0; i < DB; ++i) {
+        const uint4 w = in && (FULL || i * 64 + g * 8 < dim) ? ld_row16(p + i * 128) : make_uint4(0, 0, 0, 0);
+        vf[r][4 * i] = w.x; vf[r][4 * i + 1] = w.y; vf[r][4 * i + 2] = w.z; vf[r][4 * i + 3] = w.w;
       }
+    }
   };
   auto fetch_k = [&](int at) {
-    if (at + 16 * TS <= last) load_k(at, true);
+    if (at + 16 <= last) load_k(at, true);
     else load_k(at, false);
     kp += (long long)kStep * row_bytes;
-    if (INT4) ksp += kStep * groups;
   };
   auto fetch_v = [&](int at) {
-    if (at + 16 * TS <= last) load_v(at, true);
+    if (at + 16 <= last) load_v(at, true);
     else load_v(at, false);
     vp += (long long)kStep * row_bytes;
-    if (INT4) vsp += kStep * groups;
   };
-  if (slot0 < last) {
+  if constexpr (INT4) {
+#pragma unroll
+    for (int i = 0; i < Smem::kStages - 1; ++i) fill(i, slot0 + i * kStep);
+  } else if (slot0 < last) {
     fetch_k(slot0);
     fetch_v(slot0);
   }
 
-  // query fragments: the columns of this lane's key words, head 8 n + g (4-bit: pairs (i, i + 4) of each 8 columns)
+  // query fragments: the columns of this lane's key words, head 8 n + g
   unsigned qf[NT][J][4];
+  float qsum[NT][INT4 ? J : 1][X], scale2[NT][X];  // 4-bit, heads 8 n + 2 t + x: sum of a group's columns; units of S
 #pragma unroll
   for (int n = 0; n < NT; ++n) {
     const bool head_on = n * 8 + g < nheads;
     const T* qp = static_cast<const T*>(a.q) + stream * a.q_row + (long long)(head0 + n * 8 + g) * a.q_head;
 #pragma unroll
     for (int j = 0; j < J; ++j) {
-      const int col = INT4 ? t * 16 * DB + 8 * j : j * 32 + t * 8;
-      uint4 u = make_uint4(0, 0, 0, 0);
-      if (head_on && col < dim) u = *reinterpret_cast<const uint4*>(qp + col);
-      if (INT4) {
-        qf[n][j][0] = __byte_perm(u.x, u.z, 0x5410);  // columns 0, 4
-        qf[n][j][1] = __byte_perm(u.x, u.z, 0x7632);  // 1, 5
-        qf[n][j][2] = __byte_perm(u.y, u.w, 0x5410);  // 2, 6
-        qf[n][j][3] = __byte_perm(u.y, u.w, 0x7632);  // 3, 7
-      } else {
-        qf[n][j][0] = u.x; qf[n][j][1] = u.y; qf[n][j][2] = u.z; qf[n][j][3] = u.w;
+      uint4 w = make_uint4(0, 0, 0, 0);
+      if (head_on && j * 32 + t * 8 < dim) w = *reinterpret_cast<const uint4*>(qp + j * 32 + t * 8);
+      qf[n][j][0] = w.x; qf[n][j][1] = w.y; qf[n][j][2] = w.z; qf[n][j][3] = w.w;
+    }
+#pragma unroll
+    for (int x = 0; x < X; ++x) scale2[n][x] = a.scale2;
+    if constexpr (INT4) {
+      // the largest exponent of the head, within limits that leave both factors normal numbers
+      constexpr int kTop = std::is_same<T, __half>::value ? 10 : 100, kStep = std::is_same<T, __half>::value ? 24 : 133;
+      float top = 0.f;
+#pragma unroll
+      for (int j = 0; j < J; ++j) {
+        float f[8];
+        load8(reinterpret_cast<const T*>(qf[n][j]), f);
+#pragma unroll
+        for (int i = 0; i < 8; ++i) top = fmaxf(top, fabsf(f[i]));
       }
+      top = fmaxf(top, __shfl_xor_sync(0xffffffffu, top, 1));
+      top = fmaxf(top, __shfl_xor_sync(0xffffffffu, top, 2));
+      const int e = min(max((int)(__float_as_uint(top) >> 23), 107), 220);
+      const float up = __uint_as_float((unsigned)(254 + kTop - e) << 23);                // 2^kTop / 2^(e - 127)
+      const float unit = __uint_as_float((unsigned)(254 + kTop - kStep - e) << 23);      // up * 2^-kStep
+#pragma unroll
+      for (int j = 0; j < J; ++j) {
+        float f[8], sum = 0.f;
+        load8(reinterpret_cast<const T*>(qf[n][j]), f);
+#pragma unroll
+        for (int i = 0; i < 8; ++i) sum += f[i];
+#pragma unroll
+        for (int i = 0; i < 4; ++i) {  // columns i and i + 4 meet a word's nibbles i and i + 4
+          const float by = i & 1 ? up * 0.0625f : up;
+          qf[n][j][i] = pack2((T*)nullptr, f[i] * by, f[i + 4] * by);
+        }
+        sum += __shfl_xor_sync(0xffffffffu, sum, 1);
+        sum += __shfl_xor_sync(0xffffffffu, sum, 2);
+#pragma unroll
+        for (int x = 0; x < X; ++x) qsum[n][j][x] = __shfl_sync(0xffffffffu, sum * unit, (2 * t + x) * 4);
+      }
+#pragma unroll
+      for (int x = 0; x < X; ++x) scale2[n][x] = a.scale2 / __shfl_sync(0xffffffffu, unit, (2 * t + x) * 4);
     }
   }
 
   float o[NT][DB][4][4] = {};        // [head block][column block][m-tile]
+  float olow[NT][INT4 ? J : 1][X] = {};  // 4-bit: the fp32 part, over this lane's slots
   float m[NT][X], l[NT][X];
 #pragma unroll
   for (int n = 0; n < NT; ++n)
 #pragma unroll
     for (int x = 0; x < X; ++x) m[n][x] = -INFINITY, l[n][x] = 0.f;
 
+  int stage = 0;
   for (; slot0 < last; slot0 += kStep) {
+    const char* tile = ring + stage * Smem::kStageBytes;  // this step's stage
+    if constexpr (INT4) {
+      copy_wait<Smem::kStages - 2>();
+      __syncwarp();  // everybody's copies have landed, and nobody reads the stage before this one any more
+      fill(stage == 0 ? Smem::kStages - 1 : stage - 1, slot0 + (Smem::kStages - 1) * kStep);
+      stage = stage + 1 == Smem::kStages ? 0 : stage + 1;
+    }
     // S^T: slots g (c0, c1) and g + 8 (c2, c3) of each tile, heads 8 n + 2 t, + 1
     float s[TS][NT][4] = {};
 #pragma unroll
-    for (int u = 0; u < TS; ++u)
+    for (int u = 0; u < TS; ++u) {
+      unsigned ks[2][SW];
+      if constexpr (INT4)
+#pragma unroll
+        for (int r = 0; r < 2; ++r) read_scales(tile + 2 * kSlots * row_apart, 16 * u + 8 * r + g, ks[r]);
 #pragma unroll
       for (int j = 0; j < J; ++j) {
-        unsigned c[2][4];
         if constexpr (INT4) {
+          if (!FULL && j >= groups) break;
+          unsigned c[2][4];
 #pragma unroll
-          for (int r = 0; r < 2; ++r) {
-            unsigned scale, lowest;
-            const unsigned pair = ks[u][r][j / 4];
-            group_operands<T>(pair, pair, scale, lowest);
+          for (int r = 0; r < 2; ++r)
+            code_steps(*reinterpret_cast<const unsigned*>(tile + (16 * u + 8 * r + g) * row_apart + j * 16 + t * 4), c[r]);
 #pragma unroll
-            for (int x = 0; x < 4; ++x) c[r][x] = decode_pair<T>(kf[u][r][j], x, scale, lowest);
+          for (int n = 0; n < NT; ++n) {
+            float acc[4] = {0.f, 0.f, 0.f, 0.f};
+            mma<T>(acc, c[0][0], c[1][0], c[0][1], c[1][1], qf[n][j][0], qf[n][j][1]);
+            mma<T>(acc, c[0][2], c[1][2], c[0][3], c[1][3], qf[n][j][2], qf[n][j][3]);
+#pragma unroll
+            for (int r = 0; r < 2; ++r)
+#pragma unroll
+              for (int x = 0; x < X; ++x)
+                s[u][n][2 * r + x] = fmaf(acc[2 * r + x], group_scale(ks[r][j]),
+                                          fmaf(group_lowest(ks[r][j]), qsum[n][j][x], s[u][n][2 * r + x]));
           }
         } else {
 #pragma unroll
-          for (int r = 0; r < 2; ++r)
-#pragma unroll
-            for (int x = 0; x < 4; ++x) c[r][x] = kf[u][r][4 * j + x];
-        }
-#pragma unroll
-        for (int n = 0; n < NT; ++n) {
-          mma<T>(s[u][n], c[0][0], c[1][0], c[0][1], c[1][1], qf[n][j][0], qf[n][j][1]);
-          mma<T>(s[u][n], c[0][2], c[1][2], c[0][3], c[1][3], qf[n][j][2], qf[n][j][3]);
+          for (int n = 0; n < NT; ++n) {
+            mma<T>(s[u][n], kf[0][4 * j], kf[1][4 * j], kf[0][4 * j + 1], kf[1][4 * j + 1], qf[n][j][0], qf[n][j][1]);
+            mma<T>(s[u][n], kf[0][4 * j + 2], kf[1][4 * j + 2], kf[0][4 * j + 3], kf[1][4 * j + 3], qf[n][j][2],
+                   qf[n][j][3]);
+          }
         }
       }
+    }
     const int next = slot0 + kStep;
-    if (next < last) fetch_k(next);
+    if constexpr (!INT4)
+      if (next < last) fetch_k(next);
 
-    unsigned pf[TS][NT][2];
+    unsigned pf[TS][NT][SW][2];
 #pragma unroll
     for (int n = 0; n < NT; ++n) {
       float p[TS][2][X], top[X];
@@ -341,7 +430,7 @@ __global__ void __launch_bounds__(kAttendThreads, DB * NT == 1 ? 6 : 1) k_attend
         for (int u = 0; u < TS; ++u)
 #pragma unroll
           for (int r = 0; r < 2; ++r) {
-            p[u][r][x] = slot0 + g + 16 * u + 8 * r < last ? s[u][n][2 * r + x] * a.scale2 : -INFINITY;
+            p[u][r][x] = slot0 + g + 16 * u + 8 * r < last ? s[u][n][2 * r + x] * scale2[n][x] : -INFINITY;
             top[x] = fmaxf(top[x], p[u][r][x]);
           }
 #pragma unroll
@@ -361,58 +450,89 @@ __global__ void __launch_bounds__(kAttendThreads, DB * NT == 1 ? 6 : 1) k_attend
               o[n][i][w][x] *= keep;
               o[n][i][w][2 + x] *= keep;
             }
+          if constexpr (INT4)
+#pragma unroll
+            for (int j = 0; j < J; ++j) olow[n][j][x] *= keep;
         }
       }
 #pragma unroll
       for (int u = 0; u < TS; ++u)
 #pragma unroll
         for (int r = 0; r < 2; ++r) {
+          unsigned vs[SW];
+          if constexpr (INT4)
+            read_scales(tile + 2 * kSlots * row_apart + kSlots * scale_bytes, 16 * u + 8 * r + g, vs);
 #pragma unroll
           for (int x = 0; x < X; ++x) {
             const float ref = m[n][x] == -INFINITY ? 0.f : m[n][x] - kLift;
             p[u][r][x] = exp2_fast(p[u][r][x] - ref);
             l[n][x] += p[u][r][x];
           }
-          pf[u][n][r] = transpose8x8(pack2((PT*)nullptr, p[u][r][0], ONE ? 0.f : p[u][r][X - 1]));
+          if constexpr (INT4) {
+#pragma unroll
+            for (int j = 0; j < J; ++j) {
+              const float scale = group_scale(vs[j]), middle = fmaf(7.5f, scale, group_lowest(vs[j]));
+              const unsigned w = pack2((PT*)nullptr, p[u][r][0] * (scale * kValueLift),
+                                       ONE ? 0.f : p[u][r][X - 1] * (scale * kValueLift));
+              pf[u][n][j][r] = transpose8x8(w);
+#pragma unroll
+              for (int x = 0; x < X; ++x) {
+                const float rounded = x ? group_lowest(w) : group_scale(w);  // the halves of a word of two bf16
+                olow[n][j][x] = fmaf(p[u][r][x], middle, fmaf(rounded, -7.5f / kValueLift, olow[n][j][x]));
+              }
+            }
+          } else {
+            pf[u][n][0][r] = transpose8x8(pack2((PT*)nullptr, p[u][r][0], ONE ? 0.f : p[u][r][X - 1]));
+          }
         }
     }
 
     // O^T += V^T P^T
 #pragma unroll
     for (int u = 0; u < TS; ++u) {
-      unsigned scale[2], lowest[2];
       if constexpr (INT4) {
-        group_operands<PT>(vs[u][0], vs[u][1], scale[0], lowest[0]);
-        group_operands<PT>(vs[u][2], vs[u][3], scale[1], lowest[1]);
-      }
 #pragma unroll
-      for (int i = 0; i < DB; ++i)
+        for (int j = 0; j < J; ++j) {
+          // slots (2 t, 2 t + 1) and (2 t + 8, 2 t + 9) side by side; rows g and g + 8 of an m-tile: an even and an
+          // odd nibble
+          if (!FULL && j >= groups) break;
+          const char* p = tile + (kSlots + 16 * u + 2 * t) * row_apart + j * 16 + g * 2;
+          auto half = [&](int ahead) { return (unsigned)*reinterpret_cast<const unsigned short*>(p + ahead * row_apart); };
+          unsigned c0[4], c1[4];
+          code_steps(__byte_perm(half(0), half(1), 0x5410), c0);
+          code_steps(__byte_perm(half(8), half(9), 0x5410), c1);
 #pragma unroll
-        for (int w = 0; w < 4; ++w) {
-          unsigned c[4];
-          if constexpr (INT4) {
-            // slots (2 t, 2 t + 1) and (2 t + 8, 2 t + 9) side by side: a nibble of both halves is one column's pair
+          for (int n = 0; n < NT; ++n)
 #pragma unroll
-            for (int r = 0; r < 2; ++r) {
-              const unsigned y = __byte_perm(vf[u][2 * r][i], vf[u][2 * r + 1][i], w < 2 ? 0x5410 : 0x7632);
-              c[2 * r] = decode_pair<PT>(y, 2 * (w & 1), scale[r], lowest[r]);
-              c[2 * r + 1] = decode_pair<PT>(y, 2 * (w & 1) + 1, scale[r], lowest[r]);
-            }
-          } else {
-#pragma unroll
-            for (int r = 0; r < 2; ++r) {
-              c[2 * r] = __byte_perm(vf[u][2 * r][4 * i + w], vf[u][2 * r + 1][4 * i + w], 0x5410);
-              c[2 * r + 1] = __byte_perm(vf[u][2 * r][4 * i + w], vf[u][2 * r + 1][4 * i + w], 0x7632);
-            }
-          }
-#pragma unroll
-          for (int n = 0; n < NT; ++n) mma<PT>(o[n][i][w], c[0], c[1], c[2], c[3], pf[u][n][0], pf[u][n][1]);
+            for (int w = 0; w < 2; ++w)
+              mma<PT>(o[n][j / 2][2 * (j & 1) + w], c0[2 * w], c0[2 * w + 1], c1[2 * w], c1[2 * w + 1], pf[u][n][j][0],
+                      pf[u][n][j][1]);
         }
+      } else {
+#pragma unroll
+        for (int i = 0; i < DB; ++i)
+#pragma unroll
+          for (int w = 0; w < 4; ++w) {
+            unsigned c[4];
+#pragma unroll
+            for (int r = 0; r < 2; ++r) {
+              c[2 * r] = __byte_perm(vf[2 * r][4 * i + w], vf[2 * r + 1][4 * i + w], 0x5410);
+              c[2 * r + 1] = __byte_perm(vf[2 * r][4 * i + w], vf[2 * r + 1][4 * i + w], 0x7632);
+            }
+#pragma unroll
+            for (int n = 0; n < NT; ++n) mma<PT>(o[n][i][w], c[0], c[1], c[2], c[3], pf[u][n][0][0], pf[u][n][0][1]);
+          }
+      }
     }
-    if (next < last) fetch_v(next);
+    if constexpr (!INT4)
+      if (next < last) fetch_v(next);
   }
 
-  // this warp's part into shared memory, columns in their own order
+  // this warp's part into shared memory, columns in their own order (its own ring lies elsewhere than its part)
+  if constexpr (INT4) {
+    copy_wait<0>();
+    __syncthreads();
+  }
 #pragma unroll
   for (int n = 0; n < NT; ++n)
 #pragma unroll
@@ -421,17 +541,29 @@ __global__ void __launch_bounds__(kAttendThreads, DB * NT == 1 ? 6 : 1) k_attend
       float sum = l[n][x];
 #pragma unroll
       for (int d = 4; d < 32; d *= 2) sum += __shfl_xor_sync(0xffffffffu, sum, d);
+      if constexpr (INT4)
+#pragma unroll
+        for (int j = 0; j < J; ++j)
+#pragma unroll
+          for (int d = 4; d < 32; d *= 2) olow[n][j][x] += __shfl_xor_sync(0xffffffffu, olow[n][j][x], d);
       if (h >= nheads) continue;
       if (g == 0) {
         sh_m[warp][h] = m[n][x];
         sh_l[warp][h] = sum;
       }
 #pragma unroll
-      for (int i = 0; i < DB; ++i) {
-        float* to = &sh_o[warp][h][INT4 ? g * 8 * DB + 8 * i : i * 64 + g * 8];
+      for (int i = 0; i < DB; ++i)
 #pragma unroll
-        for (int w = 0; w < 4; ++w) *reinterpret_cast<float2*>(to + 2 * w) = make_float2(o[n][i][w][x], o[n][i][w][2 + x]);
-      }
+        for (int w = 0; w < 4; ++w) {
+          float2 v = make_float2(o[n][i][w][x], o[n][i][w][2 + x]);
+          int d = i * 64 + g * 8 + 2 * w;
+          if constexpr (INT4) {  // group 2 i + w / 2, columns 4 g + 2 (w % 2), + 1 (an odd nibble: 16 times as large)
+            const float low = olow[n][2 * i + w / 2][x];
+            v = make_float2(fmaf(v.x, kValueDrop, low), fmaf(v.y, kValueDrop * 0.0625f, low));
+            d = i * 64 + (w / 2) * 32 + g * 4 + 2 * (w & 1);
+          }
+          *reinterpret_cast<float2*>(&sh_o[warp][h][d]) = v;
+        }
     }
   __syncthreads();
   for (int e = threadIdx.x; e < nheads * dim; e += kAttendThreads) {
@@ -614,11 +746,18 @@ int splits_of(const st_cache* c, int heads) {
   return (int)std::min<long long>(std::max<long long>({fill, even, 1}), kMaxSplits);
 }
 
+template <typename T, int DB, int NT, bool INT4, bool FULL, bool ONE>
+void launch_one(const AttendArgs& a, dim3 grid, cudaStream_t s) {
+  constexpr int kBytes = AttendSmem<DB, NT, INT4>::kBytes;
+  if (kBytes > 40 * 1024)  // above what a launch may ask for by itself, with the static arrays
+    cudaFuncSetAttribute(k_attend_mma<T, DB, NT, INT4, FULL, ONE>, cudaFuncAttributeMaxDynamicSharedMemorySize, kBytes);
+  k_attend_mma<T, DB, NT, INT4, FULL, ONE><<<grid, kAttendThreads, kBytes, s>>>(a);
+}
 template <typename T, int DB, bool INT4, bool FULL>
 void launch_mma(const AttendArgs& a, int per, dim3 grid, cudaStream_t s) {
-  if (a.group == 1) k_attend_mma<T, DB, 1, INT4, FULL, true><<<grid, kAttendThreads, 0, s>>>(a);
-  else if (per == 8) k_attend_mma<T, DB, 1, INT4, FULL, false><<<grid, kAttendThreads, 0, s>>>(a);
-  else if constexpr (DB < 4) k_attend_mma<T, DB, 2, INT4, FULL, false><<<grid, kAttendThreads, 0, s>>>(a);
+  if (a.group == 1) launch_one<T, DB, 1, INT4, FULL, true>(a, grid, s);
+  else if (per == 8) launch_one<T, DB, 1, INT4, FULL, false>(a, grid, s);
+  else if constexpr (DB < 4) launch_one<T, DB, 2, INT4, FULL, false>(a, grid, s);
 }
 template <typename T, bool INT4>
 void launch_mma(const AttendArgs& a, int per, dim3 grid, cudaStream_t s) {

@@ -12,11 +12,12 @@ Attention: o = sum_j p_j v_j / sum_j p_j.
   * kernels that multiply weights and values as 16-bit operands round each weight
     once: u(T), or in fp16 2^-32 of the largest weight where that is more (they
     are held at least 2^7 times larger, and fp16 steps by 2^-24 at its low end).
-  * 4-bit rows are rounded to 16-bit operands: a key to T, which moves a logit by
-    u(T) scale sum|q k| more, a value and its weight to bf16, u(bf16) each.
+    4-bit caches fold a group's scale into the weight first and round to bf16: u(bf16).
+  * a 4-bit row enters as scale * code and lowest apart: its |k| and |v| above are
+    15 scale + |lowest|, an upper bound of both parts.
   * sums of n terms in up to n / 8 + 64 steps a chain: (n / 8 + 64) F.
   * the result is rounded to T.
-  |got - o| <= u(T) |o| + (1 + u(T)) (2 w + u(P) + u(V) + 2 (n / 8 + 64) F) sum p |v| / sum p + tiny(T) (+ n 2^-32 max|v|)
+  |got - o| <= u(T) |o| + (1 + u(T)) (2 w + u(P) + 2 (n / 8 + 64) F) sum p |v| / sum p + tiny(T) (+ n 2^-32 max|v|)
 """
 from __future__ import annotations
 
@@ -32,11 +33,11 @@ def unit(dtype):
     return torch.finfo(dtype).eps / 2
 
 
-def attention(q, k, v, see, scale, dtype, four=False):
+def attention(q, k, v, see, scale, dtype, sizes=None):
     """q [H, n, D], k and v [H, m, D] in float64, see [n, m] (or [H, n, m]):
-    the result and its bound. A row that sees nothing is 0, exactly. ``four``:
-    the rows were held in 4 bits."""
-    u, half = unit(dtype), unit(torch.bfloat16)
+    the result and its bound. A row that sees nothing is 0, exactly. ``sizes``:
+    the bounds on |k| and |v| of 4-bit rows."""
+    k_size, v_size = sizes or (k.abs(), v.abs())
     see = see.expand(q.shape[0], -1, -1)
     seen_any = see.any(-1, keepdim=True)
     logits = torch.where(see, q @ k.transpose(1, 2) * scale, -math.inf)
@@ -46,15 +47,16 @@ def attention(q, k, v, see, scale, dtype, four=False):
     # a masked value never counts, whatever it is: 0 * inf is left out by hand
     finite = torch.isfinite(v).all(-1)
     clean = torch.where(finite[..., None], v, 0.0)
-    out, size = p @ clean / total, p @ clean.abs() / total
+    clean_size = torch.where(finite[..., None], v_size, 0.0)
+    out, size = p @ clean / total, p @ clean_size / total
     spread = torch.where(see, (logits - top).abs(), 0.0).amax(-1, keepdim=True)
-    products = torch.where(see, q.abs() @ k.abs().transpose(1, 2) * abs(scale), 0.0).amax(-1, keepdim=True)
-    w = 2 * (((q.shape[-1] + 4) * F + (u if four else 0.0)) * products + 2 * F * spread) + 2.0 ** -20
+    products = torch.where(see, q.abs() @ k_size.transpose(1, 2) * abs(scale), 0.0).amax(-1, keepdim=True)
+    w = 2 * ((q.shape[-1] + 4) * F * products + 2 * F * spread) + 2.0 ** -20
     n = see.sum(-1, keepdim=True)
-    up = 2 * half if four else u
+    u, up = unit(dtype), unit(torch.bfloat16 if sizes else dtype)
     bound = u * out.abs() + (1 + u) * (2 * w + up + 2 * (n / 8 + 64) * F) * size + TINY[dtype]
-    if dtype == torch.float16 and not four:
-        bound = bound + n * 2.0 ** -32 * clean.abs().amax()
+    if dtype == torch.float16 and not sizes:
+        bound = bound + n * 2.0 ** -32 * clean_size.amax()
     return out, torch.where(seen_any, bound, 0.0)
 
 

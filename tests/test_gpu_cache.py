@@ -31,18 +31,20 @@ def starts_of(sizes, offset=0):
 
 
 def filled_cache(g, streams, heads, window, dim, sinks, mode, dtype=torch.bfloat16):
-    """(keys, values, key_scales, value_scales) and the float64 values they stand for."""
+    """(keys, values, key_scales, value_scales) and the float64 values they stand for
+    (4-bit: and the bounds of their sizes)."""
     rows = (streams, heads, sinks + window)
     if mode != "int4":
         k, v = (normal(g, *rows, dim, dtype=TYPES[mode]) for _ in range(2))
         return (k, v, None, None), (k.double(), v.double())
-    packed, scales, held = [], [], []
+    packed, scales, held, sizes = [], [], [], []
     for _ in range(2):
         codes, s, low = ref.quantise(normal(g, *rows, dim))
         packed.append(ref.pack(codes))
         scales.append(torch.stack([s, low], -1))
         held.append(ref.unpack(packed[-1], scales[-1]))
-    return (*packed, *scales), tuple(held)
+        sizes.append((15 * s.double() + low.double().abs()).repeat_interleave(32, -1))
+    return (*packed, *scales), (*held, *sizes)
 
 
 def scales_of(cache):
@@ -192,7 +194,7 @@ def test_four_bit_groups_at_their_limits():
 def test_unpack_matches_the_definition(dtype):
     g = generator(11)
     cache, held = filled_cache(g, 3, 2, 37, 96, 1, "int4")
-    for got, want in zip(ops.unpack_cache(*cache[:2], dtype=dtype, **scales_of(cache)), held):
+    for got, want in zip(ops.unpack_cache(*cache[:2], dtype=dtype, **scales_of(cache)), held[:2]):
         # lowest + scale * code: the product is exact in fp32 (8 + 4 bits), one rounding of the sum, one to the type
         ref.check(got, want, want.abs() * (ref.unit(dtype) + 2 * ref.F) + ref.TINY[dtype])
 
@@ -226,13 +228,14 @@ ATTEND = [
 ]
 
 
-def attend_reference(q, held, positions, scale, dtype, four=False):
+def attend_reference(q, held, positions, scale, dtype):
     outs, bounds = [], []
     for s, p in enumerate(positions):
         slots, kv = held[0].shape[2], held[0].shape[1]
         see = (torch.arange(slots, device="cuda") <= p)[None, None]
         group = q.shape[1] // kv
-        o, b = ref.attention(q[s].double().unflatten(0, (kv, group)), held[0][s], held[1][s], see.expand(kv, group, -1), scale, dtype, four)
+        sizes = (held[2][s], held[3][s]) if len(held) == 4 else None
+        o, b = ref.attention(q[s].double().unflatten(0, (kv, group)), held[0][s], held[1][s], see.expand(kv, group, -1), scale, dtype, sizes)
         outs.append(o.flatten(0, 1))
         bounds.append(b.flatten(0, 1))
     return torch.stack(outs), torch.stack(bounds)
@@ -248,7 +251,7 @@ def test_cache_attention_matches_the_definition(case):
     positions = torch.tensor(at, dtype=torch.int64, device="cuda")
     for scale in (None, 0.7):
         got = ops.cache_attention(q, *cache[:2], positions, scale=scale, **scales_of(cache))
-        want, bound = attend_reference(q, held, at, dim ** -0.5 if scale is None else scale, dtype, mode == "int4")
+        want, bound = attend_reference(q, held, at, dim ** -0.5 if scale is None else scale, dtype)
         ref.check(got, want, bound, f"scale {scale}")
 
 
@@ -269,7 +272,7 @@ def test_unseen_slots_do_not_count_whatever_they_hold(mode):
     q = normal(g, 4, 4, 64, dtype=dtype)
     got = ops.cache_attention(q, *cache[:2], torch.tensor(at, device="cuda"), **scales_of(cache))
     clean = [torch.where((torch.arange(150, device="cuda")[None, :] <= torch.tensor(at, device="cuda")[:, None])[:, None, :, None], h, 0.0) for h in held]
-    want, bound = attend_reference(q, clean, at, 0.125, dtype, mode == "int4")
+    want, bound = attend_reference(q, clean, at, 0.125, dtype)
     ref.check(got, want, bound)
 
 
@@ -288,7 +291,7 @@ def test_non_finite_rows_reach_their_own_heads_only(mode):
     q = normal(g, 3, 4, 64, dtype=dtype)
     at = [69, 69, 69]
     got = ops.cache_attention(q, *cache[:2], torch.tensor(at, device="cuda"), **scales_of(cache))
-    want, bound = attend_reference(q, held, at, 0.125, dtype, mode == "int4")
+    want, bound = attend_reference(q, held, at, 0.125, dtype)
     assert torch.isnan(got[1, :2]).all() and torch.isnan(got[2, 2:]).all()
     for s, h in ((0, slice(0, 4)), (1, slice(2, 4)), (2, slice(0, 2))):
         ref.check(got[s, h], want[s, h], bound[s, h])
