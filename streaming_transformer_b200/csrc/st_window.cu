@@ -1,10 +1,11 @@
 // st_window.cu -- causal attention of packed sequences with a sliding window
 // and sinks (st_window_attention).
 //
-// Two kernels. k_window_tiles: 16-bit rows of up to 128 columns, on tcgen05.
-// k_window_rows: a few lanes walk the keys that one query row of one head sees,
-// in fp32; it serves fp32 rows (there is no fp32 tensor product), wider rows,
-// and scales that are not positive.
+// Three kernels. k_window_tiles: 16-bit rows of up to 128 columns, on tcgen05.
+// k_window_fp32: fp32 rows of up to 128 columns, tiled for the fp32 units (there
+// is no fp32 tensor product). k_window_rows: a few lanes walk the keys that one
+// query row of one head sees; it serves the rest (wider rows, 16-bit rows with a
+// scale that is not positive).
 //
 // k_window_tiles. A CTA takes 128 consecutive rows of the packed input, one TMEM
 // lane each, and one head. Rows may belong to several sequences: the keys that
@@ -19,10 +20,11 @@
 // last time; P then stays below 2^8, which both 16-bit types hold, and l and O
 // share the reference, so the quotient is exact.
 //
-// Only tiles at an edge of somebody's window are masked. A masked weight is 0,
-// but 0 times an infinite or NaN value is not: in masked tiles the rows of V are
-// looked at, and if any is not finite (only then) the CTA does its rows again
-// with the row kernel's code, which never reads what a row does not see.
+// A warp masks only the blocks at an edge of one of its rows' windows, and skips
+// those that none of its rows sees. A masked weight is 0, but 0 times an infinite
+// or NaN value is NaN: when a result of the tile is not finite (only then), the
+// CTA does its rows again with the row kernel's code, which never reads what a
+// row does not see. k_window_fp32 does the same.
 //
 // Every wait has a time limit; a CTA that ran into one writes NaN.
 #include <cuda.h>
@@ -202,6 +204,32 @@ __device__ __forceinline__ float exp2_fast(float x) {
   return y;
 }
 
+__device__ __forceinline__ float max3(float a, float b, float c) {
+  float y;
+  asm("max.f32 %0, %1, %2, %3;" : "=f"(y) : "f"(a), "f"(b), "f"(c));
+  return y;
+}
+// Two fp32 operations in one instruction.
+__device__ __forceinline__ float2 fma2(float2 a, float2 b, float2 c) {
+  unsigned long long x, y, z, d;
+  asm("mov.b64 %0, {%1, %2};" : "=l"(x) : "f"(a.x), "f"(a.y));
+  asm("mov.b64 %0, {%1, %2};" : "=l"(y) : "f"(b.x), "f"(b.y));
+  asm("mov.b64 %0, {%1, %2};" : "=l"(z) : "f"(c.x), "f"(c.y));
+  asm("fma.rn.f32x2 %0, %1, %2, %3;" : "=l"(d) : "l"(x), "l"(y), "l"(z));
+  float2 r;
+  asm("mov.b64 {%0, %1}, %2;" : "=f"(r.x), "=f"(r.y) : "l"(d));
+  return r;
+}
+__device__ __forceinline__ float2 add2(float2 a, float2 b) {
+  unsigned long long x, y, d;
+  asm("mov.b64 %0, {%1, %2};" : "=l"(x) : "f"(a.x), "f"(a.y));
+  asm("mov.b64 %0, {%1, %2};" : "=l"(y) : "f"(b.x), "f"(b.y));
+  asm("add.rn.f32x2 %0, %1, %2;" : "=l"(d) : "l"(x), "l"(y));
+  float2 r;
+  asm("mov.b64 {%0, %1}, %2;" : "=f"(r.x), "=f"(r.y) : "l"(d));
+  return r;
+}
+
 // Bits lo .. hi of a 32-bit word (either end may lie outside it).
 __device__ __forceinline__ unsigned bit_range(int lo, int hi) {
   lo = max(lo, 0);
@@ -220,9 +248,10 @@ struct TileKeys {
     return block < sink_blocks ? start + block * kBlockRows : low + (block - sink_blocks) * kBlockRows;
   }
 };
+template <int ROWS>
 __device__ __forceinline__ bool tile_keys(const WindowArgs& a, int tile, TileKeys& t) {
-  t.r0 = tile * kTileRows;
-  t.r1 = (int)min((long long)a.rows, (long long)t.r0 + kTileRows) - 1;
+  t.r0 = tile * ROWS;
+  t.r1 = (int)min((long long)a.rows, (long long)t.r0 + ROWS) - 1;
   if (a.starts) {
     t.r0 = max(t.r0, clamp_row(a.starts[0], a.rows));
     t.r1 = min(t.r1, clamp_row(a.starts[a.sequences], a.rows) - 1);
@@ -237,6 +266,27 @@ __device__ __forceinline__ bool tile_keys(const WindowArgs& a, int tile, TileKey
   return true;
 }
 
+// The keys one row sees, as bits of a block of 32 key rows.
+struct RowLimits {
+  int row, start, low, sink_last;  // start -1: none
+  __device__ void set(const WindowArgs& a, const TileKeys& t, int r) {
+    row = r;
+    start = r >= t.r0 && r <= t.r1 ? sequence_start(a, r) : -1;
+    low = (int)max((long long)start, (long long)r - a.window + 1);
+    sink_last = (int)min((long long)r, (long long)start + a.sinks - 1);
+  }
+  __device__ unsigned bits(const TileKeys& t, int block) const {
+    if (start < 0 || block >= t.blocks) return 0;
+    const int base = t.base(block);
+    if (block < t.sink_blocks) return start == t.start ? bit_range(0, min(sink_last, t.sink_end - 1) - base) : 0u;
+    return bit_range(low - base, row - base) | bit_range(start - base, sink_last - base);
+  }
+};
+// First row that is inside every row's window; blocks from it up to the tile's first row need no mask.
+__device__ __forceinline__ int common_low(const WindowArgs& a, const TileKeys& t) {
+  return (int)max((long long)sequence_start(a, t.r1), (long long)t.r1 - a.window + 1);
+}
+
 template <typename T, int DP>
 __global__ void __launch_bounds__(kTileThreads, DP == 64 ? 3 : 2)
     k_window_tiles(const WindowArgs a, const __grid_constant__ TileMaps maps) {
@@ -249,7 +299,7 @@ __global__ void __launch_bounds__(kTileThreads, DP == 64 ? 3 : 2)
   const int warp = threadIdx.x >> 5;
   const int h = blockIdx.x % a.heads, tile = gridDim.x / a.heads - 1 - blockIdx.x / a.heads;  // most keys first
   TileKeys keys;
-  if (!tile_keys(a, tile, keys)) return;
+  if (!tile_keys<kTileRows>(a, tile, keys)) return;
   unsigned char* smem = raw + ((1024u - (smem_addr(raw) & 1023u)) & 1023u);
   unsigned char *sq = smem, *sk = sq + G::kQBytes, *sv = sk + G::kStages * G::kKvBytes;
   if (threadIdx.x == 0) {
@@ -340,13 +390,10 @@ __global__ void __launch_bounds__(kTileThreads, DP == 64 ? 3 : 2)
   } else {
     const int row = tile * kTileRows + threadIdx.x, lane = threadIdx.x & 31;
     const unsigned my_s = tm_s + ((unsigned)(warp * 32) << 16), my_o = tm_o + ((unsigned)(warp * 32) << 16);
-    const bool inside = row >= keys.r0 && row <= keys.r1;
-    const int start = inside ? sequence_start(a, row) : -1;
-    const int low = (int)max((long long)start, (long long)row - a.window + 1);
-    const int sink_last = (int)min((long long)row, (long long)start + a.sinks - 1);
-    // the tile's common part: keys every row sees lie in [all_low, r0]
-    const int start_last = sequence_start(a, keys.r1);
-    const int all_low = (int)max((long long)start_last, (long long)keys.r1 - a.window + 1);
+    RowLimits limits;
+    limits.set(a, keys, row);
+    const bool inside = limits.start >= 0;
+    const int all_low = common_low(a, keys);
     const float c = a.scale * 1.4426950408889634f;
     float m = -INFINITY, l = 0.f;  // m: reference of the weights, in units of S
     bool ok = true;
@@ -356,26 +403,32 @@ __global__ void __launch_bounds__(kTileThreads, DP == 64 ? 3 : 2)
                          keys.base(b0 + nb - 1) + kBlockRows - 1 <= keys.r0;
       if (!(ok = wait(&s_full, i))) break;
       tc_fence_after();
-      auto masked = [&](int b, float (&x)[32]) {
-        if (plain) return;
-        const int base = keys.base(b0 + b);
-        unsigned bits = 0;
-        if (start >= 0) {
-          if (b0 + b < keys.sink_blocks)
-            bits = start == keys.start ? bit_range(0, min(sink_last, keys.sink_end - 1) - base) : 0u;
-          else
-            bits = bit_range(low - base, row - base) | bit_range(start - base, sink_last - base);
-        }
+      // the blocks: bits of the keys this row sees; a block that no row of the warp sees is left out
+      unsigned seen[G::kBlocks];
+      bool some[G::kBlocks], edge[G::kBlocks];
 #pragma unroll
-        for (int e = 0; e < 32; ++e) x[e] = (bits >> e) & 1u ? x[e] : -INFINITY;
-      };
-      float x[32], top = -INFINITY;
-      for (int b = 0; b < nb; ++b) {
-        tmem_ld32(my_s + b * 32, x);
-        masked(b, x);
-#pragma unroll
-        for (int e = 0; e < 32; ++e) top = fmaxf(top, x[e]);
+      for (int b = 0; b < G::kBlocks; ++b) {
+        seen[b] = plain ? ~0u : b < nb ? limits.bits(keys, b0 + b) : 0u;
+        some[b] = plain || __any_sync(0xffffffffu, seen[b] != 0u);
+        edge[b] = !plain && __any_sync(0xffffffffu, seen[b] != ~0u);
       }
+      auto load = [&](int b, float (&x)[32]) {
+        tmem_ld32(my_s + b * 32, x);
+        if (edge[b])
+#pragma unroll
+          for (int e = 0; e < 32; ++e) x[e] = (seen[b] >> e) & 1u ? x[e] : -INFINITY;
+      };
+      // At 64 keys the tile stays in registers between the passes, at 128 it is read again.
+      constexpr bool kKeep = G::kBlocks <= 2;
+      float x[kKeep ? G::kBlocks : 1][32], top = -INFINITY;
+#pragma unroll
+      for (int b = 0; b < G::kBlocks; ++b)
+        if (some[b]) {
+          float(&y)[32] = x[kKeep ? b : 0];
+          load(b, y);
+#pragma unroll
+          for (int e = 0; e < 32; e += 2) top = max3(top, y[e], y[e + 1]);
+        }
       // a new reference only when the old one is too low; exp2(8) is the most a weight can be
       const bool grow = top > m && !((top - m) * c <= 8.f);
       if (__any_sync(0xffffffffu, grow)) {
@@ -396,35 +449,29 @@ __global__ void __launch_bounds__(kTileThreads, DP == 64 ? 3 : 2)
       }
       // fp16 weights 2^7 higher, up to 2^15, away from its denormals
       const float ref = m == -INFINITY ? 0.f : m * c - (std::is_same<T, __half>::value ? 7.f : 0.f);
-      for (int b = 0; b < nb; ++b) {
-        tmem_ld32(my_s + b * 32, x);
-        masked(b, x);
+      const float2 c2 = make_float2(c, c), ref2 = make_float2(-ref, -ref);
+      float2 sum = make_float2(0.f, 0.f);
+#pragma unroll
+      for (int b = 0; b < G::kBlocks; ++b) {
+        if (b >= nb) break;
         unsigned p[16];
+        if (some[b]) {
+          float(&y)[32] = x[kKeep ? b : 0];
+          if (!kKeep) load(b, y);
 #pragma unroll
-        for (int e = 0; e < 32; ++e) {
-          x[e] = exp2_fast(fmaf(x[e], c, -ref));
-          l += x[e];
+          for (int e = 0; e < 16; ++e) {
+            float2 w = fma2(make_float2(y[2 * e], y[2 * e + 1]), c2, ref2);
+            w = make_float2(exp2_fast(w.x), exp2_fast(w.y));
+            sum = add2(sum, w);
+            p[e] = pack2((T*)nullptr, w.x, w.y);
+          }
+        } else {
+#pragma unroll
+          for (int e = 0; e < 16; ++e) p[e] = 0u;
         }
-#pragma unroll
-        for (int e = 0; e < 16; ++e) p[e] = pack2((T*)nullptr, x[2 * e], x[2 * e + 1]);
         tmem_st16(my_s + b * 16, p);
       }
-      if (!plain) {
-        // a value that is not finite would reach rows that do not see it
-        const int s = i % G::kStages;
-        if (!(ok = wait(&v_full[s], i / G::kStages))) break;
-        const unsigned top_bits = std::is_same<T, __half>::value ? 0x7c007c00u : 0x7f807f80u;
-        const unsigned one = std::is_same<T, __half>::value ? 0x04000400u : 0x00800080u;  // carries into bit 15 or 31
-        unsigned bad = 0;
-        for (int p = 0; p < G::kPanels; ++p) {
-          const uint4* v = reinterpret_cast<const uint4*>(sv + s * G::kKvBytes + p * G::kKeys * 128);
-          for (int e = threadIdx.x; e < nb * kBlockRows * 8; e += 128) {
-            const uint4 u = v[e];
-            bad |= ((u.x & top_bits) + one) | ((u.y & top_bits) + one) | ((u.z & top_bits) + one) | ((u.w & top_bits) + one);
-          }
-        }
-        if (bad & 0x80008000u) sh_slow = 1;
-      }
+      l += sum.x + sum.y;
       tmem_st_wait();
       tc_fence_before();
       __syncwarp();
@@ -434,23 +481,28 @@ __global__ void __launch_bounds__(kTileThreads, DP == 64 ? 3 : 2)
     tc_fence_after();
     const bool good = __all_sync(0xffffffffu, ok);
     if (good || inside) {
+      bool odd = false;  // a result that is not finite
       T* to = static_cast<T*>(a.out) + (long long)row * a.o_row + h * a.o_head;
 #pragma unroll
       for (int d = 0; d < DP; d += 32) {
         float o[32];
         if (good) tmem_ld32(my_o + d, o);
         const float inv = good ? 1.f / l : NAN;
-        if (inside && start >= 0)
+        if (inside)
 #pragma unroll
           for (int e = 0; e < 32; e += 8) {
             if (d + e < a.head_dim) {
               float r[8];
 #pragma unroll
-              for (int w = 0; w < 8; ++w) r[w] = good ? o[e + w] * inv : NAN;
+              for (int w = 0; w < 8; ++w) {
+                r[w] = good ? o[e + w] * inv : NAN;
+                odd |= !(fabsf(r[w]) < INFINITY);
+              }
               store8(to + d + e, r);
             }
           }
       }
+      if (odd) sh_slow = 1;
     }
     tc_fence_before();
   }
@@ -462,6 +514,172 @@ __global__ void __launch_bounds__(kTileThreads, DP == 64 ? 3 : 2)
     for (int r = keys.r0 + threadIdx.x / kLanes; r <= keys.r1; r += 128 / kLanes) {
       const int start = sequence_start(a, r);
       if (start >= 0) window_row<T, kLanes>(a, r, start, h, threadIdx.x % kLanes, row_mask<kLanes>());
+    }
+  }
+}
+
+// ---------------------------------------------------------------- fp32 tiles
+// 32 query rows of one head by 128 threads; thread (ty, tx) of 8 x 16 has rows
+// 4 ty .. + 3 of everything, keys tx + 16 i of a 64-key tile in S, columns
+// 64 i + 4 tx .. + 3 of O. 16 multiply-adds for each 32 bytes read from shared
+// memory, rows padded by 16 bytes against bank conflicts. Key rows of the next
+// tile load under the second product, value rows under the first.
+constexpr int kFp32Rows = 32, kFp32Keys = 64, kFp32Threads = 128;
+
+template <int DP>
+struct Fp32Tiles {
+  static constexpr int kRow = DP + 4, kPRow = kFp32Keys + 4;
+  static constexpr int kFloats = (kFp32Rows + 2 * kFp32Keys) * kRow + kFp32Rows * kPRow;
+  static constexpr int kSmem = kFloats * 4;
+};
+
+__device__ __forceinline__ void copy16(float* dst, const float* src, bool in) {
+  asm volatile("cp.async.cg.shared.global [%0], [%1], 16, %2;" ::"r"(smem_addr(dst)), "l"(src), "r"(in ? 16 : 0) : "memory");
+}
+
+template <int DP>
+__global__ void __launch_bounds__(kFp32Threads) k_window_fp32(const WindowArgs a) {
+  using G = Fp32Tiles<DP>;
+  extern __shared__ float4 dynamic[];
+  float* sq = reinterpret_cast<float*>(dynamic);
+  float *sk = sq + kFp32Rows * G::kRow, *sv = sk + kFp32Keys * G::kRow, *sp = sv + kFp32Keys * G::kRow;
+  __shared__ int sh_slow;
+  const int h = blockIdx.x % a.heads, tile = gridDim.x / a.heads - 1 - blockIdx.x / a.heads, kv = h / (a.heads / a.kv_heads);
+  TileKeys keys;
+  if (!tile_keys<kFp32Rows>(a, tile, keys)) return;
+  const int ty = threadIdx.x / 16, tx = threadIdx.x % 16;
+  if (threadIdx.x == 0) sh_slow = 0;
+  // rows of a block beyond the tile's last, and columns past head_dim, are zeros
+  auto copy_rows = [&](float* dst, const void* src, long long row_stride, long long head, int block0) {
+    const float* p = static_cast<const float*>(src) + head;
+    for (int e = threadIdx.x; e < kFp32Keys * (DP / 4); e += kFp32Threads) {
+      const int r = e / (DP / 4), c = e % (DP / 4), block = block0 + r / kBlockRows;
+      const int row = block < keys.blocks ? keys.base(block) + r % kBlockRows : a.rows;
+      const bool in = row < a.rows && c * 4 < a.head_dim;
+      copy16(dst + r * G::kRow + c * 4, p + (in ? row * row_stride + c * 4 : 0), in);
+    }
+    asm volatile("cp.async.commit_group;" ::: "memory");
+  };
+  {
+    const float* p = static_cast<const float*>(a.q) + h * a.q_head;
+    for (int e = threadIdx.x; e < kFp32Rows * (DP / 4); e += kFp32Threads) {
+      const int r = e / (DP / 4), c = e % (DP / 4);
+      const long long row = (long long)tile * kFp32Rows + r;
+      const bool in = row < a.rows && c * 4 < a.head_dim;
+      copy16(sq + r * G::kRow + c * 4, p + (in ? row * a.q_row + c * 4 : 0), in);
+    }
+  }
+  copy_rows(sk, a.k, a.k_row, kv * a.k_head, 0);
+  copy_rows(sv, a.v, a.v_row, kv * a.v_head, 0);
+
+  RowLimits limits[4];
+#pragma unroll
+  for (int r = 0; r < 4; ++r) limits[r].set(a, keys, tile * kFp32Rows + ty * 4 + r);
+  const int all_low = common_low(a, keys);
+  const float c = a.scale * 1.4426950408889634f;
+  float o[4][DP / 64][4] = {}, m[4], l[4] = {};
+#pragma unroll
+  for (int r = 0; r < 4; ++r) m[r] = -INFINITY;
+  for (int b0 = 0; b0 < keys.blocks; b0 += 2) {
+    const bool more = b0 + 2 < keys.blocks;
+    const bool plain = b0 >= keys.sink_blocks && b0 + 1 < keys.blocks && keys.base(b0) >= all_low &&
+                       keys.base(b0 + 1) + kBlockRows - 1 <= keys.r0;
+    asm volatile("cp.async.wait_group 1;" ::: "memory");  // queries and keys; the values may still be on their way
+    __syncthreads();
+    float s[4][4] = {};
+#pragma unroll 4
+    for (int d = 0; d < DP; d += 4) {
+      float4 q[4], k[4];
+#pragma unroll
+      for (int i = 0; i < 4; ++i) {
+        q[i] = *reinterpret_cast<const float4*>(sq + (ty * 4 + i) * G::kRow + d);
+        k[i] = *reinterpret_cast<const float4*>(sk + (tx + 16 * i) * G::kRow + d);
+      }
+#pragma unroll
+      for (int r = 0; r < 4; ++r)
+#pragma unroll
+        for (int i = 0; i < 4; ++i) {
+          s[r][i] = fmaf(q[r].x, k[i].x, s[r][i]);
+          s[r][i] = fmaf(q[r].y, k[i].y, s[r][i]);
+          s[r][i] = fmaf(q[r].z, k[i].z, s[r][i]);
+          s[r][i] = fmaf(q[r].w, k[i].w, s[r][i]);
+        }
+    }
+#pragma unroll
+    for (int r = 0; r < 4; ++r) {
+      const unsigned b[2] = {plain ? ~0u : limits[r].bits(keys, b0), plain ? ~0u : limits[r].bits(keys, b0 + 1)};
+      float top = m[r];
+#pragma unroll
+      for (int i = 0; i < 4; ++i) {
+        s[r][i] = (b[i / 2] >> (tx + 16 * (i & 1))) & 1u ? s[r][i] * c : -INFINITY;
+        top = fmaxf(top, s[r][i]);
+      }
+#pragma unroll
+      for (int d = 1; d < 16; d *= 2) top = fmaxf(top, __shfl_xor_sync(0xffffffffu, top, d));
+      const float ref = top == -INFINITY ? 0.f : top, keep = m[r] == -INFINITY ? 0.f : exp2_fast(m[r] - ref);
+      m[r] = top;
+      l[r] *= keep;
+#pragma unroll
+      for (int i = 0; i < 4; ++i) {
+        s[r][i] = exp2_fast(s[r][i] - ref);
+        l[r] += s[r][i];
+        sp[(ty * 4 + r) * G::kPRow + tx + 16 * i] = s[r][i];
+      }
+#pragma unroll
+      for (int i = 0; i < DP / 64; ++i)
+#pragma unroll
+        for (int e = 0; e < 4; ++e) o[r][i][e] *= keep;
+    }
+    __syncthreads();  // everybody is done with the keys
+    if (more) copy_rows(sk, a.k, a.k_row, kv * a.k_head, b0 + 2);
+    if (more) asm volatile("cp.async.wait_group 1;" ::: "memory");
+    else asm volatile("cp.async.wait_group 0;" ::: "memory");
+    __syncthreads();  // values and weights are there
+#pragma unroll 2
+    for (int j = 0; j < kFp32Keys; j += 4) {
+      float4 p[4];
+#pragma unroll
+      for (int r = 0; r < 4; ++r) p[r] = *reinterpret_cast<const float4*>(sp + (ty * 4 + r) * G::kPRow + j);
+#pragma unroll
+      for (int e = 0; e < 4; ++e)
+#pragma unroll
+        for (int i = 0; i < DP / 64; ++i) {
+          const float4 v = *reinterpret_cast<const float4*>(sv + (j + e) * G::kRow + i * 64 + tx * 4);
+#pragma unroll
+          for (int r = 0; r < 4; ++r) {
+            const float w = e == 0 ? p[r].x : e == 1 ? p[r].y : e == 2 ? p[r].z : p[r].w;
+            o[r][i][0] = fmaf(w, v.x, o[r][i][0]);
+            o[r][i][1] = fmaf(w, v.y, o[r][i][1]);
+            o[r][i][2] = fmaf(w, v.z, o[r][i][2]);
+            o[r][i][3] = fmaf(w, v.w, o[r][i][3]);
+          }
+        }
+    }
+    __syncthreads();  // everybody is done with the values and weights
+    if (more) copy_rows(sv, a.v, a.v_row, kv * a.v_head, b0 + 2);
+  }
+  bool odd = false;  // a result that is not finite
+#pragma unroll
+  for (int r = 0; r < 4; ++r) {
+#pragma unroll
+    for (int d = 1; d < 16; d *= 2) l[r] += __shfl_xor_sync(0xffffffffu, l[r], d);
+    if (limits[r].start < 0) continue;
+    float* to = static_cast<float*>(a.out) + (long long)limits[r].row * a.o_row + h * a.o_head;
+#pragma unroll
+    for (int i = 0; i < DP / 64; ++i)
+      if (i * 64 + tx * 4 < a.head_dim) {
+        const float4 v = make_float4(o[r][i][0] / l[r], o[r][i][1] / l[r], o[r][i][2] / l[r], o[r][i][3] / l[r]);
+        odd |= !(fabsf(v.x) < INFINITY && fabsf(v.y) < INFINITY && fabsf(v.z) < INFINITY && fabsf(v.w) < INFINITY);
+        *reinterpret_cast<float4*>(to + i * 64 + tx * 4) = v;
+      }
+  }
+  if (odd) sh_slow = 1;
+  __syncthreads();
+  if (sh_slow) {
+    constexpr int kLanes = DP / 8;
+    for (int r = keys.r0 + threadIdx.x / kLanes; r <= keys.r1; r += kFp32Threads / kLanes) {
+      const int start = sequence_start(a, r);
+      if (start >= 0) window_row<float, kLanes>(a, r, start, h, threadIdx.x % kLanes, row_mask<kLanes>());
     }
   }
 }
@@ -514,6 +732,16 @@ bool encode_rows(CUtensorMap* map, const st_rows& r, int mode, long long rows, i
                           CU_TENSOR_MAP_L2_PROMOTION_L2_256B, CU_TENSOR_MAP_FLOAT_OOB_FILL_NONE) == CUDA_SUCCESS;
 }
 
+template <int DP>
+cudaError_t launch_fp32(const WindowArgs& a, cudaStream_t s) {
+  const cudaError_t e =
+      cudaFuncSetAttribute(k_window_fp32<DP>, cudaFuncAttributeMaxDynamicSharedMemorySize, Fp32Tiles<DP>::kSmem);
+  if (e != cudaSuccess) return e;
+  const unsigned tiles = (unsigned)((a.rows + kFp32Rows - 1ll) / kFp32Rows);
+  k_window_fp32<DP><<<tiles * a.heads, kFp32Threads, Fp32Tiles<DP>::kSmem, s>>>(a);
+  return cudaSuccess;
+}
+
 template <typename T, int DP>
 cudaError_t launch_tiles(const WindowArgs& a, const TileMaps& maps, cudaStream_t s) {
   const cudaError_t e =
@@ -561,6 +789,13 @@ extern "C" int st_window_attention(const st_window* p, void* stream) {
   a.heads = p->heads; a.kv_heads = p->kv_heads; a.head_dim = p->head_dim;
   a.window = p->window; a.sinks = p->sinks; a.scale = p->scale;
   cudaStream_t s = static_cast<cudaStream_t>(stream);
+  if (p->mode == ST_MODE_FP32 && p->head_dim <= 128 && (p->rows + kFp32Rows - 1) / kFp32Rows * p->heads <= INT32_MAX) {
+    if ((rc = cache_cuda(p->head_dim <= 64 ? launch_fp32<64>(a, s) : launch_fp32<128>(a, s), "window attention: ")) != ST_OK) {
+      cudaGetLastError();  // reported here, so not left pending
+      return rc;
+    }
+    return cache_cuda(cudaGetLastError(), "window attention launch: ");
+  }
   TileMaps maps;
   const long long ctas = (p->rows + kTileRows - 1) / kTileRows * p->heads;
   const bool tiles = p->mode != ST_MODE_FP32 && p->head_dim <= 128 && p->scale > 0.f && ctas <= INT32_MAX &&
