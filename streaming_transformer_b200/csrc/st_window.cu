@@ -7,18 +7,23 @@
 // query row of one head sees; it serves the rest (wider rows, 16-bit rows with a
 // scale that is not positive).
 //
-// k_window_tiles. A CTA takes 128 consecutive rows of the packed input, one TMEM
-// lane each, and one head. Rows may belong to several sequences: the keys that
-// the tile needs are those from its first row's window on, which covers every
-// sequence that begins inside the tile, and the sinks of the first row's
-// sequence. They are walked in blocks of 32 rows (sinks first, then the window
-// from exactly its first key), several blocks to a key tile:
+// k_window_tiles. A CTA takes two tiles of 128 query rows, one TMEM lane a row,
+// that share their keys: two heads of one key head, or where a key head has an
+// odd number of them two neighbouring tiles of one head. Rows may belong to
+// several sequences: the keys that are needed are those from the first row's
+// window on, which covers every sequence that begins behind it, and the sinks of
+// the first row's sequence. They are walked in blocks of 32 rows (sinks first,
+// then the window from exactly its first key), several blocks to a key tile:
 //   S = Q K^T          one MMA per 16 columns, both operands in shared memory, S in TMEM
 //   P = 2^(c S - m)    one thread a row; m, and the sum l, in fp32
 //   O += P V           P from TMEM (written over S), V as it lies in memory (N contiguous)
-// O is rescaled only when a row's maximum has grown by more than 2^8 since the
-// last time; P then stays below 2^8, which both 16-bit types hold, and l and O
-// share the reference, so the quotient is exact.
+// While the four warps of one tile are in their exponentials, the products of
+// the other run, and the copies of the next key tile: with one tile a CTA and
+// room for one key tile, the wait for its copy set the pace (529 us for 8192
+// rows, window 4096, 32 heads of 128). O is rescaled only when a row's maximum
+// has grown by more than 2^8 since the last time; P then stays below 2^8, which
+// both 16-bit types hold, and l and O share the reference, so the quotient is
+// exact.
 //
 // A warp masks only the blocks at an edge of one of its rows' windows, and skips
 // those that none of its rows sees. A masked weight is 0, but 0 times an infinite
@@ -26,7 +31,7 @@
 // CTA does its rows again with the row kernel's code, which never reads what a
 // row does not see. k_window_fp32 does the same.
 //
-// Every wait has a time limit; a CTA that ran into one writes NaN.
+// Every wait has a limit; a CTA that ran into one writes NaN.
 #include <cuda.h>
 
 #include <atomic>
@@ -117,16 +122,30 @@ __global__ void __launch_bounds__(kWindowThreads) k_window_rows(const WindowArgs
 // ---------------------------------------------------------------- tcgen05
 constexpr int kTileRows = 128;      // query rows of a CTA: TMEM lanes
 constexpr int kBlockRows = 32;      // key rows of one copy
-constexpr int kTileThreads = 192;   // 4 warps of rows, one that copies, one that issues products
-constexpr unsigned long long kWaitNs = 2000000000ull;
+constexpr int kWaitTries = 1 << 26;  // about two seconds
 
-// DP: columns, padded to 64 or 128 with zeros by the copies. Key tiles are DP rows: S takes DP TMEM columns beside
-// O's DP, so that 2 (DP 128) or 3 (DP 64) CTAs share an SM and one's products run under another's softmax.
+// Whether a phase of `bar` completed within the limit. It polls: a try_wait that suspends the thread costs more to
+// wake from than most of these waits last (8192 rows, window 4096: XXX us with it).
+__device__ __forceinline__ bool wait_phase(unsigned long long* bar, unsigned parity) {
+#pragma unroll 1
+  for (int i = 0; i < kWaitTries; ++i)
+    if (mbar_test_wait(bar, parity)) return true;
+  return false;
+}
+
+// DP: columns, padded to 64 or 128 with zeros by the copies. Key tiles are DP rows: S and O take DP TMEM columns each
+// for each tile, so that one CTA of 128 columns or two of 64 fill an SM's TMEM.
 template <int DP>
 struct Tiles {
-  static constexpr int kKeys = DP, kBlocks = kKeys / kBlockRows, kPanels = DP / 64, kStages = DP == 64 ? 2 : 1;
+  static constexpr int kKeys = DP, kBlocks = kKeys / kBlockRows, kPanels = DP / 64;
   static constexpr int kQBytes = kPanels * kTileRows * 128, kKvBytes = kPanels * kKeys * 128;
-  static constexpr int kSmem = kQBytes + 2 * kStages * kKvBytes + 1024;
+  // 4 warps of rows for each tile, one that copies, one that issues products; at 128 columns two more, which make the
+  // last four a warpgroup that hands registers to the others
+  static constexpr int kThreads = DP == 128 ? 384 : 320;
+  // One ring for K and V tiles in the order of their use: two are being read, the others are on their way. With two
+  // slots each (one ahead) the products waited for the copies.
+  static constexpr int kSlots = DP == 64 ? 8 : 5;
+  static constexpr int kSmem = 2 * kQBytes + kSlots * kKvBytes + 1024;
 };
 
 struct TileMaps {
@@ -148,6 +167,17 @@ __device__ __forceinline__ void copy_box(void* dst, const CUtensorMap* map, int 
       :: "r"(smem_addr(dst)), "l"(map), "r"(col), "r"(head), "r"(row), "r"(smem_addr(bar)) : "memory");
 }
 
+// One lane of a converged warp.
+__device__ __forceinline__ bool elect_one() {
+  unsigned yes;
+  asm volatile(
+      "{\n\t.reg .pred p;\n\t"
+      "elect.sync _|p, 0xffffffff;\n\t"
+      "selp.u32 %0, 1, 0, p;\n\t}"
+      : "=r"(yes));
+  return yes != 0;
+}
+
 // A from TMEM, B by descriptor.
 __device__ __forceinline__ void umma_f16_ts(unsigned d, unsigned at, unsigned long long bdesc, unsigned idesc,
                                             unsigned accumulate) {
@@ -159,7 +189,7 @@ __device__ __forceinline__ void umma_f16_ts(unsigned d, unsigned at, unsigned lo
       : "memory");
 }
 
-// 32 lanes x 32 columns between registers and TMEM.
+// 32 lanes x 32 columns between registers and TMEM. A load's registers may be used after tmem_ld_wait() and hold().
 __device__ __forceinline__ void tmem_ld32(unsigned addr, float (&v)[32]) {
   unsigned r[32];
   asm volatile(
@@ -172,7 +202,6 @@ __device__ __forceinline__ void tmem_ld32(unsigned addr, float (&v)[32]) {
         "=r"(r[25]), "=r"(r[26]), "=r"(r[27]), "=r"(r[28]), "=r"(r[29]), "=r"(r[30]), "=r"(r[31])
       : "r"(addr)
       : "memory");
-  asm volatile("tcgen05.wait::ld.sync.aligned;" ::: "memory");
 #pragma unroll
   for (int i = 0; i < 32; ++i) v[i] = __uint_as_float(r[i]);
 }
@@ -195,6 +224,12 @@ __device__ __forceinline__ void tmem_st16(unsigned addr, const unsigned (&r)[16]
       "r"(r[1]), "r"(r[2]), "r"(r[3]), "r"(r[4]), "r"(r[5]), "r"(r[6]), "r"(r[7]), "r"(r[8]), "r"(r[9]), "r"(r[10]),
       "r"(r[11]), "r"(r[12]), "r"(r[13]), "r"(r[14]), "r"(r[15]), "r"(addr)
       : "memory");
+}
+__device__ __forceinline__ void tmem_ld_wait() { asm volatile("tcgen05.wait::ld.sync.aligned;" ::: "memory"); }
+// Keeps uses of loaded registers behind the wait above it.
+__device__ __forceinline__ void hold(float (&v)[32]) {
+#pragma unroll
+  for (int i = 0; i < 32; ++i) asm volatile("" : "+f"(v[i]));
 }
 __device__ __forceinline__ void tmem_st_wait() { asm volatile("tcgen05.wait::st.sync.aligned;" ::: "memory"); }
 
@@ -220,6 +255,15 @@ __device__ __forceinline__ float2 fma2(float2 a, float2 b, float2 c) {
   asm("mov.b64 {%0, %1}, %2;" : "=f"(r.x), "=f"(r.y) : "l"(d));
   return r;
 }
+__device__ __forceinline__ float2 mul2(float2 a, float2 b) {
+  unsigned long long x, y, d;
+  asm("mov.b64 %0, {%1, %2};" : "=l"(x) : "f"(a.x), "f"(a.y));
+  asm("mov.b64 %0, {%1, %2};" : "=l"(y) : "f"(b.x), "f"(b.y));
+  asm("mul.rn.f32x2 %0, %1, %2;" : "=l"(d) : "l"(x), "l"(y));
+  float2 r;
+  asm("mov.b64 {%0, %1}, %2;" : "=f"(r.x), "=f"(r.y) : "l"(d));
+  return r;
+}
 __device__ __forceinline__ float2 add2(float2 a, float2 b) {
   unsigned long long x, y, d;
   asm("mov.b64 %0, {%1, %2};" : "=l"(x) : "f"(a.x), "f"(a.y));
@@ -228,6 +272,29 @@ __device__ __forceinline__ float2 add2(float2 a, float2 b) {
   float2 r;
   asm("mov.b64 {%0, %1}, %2;" : "=f"(r.x), "=f"(r.y) : "l"(d));
   return r;
+}
+
+#ifndef X_POLY
+#define X_POLY 1
+#endif
+// 2^x of two numbers of at most 2^7 on the fp32 units: x = n + r with |r| <= 1/2, a polynomial of degree 5 in r (its
+// coefficients minimise the largest relative error, 2e-7 in fp32) times 2^n. From -127 down, -inf too, it is 0; a NaN stays one.
+__device__ __forceinline__ float2 exp2_poly(float2 x) {
+  asm("max.NaN.f32 %0, %0, 0fC2FE0000;" : "+f"(x.x));  // -127
+  asm("max.NaN.f32 %0, %0, 0fC2FE0000;" : "+f"(x.y));
+  constexpr float kRound = 12582912.f;                  // 1.5 * 2^23: the sum's low bits are the nearest integer
+  const float2 t = add2(x, make_float2(kRound, kRound));
+  const float2 n = add2(t, make_float2(-kRound, -kRound));
+  const float2 r = add2(x, make_float2(-n.x, -n.y));
+  float2 p = make_float2(0.001327647129073739f, 0.001327647129073739f);
+  p = fma2(p, r, make_float2(0.009675541892647743f, 0.009675541892647743f));
+  p = fma2(p, r, make_float2(0.05550713092088699f, 0.05550713092088699f));
+  p = fma2(p, r, make_float2(0.24022120237350464f, 0.24022120237350464f));
+  p = fma2(p, r, make_float2(0.6931469440460205f, 0.6931469440460205f));
+  p = fma2(p, r, make_float2(1.0000001192092896f, 1.0000001192092896f));
+  const float2 scale = make_float2(__uint_as_float((__float_as_uint(t.x) << 23) + 0x3f800000u),
+                                   __uint_as_float((__float_as_uint(t.y) << 23) + 0x3f800000u));
+  return mul2(p, scale);
 }
 
 // Bits lo .. hi of a 32-bit word (either end may lie outside it).
@@ -248,10 +315,10 @@ struct TileKeys {
     return block < sink_blocks ? start + block * kBlockRows : low + (block - sink_blocks) * kBlockRows;
   }
 };
-template <int ROWS>
-__device__ __forceinline__ bool tile_keys(const WindowArgs& a, int tile, TileKeys& t) {
-  t.r0 = tile * ROWS;
-  t.r1 = (int)min((long long)a.rows, (long long)t.r0 + ROWS) - 1;
+__device__ __forceinline__ bool tile_keys(const WindowArgs& a, long long first, int rows, TileKeys& t) {
+  if (first >= a.rows) return false;
+  t.r0 = (int)first;
+  t.r1 = (int)min((long long)a.rows, first + rows) - 1;
   if (a.starts) {
     t.r0 = max(t.r0, clamp_row(a.starts[0], a.rows));
     t.r1 = min(t.r1, clamp_row(a.starts[a.sequences], a.rows) - 1);
@@ -282,128 +349,230 @@ struct RowLimits {
     return bit_range(low - base, row - base) | bit_range(start - base, sink_last - base);
   }
 };
-// First row that is inside every row's window; blocks from it up to the tile's first row need no mask.
-__device__ __forceinline__ int common_low(const WindowArgs& a, const TileKeys& t) {
-  return (int)max((long long)sequence_start(a, t.r1), (long long)t.r1 - a.window + 1);
+// First row that is inside the window of every row up to r1 of r1's sequence.
+__device__ __forceinline__ int common_low(const WindowArgs& a, int r1) {
+  return (int)max((long long)sequence_start(a, r1), (long long)r1 - a.window + 1);
 }
 
+// One of a CTA's two tiles: which key blocks any of its rows can see, and which all of them do.
+struct SubTile {
+  int r0, r1, start, low, sink_end, all_low;
+  bool any;
+  __device__ void set(const WindowArgs& a, const TileKeys& t, long long first) {
+    any = first <= t.r1;
+    if (!any) return;
+    r0 = max((int)first, t.r0);
+    r1 = (int)min((long long)t.r1, first + kTileRows - 1);
+    any = r0 <= r1;
+    if (!any) return;
+    start = max(sequence_start(a, r0), 0);
+    low = (int)max((long long)start, (long long)r0 - a.window + 1);
+    sink_end = (int)min((long long)r0, (long long)start + a.sinks);
+    all_low = common_low(a, r1);
+  }
+  __device__ bool needs(const TileKeys& t, int b0, int nb) const {
+    if (!any) return false;
+    if (b0 < t.sink_blocks) return start == t.start || b0 + nb > t.sink_blocks;
+    const int first = t.base(b0), last = t.base(b0 + nb - 1) + kBlockRows - 1;
+    return (last >= low && first <= r1) || (last >= start && first < sink_end);
+  }
+  __device__ bool sees_all(const TileKeys& t, int b0, int nb) const {
+    return b0 >= t.sink_blocks && t.base(b0) >= all_low && t.base(b0 + nb - 1) + kBlockRows - 1 <= r0;
+  }
+};
+
 template <typename T, int DP>
-__global__ void __launch_bounds__(kTileThreads, DP == 64 ? 3 : 2)
+__global__ void __launch_bounds__(Tiles<DP>::kThreads, DP == 64 ? 2 : 1)
     k_window_tiles(const WindowArgs a, const __grid_constant__ TileMaps maps) {
   using G = Tiles<DP>;
   extern __shared__ unsigned char raw[];
-  __shared__ unsigned long long q_full, k_full[G::kStages], k_free[G::kStages], v_full[G::kStages], v_free[G::kStages],
-      s_full, p_full, o_full;
+  __shared__ unsigned long long q_full, full[G::kSlots], free[G::kSlots], s_full[2], p_full[2], o_full[2];
   __shared__ unsigned tmem_base;
   __shared__ int sh_slow, sh_dead;
   const int warp = threadIdx.x >> 5;
-  const int h = blockIdx.x % a.heads, tile = gridDim.x / a.heads - 1 - blockIdx.x / a.heads;  // most keys first
+  // the pair: two heads of one tile of rows, or two tiles of one head; those with most keys first
+  const bool two_heads = (a.heads / a.kv_heads) % 2 == 0;
+  const int per_row = two_heads ? a.heads / 2 : a.heads;
+  const int h0 = two_heads ? blockIdx.x % per_row * 2 : blockIdx.x % per_row;
+  const long long pair_row = (long long)(gridDim.x / per_row - 1 - blockIdx.x / per_row) * (two_heads ? 1 : 2) * kTileRows;
+  auto head_of = [&](int s) { return two_heads ? h0 + s : h0; };
+  auto first_row = [&](int s) { return pair_row + (two_heads ? 0 : s * kTileRows); };
   TileKeys keys;
-  if (!tile_keys<kTileRows>(a, tile, keys)) return;
+  if (!tile_keys(a, pair_row, (two_heads ? 1 : 2) * kTileRows, keys)) return;
   unsigned char* smem = raw + ((1024u - (smem_addr(raw) & 1023u)) & 1023u);
-  unsigned char *sq = smem, *sk = sq + G::kQBytes, *sv = sk + G::kStages * G::kKvBytes;
+  unsigned char *sq = smem, *ring = sq + 2 * G::kQBytes;  // ring item 2 i: K of key tile i, 2 i + 1: V
   if (threadIdx.x == 0) {
     mbar_init(&q_full, 1);
-    for (int s = 0; s < G::kStages; ++s) {
-      mbar_init(&k_full[s], 1);
-      mbar_init(&k_free[s], 1);
-      mbar_init(&v_full[s], 1);
-      mbar_init(&v_free[s], 1);
+    for (int s = 0; s < G::kSlots; ++s) {
+      mbar_init(&full[s], 1);
+      mbar_init(&free[s], 1);
     }
-    mbar_init(&s_full, 1);
-    mbar_init(&p_full, 4);
-    mbar_init(&o_full, 1);
+    for (int s = 0; s < 2; ++s) {
+      mbar_init(&s_full[s], 1);
+      mbar_init(&p_full[s], 4);
+      mbar_init(&o_full[s], 1);
+    }
     fence_mbar_init();
     sh_slow = sh_dead = 0;
   }
-  if (warp == 5) {
-    tmem_alloc(&tmem_base, 2 * DP);
+  if (warp == 9) {
+    tmem_alloc(&tmem_base, 4 * DP);
     tmem_relinquish();
   }
   tc_fence_before();
   __syncthreads();
   tc_fence_after();
-  const unsigned tm_s = tmem_base, tm_o = tmem_base + DP;
+  // TMEM: S of both tiles, then O of both
+  const unsigned tmem = tmem_base;
   const int tiles = (keys.blocks + G::kBlocks - 1) / G::kBlocks;
   // A wait that runs out ends its role; the others' waits then run out as well.
   auto wait = [&](unsigned long long* bar, int use) -> bool {
-    if (mbar_wait_bounded(bar, use & 1, kWaitNs)) return true;
+    if (wait_phase(bar, use & 1)) return true;
     *(volatile int*)&sh_dead = 1;
     return false;
   };
 
-  if (warp == 4) {
-    if ((threadIdx.x & 31) == 0) {
-      const int kv = h / (a.heads / a.kv_heads);
-      mbar_expect_tx(&q_full, G::kQBytes);
-      for (int p = 0; p < G::kPanels; ++p)
-        copy_box(sq + p * kTileRows * 128, &maps.q, p * 64, h, tile * kTileRows, &q_full);
-      int issued = 0;
-      for (; issued < tiles; ++issued) {
-        const int s = issued % G::kStages, use = issued / G::kStages, b0 = issued * G::kBlocks;
-        const int nb = min(G::kBlocks, keys.blocks - b0);
-        bool ok = true;
-        for (int side = 0; side < 2 && ok; ++side) {
-          unsigned long long *full = side ? &v_full[s] : &k_full[s], *free = side ? &v_free[s] : &k_free[s];
-          if (use > 0 && !(ok = wait(free, use - 1))) break;
-          unsigned char* dst = (side ? sv : sk) + s * G::kKvBytes;
-          mbar_expect_tx(full, nb * G::kPanels * kBlockRows * 128);
-          for (int b = 0; b < nb; ++b)
-            for (int p = 0; p < G::kPanels; ++p)
-              copy_box(dst + p * G::kKeys * 128 + b * kBlockRows * 128, side ? &maps.v : &maps.k, p * 64, kv,
-                       keys.base(b0 + b), full);
+  if (warp >= 8) {
+    // 384 threads start with 168 registers each: 2 * 128 * 208 + 128 * 88 is as many
+    if constexpr (DP == 128) asm volatile("setmaxnreg.dec.sync.aligned.u32 88;");
+    // Both warps run as a whole, and one lane issues: what an instruction takes then stays in uniform registers. The
+    // products' issue is on the critical path (by one lane alone, with descriptors built for each: XXX us).
+    if (warp == 8) {
+      const bool lead = elect_one();
+      const int kv = h0 / (a.heads / a.kv_heads);
+      if (lead) {
+        mbar_expect_tx(&q_full, 2 * G::kQBytes);
+        for (int s = 0; s < 2; ++s)
+          for (int p = 0; p < G::kPanels; ++p)
+            copy_box(sq + s * G::kQBytes + p * kTileRows * 128, &maps.q, p * 64, head_of(s), (int)first_row(s), &q_full);
+      }
+      int item = 0, slot = 0, use = 0;
+      for (; item < 2 * tiles; ++item) {
+        const int b0 = item / 2 * G::kBlocks, nb = min(G::kBlocks, keys.blocks - b0);
+        if (use > 0 && !wait(&free[slot], use - 1)) break;
+        if (lead) {
+          mbar_expect_tx(&full[slot], nb * G::kPanels * kBlockRows * 128);
+          unsigned char* to = ring + slot * G::kKvBytes;
+          const CUtensorMap* map = item & 1 ? &maps.v : &maps.k;
+          for (int b = 0; b < nb; ++b, to += kBlockRows * 128) {
+            const int row = keys.base(b0 + b);
+#pragma unroll
+            for (int p = 0; p < G::kPanels; ++p) copy_box(to + p * G::kKeys * 128, map, p * 64, kv, row, &full[slot]);
+          }
         }
-        if (!ok) break;
+        if (++slot == G::kSlots) slot = 0, ++use;
       }
       if (*(volatile int*)&sh_dead) {  // no copy may land after the CTA has left
-        wait(&q_full, 0);
-        for (int i = max(0, issued - G::kStages); i < min(tiles, issued + 1); ++i) {
-          mbar_wait_bounded(&k_full[i % G::kStages], (i / G::kStages) & 1, kWaitNs);
-          mbar_wait_bounded(&v_full[i % G::kStages], (i / G::kStages) & 1, kWaitNs);
-        }
+        wait_phase(&q_full, 0);
+        for (int i = max(0, item - G::kSlots); i < item; ++i) wait_phase(&full[i % G::kSlots], (i / G::kSlots) & 1);
       }
-    }
-  } else if (warp == 5) {
-    if ((threadIdx.x & 31) == 0 && wait(&q_full, 0)) {
-      const int ksteps = (a.head_dim + 15) / 16, n_o = ksteps * 16;
-      const unsigned idesc_o = umma_idesc<T>(kTileRows, n_o) | (1u << 16);  // V: N contiguous
-      for (int i = 0; i < tiles; ++i) {
-        const int s = i % G::kStages, use = i / G::kStages, nb = min(G::kBlocks, keys.blocks - i * G::kBlocks);
-        if (!wait(&k_full[s], use)) break;
-        if (i > 0 && !wait(&o_full, i - 1)) break;  // P(i - 1), under S, has been read
+    } else if (warp == 9) {
+      const bool lead = elect_one();
+      SubTile sub[2];
+      for (int s = 0; s < 2; ++s) sub[s].set(a, keys, first_row(s));
+      const int ksteps = (a.head_dim + 15) / 16;
+      const unsigned idesc_s = umma_idesc<T>(kTileRows, G::kKeys);
+      const unsigned idesc_o = umma_idesc<T>(kTileRows, ksteps * 16) | (1u << 16);  // V: N contiguous
+      const unsigned long long dq = swizzled_desc(sq, 0), dk = swizzled_desc(ring, 0), dv = swizzled_desc(ring, G::kKeys * 128);
+      constexpr unsigned kSlotStep = G::kKvBytes >> 4;
+      int done[2] = {0, 0};  // second products issued
+      auto needs = [&](int s, int i) {
+        return i < tiles && sub[s].needs(keys, i * G::kBlocks, min(G::kBlocks, keys.blocks - i * G::kBlocks));
+      };
+      // S of a key tile, once P of the last one, under it, has been read
+      auto first_product = [&](int s, int slot, int nb) -> bool {
+        if (done[s] > 0 && !wait(&o_full[s], done[s] - 1)) return false;
         tc_fence_after();
-        const unsigned idesc_s = umma_idesc<T>(kTileRows, nb * kBlockRows);
-        for (int k = 0; k < ksteps; ++k)
-          umma_f16(tm_s, swizzled_desc(sq + (k / 4) * kTileRows * 128 + (k % 4) * 32, 0),
-                   swizzled_desc(sk + s * G::kKvBytes + (k / 4) * G::kKeys * 128 + (k % 4) * 32, 0), idesc_s, k > 0);
-        umma_commit(&k_free[s]);
-        umma_commit(&s_full);
-        if (!wait(&v_full[s], use) || !wait(&p_full, i)) break;
+        const unsigned idesc = nb == G::kBlocks ? idesc_s : umma_idesc<T>(kTileRows, nb * kBlockRows);
+        const unsigned long long q = dq + s * (G::kQBytes >> 4), k = dk + slot * kSlotStep;
+        if (lead) {
+#pragma unroll
+          for (int e = 0; e < DP / 16; ++e)
+            if (e < ksteps)
+              umma_f16(tmem + s * DP, q + (e / 4) * (kTileRows * 128 >> 4) + (e % 4) * 2,
+                       k + (e / 4) * (G::kKeys * 128 >> 4) + (e % 4) * 2, idesc, e > 0);
+          umma_commit(&s_full[s]);
+        }
+        __syncwarp();
+        return true;
+      };
+      auto second_product = [&](int s, int slot, int nb) -> bool {
+        if (!wait(&p_full[s], done[s])) return false;
         tc_fence_after();
-        for (int k = 0; k < nb * 2; ++k)
-          umma_f16_ts(tm_o, tm_s + k * 8, swizzled_desc(sv + s * G::kKvBytes + k * 2048, G::kKeys * 128), idesc_o,
-                      i > 0 || k > 0);
-        umma_commit(&v_free[s]);
-        umma_commit(&o_full);
+        const unsigned long long v = dv + slot * kSlotStep;
+        if (lead) {
+#pragma unroll
+          for (int e = 0; e < G::kBlocks * 2; ++e)
+            if (e < nb * 2)
+              umma_f16_ts(tmem + (2 + s) * DP, tmem + s * DP + e * 8, v + e * (2048 >> 4), idesc_o, e > 0 || done[s] > 0);
+          umma_commit(&o_full[s]);
+        }
+        __syncwarp();
+        ++done[s];
+        return true;
+      };
+      int slot = 0, use = 0;   // of the next ring item
+      auto here = [&]() { return wait(&full[slot], use); };
+      auto advance = [&]() {
+        const int was = slot;
+        if (++slot == G::kSlots) slot = 0, ++use;
+        return was;
+      };
+      auto release = [&](int which) {
+        if (lead) umma_commit(&free[which]);
+        __syncwarp();
+      };
+      int nb = min(G::kBlocks, keys.blocks);
+      bool need0 = needs(0, 0), need1 = needs(1, 0);
+      bool ok = wait(&q_full, 0) && here();
+      if (ok) {
+        const int k = advance();
+        ok = (!need0 || first_product(0, k, nb)) && (!need1 || first_product(1, k, nb));
+        if (ok) release(k);
+      }
+      for (int i = 0; i < tiles && ok; ++i) {
+        const bool next0 = needs(0, i + 1), next1 = needs(1, i + 1), more = i + 1 < tiles;
+        const int next_nb = min(G::kBlocks, keys.blocks - (i + 1) * G::kBlocks);
+        if (!(ok = here())) break;
+        const int v = advance();
+        if (need0 && !(ok = second_product(0, v, nb))) break;
+        int k = 0;
+        if (more) {
+          if (!(ok = here())) break;
+          k = advance();
+          if (next0 && !(ok = first_product(0, k, next_nb))) break;
+        }
+        if (need1 && !(ok = second_product(1, v, nb))) break;
+        release(v);
+        if (more) {
+          if (next1 && !(ok = first_product(1, k, next_nb))) break;
+          release(k);
+        }
+        need0 = next0;
+        need1 = next1;
+        nb = next_nb;
       }
     }
   } else {
-    const int row = tile * kTileRows + threadIdx.x, lane = threadIdx.x & 31;
-    const unsigned my_s = tm_s + ((unsigned)(warp * 32) << 16), my_o = tm_o + ((unsigned)(warp * 32) << 16);
+    if constexpr (DP == 128) asm volatile("setmaxnreg.inc.sync.aligned.u32 208;");
+    const int side = warp >> 2, h = head_of(side), lane = threadIdx.x & 31;
+    SubTile sub;
+    sub.set(a, keys, first_row(side));
+    const long long row = first_row(side) + (threadIdx.x & 127);
+    const unsigned lanes = (unsigned)((warp & 3) * 32) << 16;
+    const unsigned my_s = tmem + side * DP + lanes, my_o = tmem + (2 + side) * DP + lanes;
     RowLimits limits;
-    limits.set(a, keys, row);
+    limits.set(a, keys, (int)min(row, (long long)INT32_MAX));
     const bool inside = limits.start >= 0;
-    const int all_low = common_low(a, keys);
     const float c = a.scale * 1.4426950408889634f;
     float m = -INFINITY, l = 0.f;  // m: reference of the weights, in units of S
     bool ok = true;
+    int n = 0;                     // key tiles of this side so far
     for (int i = 0; i < tiles && ok; ++i) {
       const int b0 = i * G::kBlocks, nb = min(G::kBlocks, keys.blocks - b0);
-      const bool plain = b0 >= keys.sink_blocks && keys.base(b0) >= all_low &&
-                         keys.base(b0 + nb - 1) + kBlockRows - 1 <= keys.r0;
-      if (!(ok = wait(&s_full, i))) break;
-      tc_fence_after();
+      if (!sub.needs(keys, b0, nb)) continue;
       // the blocks: bits of the keys this row sees; a block that no row of the warp sees is left out
+      const bool plain = nb == G::kBlocks && sub.sees_all(keys, b0, nb);
       unsigned seen[G::kBlocks];
       bool some[G::kBlocks], edge[G::kBlocks];
 #pragma unroll
@@ -412,23 +581,41 @@ __global__ void __launch_bounds__(kTileThreads, DP == 64 ? 3 : 2)
         some[b] = plain || __any_sync(0xffffffffu, seen[b] != 0u);
         edge[b] = !plain && __any_sync(0xffffffffu, seen[b] != ~0u);
       }
-      auto load = [&](int b, float (&x)[32]) {
-        tmem_ld32(my_s + b * 32, x);
+      if (!(ok = wait(&s_full[side], n))) break;
+      tc_fence_after();
+      auto mask = [&](int b, float (&x)[32]) {
         if (edge[b])
 #pragma unroll
           for (int e = 0; e < 32; ++e) x[e] = (seen[b] >> e) & 1u ? x[e] : -INFINITY;
       };
-      // At 64 keys the tile stays in registers between the passes, at 128 it is read again.
-      constexpr bool kKeep = G::kBlocks <= 2;
-      float x[kKeep ? G::kBlocks : 1][32], top = -INFINITY;
+      // At 128 columns the registers hold the tile between the passes, at 64 (two CTAs an SM) it is read again.
+      constexpr bool kKeep = DP == 128;
+      float x[kKeep ? G::kBlocks : 1][32], tops[4] = {-INFINITY, -INFINITY, -INFINITY, -INFINITY};
+      // a block's load is on its way while the one before it is looked at; four maxima, for the latency of each
+      auto look = [&](int b, float (&y)[32]) {
+        hold(y);
+        mask(b, y);
 #pragma unroll
-      for (int b = 0; b < G::kBlocks; ++b)
-        if (some[b]) {
-          float(&y)[32] = x[kKeep ? b : 0];
-          load(b, y);
+        for (int e = 0; e < 32; e += 2) tops[e / 2 % 4] = max3(tops[e / 2 % 4], y[e], y[e + 1]);
+      };
+      if constexpr (kKeep) {
+        if (some[0]) tmem_ld32(my_s, x[0]);
 #pragma unroll
-          for (int e = 0; e < 32; e += 2) top = max3(top, y[e], y[e + 1]);
+        for (int b = 0; b < G::kBlocks; ++b) {
+          if (some[b]) tmem_ld_wait();
+          if (b + 1 < G::kBlocks && some[b + 1]) tmem_ld32(my_s + (b + 1) * 32, x[b + 1]);
+          if (some[b]) look(b, x[b]);
         }
+      } else {
+#pragma unroll
+        for (int b = 0; b < G::kBlocks; ++b)
+          if (some[b]) {
+            tmem_ld32(my_s + b * 32, x[0]);
+            tmem_ld_wait();
+            look(b, x[0]);
+          }
+      }
+      const float top = fmaxf(fmaxf(tops[0], tops[1]), fmaxf(tops[2], tops[3]));
       // a new reference only when the old one is too low; exp2(8) is the most a weight can be
       const bool grow = top > m && !((top - m) * c <= 8.f);
       if (__any_sync(0xffffffffu, grow)) {
@@ -436,11 +623,13 @@ __global__ void __launch_bounds__(kTileThreads, DP == 64 ? 3 : 2)
         const float keep = next == -INFINITY ? 1.f : exp2_fast((m - next) * c);
         m = next;
         l *= keep;
-        if (i > 0) {
+        if (n > 0) {
 #pragma unroll
           for (int d = 0; d < DP; d += 32) {
             float o[32];
             tmem_ld32(my_o + d, o);
+            tmem_ld_wait();
+            hold(o);
 #pragma unroll
             for (int e = 0; e < 32; ++e) o[e] *= keep;
             tmem_st32(my_o + d, o);
@@ -450,19 +639,25 @@ __global__ void __launch_bounds__(kTileThreads, DP == 64 ? 3 : 2)
       // fp16 weights 2^7 higher, up to 2^15, away from its denormals
       const float ref = m == -INFINITY ? 0.f : m * c - (std::is_same<T, __half>::value ? 7.f : 0.f);
       const float2 c2 = make_float2(c, c), ref2 = make_float2(-ref, -ref);
-      float2 sum = make_float2(0.f, 0.f);
+      float2 sums[2] = {make_float2(0.f, 0.f), make_float2(0.f, 0.f)};
 #pragma unroll
       for (int b = 0; b < G::kBlocks; ++b) {
         if (b >= nb) break;
         unsigned p[16];
         if (some[b]) {
           float(&y)[32] = x[kKeep ? b : 0];
-          if (!kKeep) load(b, y);
+          if (!kKeep) {
+            tmem_ld32(my_s + b * 32, y);
+            tmem_ld_wait();
+            hold(y);
+            mask(b, y);
+          }
 #pragma unroll
           for (int e = 0; e < 16; ++e) {
             float2 w = fma2(make_float2(y[2 * e], y[2 * e + 1]), c2, ref2);
-            w = make_float2(exp2_fast(w.x), exp2_fast(w.y));
-            sum = add2(sum, w);
+            if (e % 4 >= 4 - X_POLY) w = exp2_poly(w);
+            else w = make_float2(exp2_fast(w.x), exp2_fast(w.y));
+            sums[e & 1] = add2(sums[e & 1], w);
             p[e] = pack2((T*)nullptr, w.x, w.y);
           }
         } else {
@@ -471,22 +666,27 @@ __global__ void __launch_bounds__(kTileThreads, DP == 64 ? 3 : 2)
         }
         tmem_st16(my_s + b * 16, p);
       }
-      l += sum.x + sum.y;
+      l += (sums[0].x + sums[0].y) + (sums[1].x + sums[1].y);
       tmem_st_wait();
       tc_fence_before();
       __syncwarp();
-      if (lane == 0) mbar_arrive(&p_full);
+      if (lane == 0) mbar_arrive(&p_full[side]);
+      ++n;
     }
-    if (ok) ok = wait(&o_full, tiles - 1);
+    if (ok && n > 0) ok = wait(&o_full[side], n - 1);
     tc_fence_after();
-    const bool good = __all_sync(0xffffffffu, ok);
+    const bool good = __all_sync(0xffffffffu, ok && n > 0);
     if (good || inside) {
       bool odd = false;  // a result that is not finite
-      T* to = static_cast<T*>(a.out) + (long long)row * a.o_row + h * a.o_head;
+      T* to = static_cast<T*>(a.out) + row * a.o_row + h * a.o_head;
 #pragma unroll
       for (int d = 0; d < DP; d += 32) {
         float o[32];
-        if (good) tmem_ld32(my_o + d, o);
+        if (good) {
+          tmem_ld32(my_o + d, o);
+          tmem_ld_wait();
+          hold(o);
+        }
         const float inv = good ? 1.f / l : NAN;
         if (inside)
 #pragma unroll
@@ -508,13 +708,17 @@ __global__ void __launch_bounds__(kTileThreads, DP == 64 ? 3 : 2)
   }
   __syncthreads();
   tc_fence_after();
-  if (warp == 5) tmem_dealloc(tmem_base, 2 * DP);
-  if (sh_slow && !sh_dead && warp < 4) {
+  if (warp == 9) tmem_dealloc(tmem, 4 * DP);
+  if (sh_slow && !sh_dead && warp < 8) {
     constexpr int kLanes = DP / 8;
-    for (int r = keys.r0 + threadIdx.x / kLanes; r <= keys.r1; r += 128 / kLanes) {
-      const int start = sequence_start(a, r);
-      if (start >= 0) window_row<T, kLanes>(a, r, start, h, threadIdx.x % kLanes, row_mask<kLanes>());
-    }
+    const int side = warp >> 2;
+    SubTile sub;
+    sub.set(a, keys, first_row(side));
+    if (sub.any)
+      for (int r = sub.r0 + (threadIdx.x & 127) / kLanes; r <= sub.r1; r += 128 / kLanes) {
+        const int start = sequence_start(a, r);
+        if (start >= 0) window_row<T, kLanes>(a, r, start, head_of(side), threadIdx.x % kLanes, row_mask<kLanes>());
+      }
   }
 }
 
@@ -546,7 +750,7 @@ __global__ void __launch_bounds__(kFp32Threads) k_window_fp32(const WindowArgs a
   __shared__ int sh_slow;
   const int h = blockIdx.x % a.heads, tile = gridDim.x / a.heads - 1 - blockIdx.x / a.heads, kv = h / (a.heads / a.kv_heads);
   TileKeys keys;
-  if (!tile_keys<kFp32Rows>(a, tile, keys)) return;
+  if (!tile_keys(a, (long long)tile * kFp32Rows, kFp32Rows, keys)) return;
   const int ty = threadIdx.x / 16, tx = threadIdx.x % 16;
   if (threadIdx.x == 0) sh_slow = 0;
   // rows of a block beyond the tile's last, and columns past head_dim, are zeros
@@ -575,7 +779,7 @@ __global__ void __launch_bounds__(kFp32Threads) k_window_fp32(const WindowArgs a
   RowLimits limits[4];
 #pragma unroll
   for (int r = 0; r < 4; ++r) limits[r].set(a, keys, tile * kFp32Rows + ty * 4 + r);
-  const int all_low = common_low(a, keys);
+  const int all_low = common_low(a, keys.r1);
   const float c = a.scale * 1.4426950408889634f;
   float o[4][DP / 64][4] = {}, m[4], l[4] = {};
 #pragma unroll
@@ -748,7 +952,8 @@ cudaError_t launch_tiles(const WindowArgs& a, const TileMaps& maps, cudaStream_t
       cudaFuncSetAttribute(k_window_tiles<T, DP>, cudaFuncAttributeMaxDynamicSharedMemorySize, Tiles<DP>::kSmem);
   if (e != cudaSuccess) return e;
   const unsigned tiles = (unsigned)((a.rows + kTileRows - 1ll) / kTileRows);
-  k_window_tiles<T, DP><<<tiles * a.heads, kTileThreads, Tiles<DP>::kSmem, s>>>(a, maps);
+  const unsigned ctas = a.heads / a.kv_heads % 2 == 0 ? tiles * (a.heads / 2) : (tiles + 1) / 2 * a.heads;
+  k_window_tiles<T, DP><<<ctas, Tiles<DP>::kThreads, Tiles<DP>::kSmem, s>>>(a, maps);
   return cudaSuccess;
 }
 
