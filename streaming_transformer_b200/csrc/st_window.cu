@@ -19,8 +19,10 @@
 //   O += P V           P from TMEM (written over S), V as it lies in memory (N contiguous)
 // While the four warps of one tile are in their exponentials, the products of
 // the other run, and the copies of the next key tile: with one tile a CTA and
-// room for one key tile, the wait for its copy set the pace (529 us for 8192
-// rows, window 4096, 32 heads of 128). O is rescaled only when a row's maximum
+// room for one key tile, the waits for its copy and for the products set the pace
+// (8192 rows, window 4096, 32 heads of 128: 529 us, now 467, 0.53 of the measured
+// dense rate; what bounds it is the chain S, softmax, O of each query tile, 3700
+// cycles a key tile where exponentials and products take 2050 each). O is rescaled only when a row's maximum
 // has grown by more than 2^8 since the last time; P then stays below 2^8, which
 // both 16-bit types hold, and l and O share the reference, so the quotient is
 // exact.
@@ -189,21 +191,39 @@ __device__ __forceinline__ void umma_f16_ts(unsigned d, unsigned at, unsigned lo
       : "memory");
 }
 
-// 32 lanes x 32 columns between registers and TMEM. A load's registers may be used after tmem_ld_wait() and hold().
+// 32 lanes x 32 or 64 columns between registers and TMEM. The wait belongs to the load's own statement: its registers
+// have no value before it, and nothing may move them.
 __device__ __forceinline__ void tmem_ld32(unsigned addr, float (&v)[32]) {
-  unsigned r[32];
   asm volatile(
-      "tcgen05.ld.sync.aligned.32x32b.x32.b32 "
-      "{%0,%1,%2,%3,%4,%5,%6,%7,%8,%9,%10,%11,%12,%13,%14,%15,%16,%17,%18,%19,%20,%21,%22,%23,%24,%25,%26,%27,%28,%29,"
-      "%30,%31}, [%32];"
-      : "=r"(r[0]), "=r"(r[1]), "=r"(r[2]), "=r"(r[3]), "=r"(r[4]), "=r"(r[5]), "=r"(r[6]), "=r"(r[7]), "=r"(r[8]),
-        "=r"(r[9]), "=r"(r[10]), "=r"(r[11]), "=r"(r[12]), "=r"(r[13]), "=r"(r[14]), "=r"(r[15]), "=r"(r[16]),
-        "=r"(r[17]), "=r"(r[18]), "=r"(r[19]), "=r"(r[20]), "=r"(r[21]), "=r"(r[22]), "=r"(r[23]), "=r"(r[24]),
-        "=r"(r[25]), "=r"(r[26]), "=r"(r[27]), "=r"(r[28]), "=r"(r[29]), "=r"(r[30]), "=r"(r[31])
+      "tcgen05.ld.sync.aligned.32x32b.x32.b32 {"
+      "%0,%1,%2,%3,%4,%5,%6,%7,%8,%9,%10,%11,%12,%13,%14,%15,"
+      "%16,%17,%18,%19,%20,%21,%22,%23,%24,%25,%26,%27,%28,%29,%30,%31"
+      "}, [%32];\n\ttcgen05.wait::ld.sync.aligned;"
+      : "=f"(v[0]), "=f"(v[1]), "=f"(v[2]), "=f"(v[3]), "=f"(v[4]), "=f"(v[5]), "=f"(v[6]), "=f"(v[7]),
+        "=f"(v[8]), "=f"(v[9]), "=f"(v[10]), "=f"(v[11]), "=f"(v[12]), "=f"(v[13]), "=f"(v[14]), "=f"(v[15]),
+        "=f"(v[16]), "=f"(v[17]), "=f"(v[18]), "=f"(v[19]), "=f"(v[20]), "=f"(v[21]), "=f"(v[22]), "=f"(v[23]),
+        "=f"(v[24]), "=f"(v[25]), "=f"(v[26]), "=f"(v[27]), "=f"(v[28]), "=f"(v[29]), "=f"(v[30]), "=f"(v[31])
       : "r"(addr)
       : "memory");
-#pragma unroll
-  for (int i = 0; i < 32; ++i) v[i] = __uint_as_float(r[i]);
+}
+__device__ __forceinline__ void tmem_ld64(unsigned addr, float (&v)[64]) {
+  asm volatile(
+      "tcgen05.ld.sync.aligned.32x32b.x64.b32 {"
+      "%0,%1,%2,%3,%4,%5,%6,%7,%8,%9,%10,%11,%12,%13,%14,%15,"
+      "%16,%17,%18,%19,%20,%21,%22,%23,%24,%25,%26,%27,%28,%29,%30,%31,"
+      "%32,%33,%34,%35,%36,%37,%38,%39,%40,%41,%42,%43,%44,%45,%46,%47,"
+      "%48,%49,%50,%51,%52,%53,%54,%55,%56,%57,%58,%59,%60,%61,%62,%63"
+      "}, [%64];\n\ttcgen05.wait::ld.sync.aligned;"
+      : "=f"(v[0]), "=f"(v[1]), "=f"(v[2]), "=f"(v[3]), "=f"(v[4]), "=f"(v[5]), "=f"(v[6]), "=f"(v[7]),
+        "=f"(v[8]), "=f"(v[9]), "=f"(v[10]), "=f"(v[11]), "=f"(v[12]), "=f"(v[13]), "=f"(v[14]), "=f"(v[15]),
+        "=f"(v[16]), "=f"(v[17]), "=f"(v[18]), "=f"(v[19]), "=f"(v[20]), "=f"(v[21]), "=f"(v[22]), "=f"(v[23]),
+        "=f"(v[24]), "=f"(v[25]), "=f"(v[26]), "=f"(v[27]), "=f"(v[28]), "=f"(v[29]), "=f"(v[30]), "=f"(v[31]),
+        "=f"(v[32]), "=f"(v[33]), "=f"(v[34]), "=f"(v[35]), "=f"(v[36]), "=f"(v[37]), "=f"(v[38]), "=f"(v[39]),
+        "=f"(v[40]), "=f"(v[41]), "=f"(v[42]), "=f"(v[43]), "=f"(v[44]), "=f"(v[45]), "=f"(v[46]), "=f"(v[47]),
+        "=f"(v[48]), "=f"(v[49]), "=f"(v[50]), "=f"(v[51]), "=f"(v[52]), "=f"(v[53]), "=f"(v[54]), "=f"(v[55]),
+        "=f"(v[56]), "=f"(v[57]), "=f"(v[58]), "=f"(v[59]), "=f"(v[60]), "=f"(v[61]), "=f"(v[62]), "=f"(v[63])
+      : "r"(addr)
+      : "memory");
 }
 __device__ __forceinline__ void tmem_st32(unsigned addr, const float (&v)[32]) {
   unsigned r[32];
@@ -224,12 +244,6 @@ __device__ __forceinline__ void tmem_st16(unsigned addr, const unsigned (&r)[16]
       "r"(r[1]), "r"(r[2]), "r"(r[3]), "r"(r[4]), "r"(r[5]), "r"(r[6]), "r"(r[7]), "r"(r[8]), "r"(r[9]), "r"(r[10]),
       "r"(r[11]), "r"(r[12]), "r"(r[13]), "r"(r[14]), "r"(r[15]), "r"(addr)
       : "memory");
-}
-__device__ __forceinline__ void tmem_ld_wait() { asm volatile("tcgen05.wait::ld.sync.aligned;" ::: "memory"); }
-// Keeps uses of loaded registers behind the wait above it.
-__device__ __forceinline__ void hold(float (&v)[32]) {
-#pragma unroll
-  for (int i = 0; i < 32; ++i) asm volatile("" : "+f"(v[i]));
 }
 __device__ __forceinline__ void tmem_st_wait() { asm volatile("tcgen05.wait::st.sync.aligned;" ::: "memory"); }
 
@@ -255,15 +269,6 @@ __device__ __forceinline__ float2 fma2(float2 a, float2 b, float2 c) {
   asm("mov.b64 {%0, %1}, %2;" : "=f"(r.x), "=f"(r.y) : "l"(d));
   return r;
 }
-__device__ __forceinline__ float2 mul2(float2 a, float2 b) {
-  unsigned long long x, y, d;
-  asm("mov.b64 %0, {%1, %2};" : "=l"(x) : "f"(a.x), "f"(a.y));
-  asm("mov.b64 %0, {%1, %2};" : "=l"(y) : "f"(b.x), "f"(b.y));
-  asm("mul.rn.f32x2 %0, %1, %2;" : "=l"(d) : "l"(x), "l"(y));
-  float2 r;
-  asm("mov.b64 {%0, %1}, %2;" : "=f"(r.x), "=f"(r.y) : "l"(d));
-  return r;
-}
 __device__ __forceinline__ float2 add2(float2 a, float2 b) {
   unsigned long long x, y, d;
   asm("mov.b64 %0, {%1, %2};" : "=l"(x) : "f"(a.x), "f"(a.y));
@@ -272,29 +277,6 @@ __device__ __forceinline__ float2 add2(float2 a, float2 b) {
   float2 r;
   asm("mov.b64 {%0, %1}, %2;" : "=f"(r.x), "=f"(r.y) : "l"(d));
   return r;
-}
-
-#ifndef X_POLY
-#define X_POLY 1
-#endif
-// 2^x of two numbers of at most 2^7 on the fp32 units: x = n + r with |r| <= 1/2, a polynomial of degree 5 in r (its
-// coefficients minimise the largest relative error, 2e-7 in fp32) times 2^n. From -127 down, -inf too, it is 0; a NaN stays one.
-__device__ __forceinline__ float2 exp2_poly(float2 x) {
-  asm("max.NaN.f32 %0, %0, 0fC2FE0000;" : "+f"(x.x));  // -127
-  asm("max.NaN.f32 %0, %0, 0fC2FE0000;" : "+f"(x.y));
-  constexpr float kRound = 12582912.f;                  // 1.5 * 2^23: the sum's low bits are the nearest integer
-  const float2 t = add2(x, make_float2(kRound, kRound));
-  const float2 n = add2(t, make_float2(-kRound, -kRound));
-  const float2 r = add2(x, make_float2(-n.x, -n.y));
-  float2 p = make_float2(0.001327647129073739f, 0.001327647129073739f);
-  p = fma2(p, r, make_float2(0.009675541892647743f, 0.009675541892647743f));
-  p = fma2(p, r, make_float2(0.05550713092088699f, 0.05550713092088699f));
-  p = fma2(p, r, make_float2(0.24022120237350464f, 0.24022120237350464f));
-  p = fma2(p, r, make_float2(0.6931469440460205f, 0.6931469440460205f));
-  p = fma2(p, r, make_float2(1.0000001192092896f, 1.0000001192092896f));
-  const float2 scale = make_float2(__uint_as_float((__float_as_uint(t.x) << 23) + 0x3f800000u),
-                                   __uint_as_float((__float_as_uint(t.y) << 23) + 0x3f800000u));
-  return mul2(p, scale);
 }
 
 // Bits lo .. hi of a 32-bit word (either end may lie outside it).
@@ -436,7 +418,8 @@ __global__ void __launch_bounds__(Tiles<DP>::kThreads, DP == 64 ? 2 : 1)
     // 384 threads start with 168 registers each: 2 * 128 * 208 + 128 * 88 is as many
     if constexpr (DP == 128) asm volatile("setmaxnreg.dec.sync.aligned.u32 88;");
     // Both warps run as a whole, and one lane issues: what an instruction takes then stays in uniform registers. The
-    // products' issue is on the critical path (by one lane alone, with descriptors built for each: XXX us).
+    // products' issue is on the critical path (by one lane alone, with descriptors built for each, 8192 rows, window
+    // 4096: 557 us, so 489).
     if (warp == 8) {
       const bool lead = elect_one();
       const int kv = h0 / (a.heads / a.kv_heads);
@@ -583,36 +566,37 @@ __global__ void __launch_bounds__(Tiles<DP>::kThreads, DP == 64 ? 2 : 1)
       }
       if (!(ok = wait(&s_full[side], n))) break;
       tc_fence_after();
-      auto mask = [&](int b, float (&x)[32]) {
-        if (edge[b])
-#pragma unroll
-          for (int e = 0; e < 32; ++e) x[e] = (seen[b] >> e) & 1u ? x[e] : -INFINITY;
-      };
       // At 128 columns the registers hold the tile between the passes, at 64 (two CTAs an SM) it is read again.
       constexpr bool kKeep = DP == 128;
-      float x[kKeep ? G::kBlocks : 1][32], tops[4] = {-INFINITY, -INFINITY, -INFINITY, -INFINITY};
-      // a block's load is on its way while the one before it is looked at; four maxima, for the latency of each
-      auto look = [&](int b, float (&y)[32]) {
-        hold(y);
-        mask(b, y);
+      float x[kKeep ? 2 : 1][kKeep ? 64 : 32], tops[4] = {-INFINITY, -INFINITY, -INFINITY, -INFINITY};  // for latency
+      auto mask = [&](int b, auto& y, int from) {
+        if (edge[b])
 #pragma unroll
-        for (int e = 0; e < 32; e += 2) tops[e / 2 % 4] = max3(tops[e / 2 % 4], y[e], y[e + 1]);
+          for (int e = 0; e < 32; ++e) y[from + e] = (seen[b] >> e) & 1u ? y[from + e] : -INFINITY;
+      };
+      auto look = [&](auto& y, int from) {
+#pragma unroll
+        for (int e = 0; e < 32; e += 2) tops[e / 2 % 4] = max3(tops[e / 2 % 4], y[from + e], y[from + e + 1]);
       };
       if constexpr (kKeep) {
-        if (some[0]) tmem_ld32(my_s, x[0]);
 #pragma unroll
-        for (int b = 0; b < G::kBlocks; ++b) {
-          if (some[b]) tmem_ld_wait();
-          if (b + 1 < G::kBlocks && some[b + 1]) tmem_ld32(my_s + (b + 1) * 32, x[b + 1]);
-          if (some[b]) look(b, x[b]);
-        }
+        for (int half = 0; half < 2; ++half)
+          if (some[2 * half] || some[2 * half + 1]) {
+            tmem_ld64(my_s + half * 64, x[half]);
+#pragma unroll
+            for (int b = 0; b < 2; ++b)
+              if (some[2 * half + b]) {
+                mask(2 * half + b, x[half], b * 32);
+                look(x[half], b * 32);
+              }
+          }
       } else {
 #pragma unroll
         for (int b = 0; b < G::kBlocks; ++b)
           if (some[b]) {
             tmem_ld32(my_s + b * 32, x[0]);
-            tmem_ld_wait();
-            look(b, x[0]);
+            mask(b, x[0], 0);
+            look(x[0], 0);
           }
       }
       const float top = fmaxf(fmaxf(tops[0], tops[1]), fmaxf(tops[2], tops[3]));
@@ -628,8 +612,6 @@ __global__ void __launch_bounds__(Tiles<DP>::kThreads, DP == 64 ? 2 : 1)
           for (int d = 0; d < DP; d += 32) {
             float o[32];
             tmem_ld32(my_o + d, o);
-            tmem_ld_wait();
-            hold(o);
 #pragma unroll
             for (int e = 0; e < 32; ++e) o[e] *= keep;
             tmem_st32(my_o + d, o);
@@ -645,18 +627,16 @@ __global__ void __launch_bounds__(Tiles<DP>::kThreads, DP == 64 ? 2 : 1)
         if (b >= nb) break;
         unsigned p[16];
         if (some[b]) {
-          float(&y)[32] = x[kKeep ? b : 0];
-          if (!kKeep) {
-            tmem_ld32(my_s + b * 32, y);
-            tmem_ld_wait();
-            hold(y);
-            mask(b, y);
+          if constexpr (!kKeep) {
+            tmem_ld32(my_s + b * 32, x[0]);
+            mask(b, x[0], 0);
           }
+          auto& y = x[kKeep ? b / 2 : 0];
+          const int from = kKeep ? b % 2 * 32 : 0;
 #pragma unroll
           for (int e = 0; e < 16; ++e) {
-            float2 w = fma2(make_float2(y[2 * e], y[2 * e + 1]), c2, ref2);
-            if (e % 4 >= 4 - X_POLY) w = exp2_poly(w);
-            else w = make_float2(exp2_fast(w.x), exp2_fast(w.y));
+            float2 w = fma2(make_float2(y[from + 2 * e], y[from + 2 * e + 1]), c2, ref2);
+            w = make_float2(exp2_fast(w.x), exp2_fast(w.y));
             sums[e & 1] = add2(sums[e & 1], w);
             p[e] = pack2((T*)nullptr, w.x, w.y);
           }
@@ -682,11 +662,7 @@ __global__ void __launch_bounds__(Tiles<DP>::kThreads, DP == 64 ? 2 : 1)
 #pragma unroll
       for (int d = 0; d < DP; d += 32) {
         float o[32];
-        if (good) {
-          tmem_ld32(my_o + d, o);
-          tmem_ld_wait();
-          hold(o);
-        }
+        if (good) tmem_ld32(my_o + d, o);
         const float inv = good ? 1.f / l : NAN;
         if (inside)
 #pragma unroll
