@@ -9,13 +9,17 @@
 // 2^-24 turns, where an fp32 product would lose it to 2^-4).
 // A head's row is a group of lanes with 8 columns each; the mean square is a
 // shuffle sum inside the group. Every row is read once and written once: the
-// bound is memory.
+// bound is memory. The first rows of every group are on their way before the
+// CTA knows whose they are.
 #include "st_cache.cuh"
 #include "st_cache_host.h"
 
 namespace st {
 namespace {
 
+#ifndef X_MINB
+#define X_MINB 5
+#endif
 constexpr int kAppendThreads = 256;
 constexpr int kMaxPairs = ST_CACHE_MAX_HEAD_DIM / 2;
 
@@ -30,15 +34,43 @@ struct AppendArgs {
   const long long* positions;
   const int* starts;
   int rows, streams, heads, kv_heads, head_dim, rotary, sinks, window;
-  float epsilon;
+  float epsilon, per_column;  // per_column: 1 / head_dim
 };
 
+// 8 columns as they were loaded.
+template <typename T>
+struct Raw8 {
+  uint4 u[sizeof(T) / 2];
+  __device__ __forceinline__ void load(const T* p) {
+#pragma unroll
+    for (int i = 0; i < (int)sizeof(T) / 2; ++i) u[i] = reinterpret_cast<const uint4*>(p)[i];
+  }
+};
+constexpr int kAhead = 3;  // rows a group of lanes loads ahead of their use
+
 template <typename T, int LANES, bool INT4>
-__global__ void __launch_bounds__(kAppendThreads) k_cache_append(const AppendArgs a) {
-  __shared__ float2 turn[kMaxPairs];
+__global__ void __launch_bounds__(kAppendThreads, X_MINB) k_cache_append(const AppendArgs a) {
+  __shared__ alignas(16) float2 turn[kMaxPairs];
   __shared__ int sh_slot;
-  __shared__ int sh_stream;
   const int row = blockIdx.x, tid = threadIdx.x;
+  constexpr int kGroups = kAppendThreads / LANES;
+  const int lane = tid % LANES, col = lane * 8;
+  const unsigned mask = LANES == 32 ? 0xffffffffu : ((1u << LANES) - 1u) << ((tid & 31) / LANES * LANES);
+  const bool on = col < a.head_dim;
+  const int tasks = a.heads + 2 * a.kv_heads;
+  // task: a query head, then the key heads, then the value heads
+  auto source = [&](int task) {
+    const int k = task - a.heads, v = k - a.kv_heads;
+    return k < 0   ? static_cast<const T*>(a.q) + row * a.q_row + task * a.q_head + col
+           : v < 0 ? static_cast<const T*>(a.k) + row * a.k_row + k * a.k_head + col
+                   : static_cast<const T*>(a.v) + row * a.v_row + v * a.v_head + col;
+  };
+  Raw8<T> ahead[kAhead];
+#pragma unroll
+  for (int u = 0; u < kAhead; ++u) {
+    const int task = tid / LANES + u * kGroups;
+    if (on && task < tasks) ahead[u].load(source(task));
+  }
   // the stream that owns this row: the number of streams that end at or before it
   int stream = row, first = row, last = row + 1;
   if (a.starts) {
@@ -56,13 +88,17 @@ __global__ void __launch_bounds__(kAppendThreads) k_cache_append(const AppendArg
   const long long p0 = a.positions[stream];
   const bool idle = p0 < 0;
   const long long position = p0 + (row - first);
-  for (int p = tid; p < a.rotary; p += kAppendThreads) {
+  for (int p = tid; p < (a.rotary + 3) / 4 * 4; p += kAppendThreads) {  // a lane's 4 pairs: those past the last turn by 0
+    if (p >= a.rotary) {
+      turn[p] = make_float2(1.f, 0.f);
+      continue;
+    }
     const double t = (double)position * a.frequencies[p] * 0.15915494309189533577;  // 1 / (2 pi)
     float s, c;
     sincospif(2.f * (float)(t - rint(t)), &s, &c);
     turn[p] = make_float2(c, s);
   }
-  if (tid == 0) {
+  if (tid == kAppendThreads - 1) {  // in a warp that has no pairs, mostly
     // inserted: sink positions, and those the stream's last `window` rows hold
     const long long newest = p0 + (last - 1 - first);
     int slot = -1;
@@ -71,65 +107,65 @@ __global__ void __launch_bounds__(kAppendThreads) k_cache_append(const AppendArg
       else if (position > newest - a.window) slot = a.sinks + (int)((position - a.sinks) % a.window);
     }
     sh_slot = slot;
-    sh_stream = stream;
   }
   __syncthreads();
   const int slot = sh_slot;
-  const int lane = tid % LANES, col = lane * 8;
-  const unsigned mask = LANES == 32 ? 0xffffffffu : ((1u << LANES) - 1u) << ((tid & 31) / LANES * LANES);
-  const bool on = col < a.head_dim;
-  const int tasks = a.heads + 2 * a.kv_heads;
-  for (int task = tid / LANES; task < tasks; task += kAppendThreads / LANES) {
-    const bool is_q = task < a.heads, is_v = task >= a.heads + a.kv_heads;
-    const int head = is_q ? task : is_v ? task - a.heads - a.kv_heads : task - a.heads;
-    if (!is_q && slot < 0 && (is_v || !a.k_out)) continue;
-    const T* in = is_q ? static_cast<const T*>(a.q) + row * a.q_row + head * a.q_head
-                : is_v ? static_cast<const T*>(a.v) + row * a.v_row + head * a.v_head
-                       : static_cast<const T*>(a.k) + row * a.k_row + head * a.k_head;
-    float f[8] = {};
-    if (on && !idle) load8(in + col, f);
-    if (!is_v && !idle) {
-      const float* gain = is_q ? a.q_gain : a.k_gain;
-      if (gain) {
-        float sum = 0.f;
+  for (int first = tid / LANES; first < tasks; first += kAhead * kGroups) {
 #pragma unroll
-        for (int i = 0; i < 8; ++i) sum = fmaf(f[i], f[i], sum);
+    for (int u = 0; u < kAhead; ++u) {
+      const int task = first + u * kGroups;
+      if (task >= tasks) break;
+      const bool is_q = task < a.heads, is_v = task >= a.heads + a.kv_heads;
+      const int head = is_q ? task : is_v ? task - a.heads - a.kv_heads : task - a.heads;
+      float f[8] = {};
+      if (on && !idle) load8(reinterpret_cast<const T*>(ahead[u].u), f);
+      if (on && task + kAhead * kGroups < tasks) ahead[u].load(source(task + kAhead * kGroups));
+      if (!is_v && !idle) {
+        const float* gain = is_q ? a.q_gain : a.k_gain;
+        if (gain) {
+          float sum = 0.f;
 #pragma unroll
-        for (int o = 1; o < LANES; o *= 2) sum += __shfl_xor_sync(mask, sum, o);
-        const float scale = 1.0f / sqrtf(sum / (float)a.head_dim + a.epsilon);
+          for (int i = 0; i < 8; ++i) sum = fmaf(f[i], f[i], sum);
+#pragma unroll
+          for (int o = 1; o < LANES; o *= 2) sum += __shfl_xor_sync(mask, sum, o);
+          const float scale = rsqrtf(fmaf(sum, a.per_column, a.epsilon));
+          if (on) {
+            float g[8];
+            load8(gain + col, g);
+#pragma unroll
+            for (int i = 0; i < 8; ++i) f[i] = f[i] * scale * g[i];
+          }
+        }
+        if (col / 2 < a.rotary) {
+          const float4* w = reinterpret_cast<const float4*>(&turn[col / 2]);
+#pragma unroll
+          for (int i = 0; i < 2; ++i) {
+            const float4 t = w[i];
+            const float x0 = f[4 * i], y0 = f[4 * i + 1], x1 = f[4 * i + 2], y1 = f[4 * i + 3];
+            f[4 * i] = x0 * t.x - y0 * t.y;
+            f[4 * i + 1] = x0 * t.y + y0 * t.x;
+            f[4 * i + 2] = x1 * t.z - y1 * t.w;
+            f[4 * i + 3] = x1 * t.w + y1 * t.z;
+          }
+        }
+      }
+      if (is_q) {
+        if (on) store8(static_cast<T*>(a.q_out) + row * a.qo_row + head * a.qo_head + col, f);
+        continue;
+      }
+      if (!is_v && a.k_out && on) store8(static_cast<T*>(a.k_out) + row * a.ko_row + head * a.ko_head + col, f);
+      if (slot < 0) continue;
+      const long long at = stream * a.stream_stride + head * a.head_stride + slot;
+      if (INT4) {
+        unsigned pair;
+        const unsigned codes = encode8(f, mask, &pair);
         if (on) {
-          float g[8];
-          load8(gain + col, g);
-#pragma unroll
-          for (int i = 0; i < 8; ++i) f[i] = f[i] * scale * g[i];
+          static_cast<unsigned*>(is_v ? a.values : a.keys)[at * (a.head_dim / 8) + lane] = codes;
+          if (lane % 4 == 0) (is_v ? a.value_scales : a.key_scales)[at * (a.head_dim / 32) + lane / 4] = pair;
         }
+      } else if (on) {
+        store8(static_cast<T*>(is_v ? a.values : a.keys) + at * a.head_dim + col, f);
       }
-#pragma unroll
-      for (int i = 0; i < 4; ++i) {
-        if (col / 2 + i < a.rotary) {
-          const float2 t = turn[col / 2 + i];
-          const float x = f[2 * i], y = f[2 * i + 1];
-          f[2 * i] = x * t.x - y * t.y;
-          f[2 * i + 1] = x * t.y + y * t.x;
-        }
-      }
-    }
-    if (is_q) {
-      if (on) store8(static_cast<T*>(a.q_out) + row * a.qo_row + head * a.qo_head + col, f);
-      continue;
-    }
-    if (!is_v && a.k_out && on) store8(static_cast<T*>(a.k_out) + row * a.ko_row + head * a.ko_head + col, f);
-    if (slot < 0) continue;
-    const long long at = stream * a.stream_stride + head * a.head_stride + slot;
-    if (INT4) {
-      unsigned pair;
-      const unsigned codes = encode8(f, mask, &pair);
-      if (on) {
-        static_cast<unsigned*>(is_v ? a.values : a.keys)[at * (a.head_dim / 8) + lane] = codes;
-        if (lane % 4 == 0) (is_v ? a.value_scales : a.key_scales)[at * (a.head_dim / 32) + lane / 4] = pair;
-      }
-    } else if (on) {
-      store8(static_cast<T*>(is_v ? a.values : a.keys) + at * a.head_dim + col, f);
     }
   }
 }
@@ -150,21 +186,25 @@ struct UnpackArgs {
   const unsigned* codes[2];
   const unsigned* scales[2];
   void* out[2];
-  long long stream_stride, head_stride, total;  // total: 8-column pieces of one side
-  int heads, slots, pieces;                     // pieces per row
+  long long stream_stride, head_stride;
+  int heads, slots, pieces;  // pieces: of 8 columns, per row
 };
 
+// A thread takes 8 columns of a key row and of the value row beside it.
 template <typename T>
 __global__ void __launch_bounds__(256) k_cache_unpack(const UnpackArgs a) {
-  const int side = blockIdx.y;
-  for (long long i = blockIdx.x * 256ll + threadIdx.x; i < a.total; i += gridDim.x * 256ll) {
-    const long long r = i / a.pieces;
-    const int piece = (int)(i - r * a.pieces);
-    const long long sh = r / a.slots, stream = sh / a.heads;
-    const long long at = stream * a.stream_stride + (sh - stream * a.heads) * a.head_stride + (r - sh * a.slots);
+  const long long begin = blockIdx.x * 256ll;
+  const int head = blockIdx.y, stream = blockIdx.z;
+  const int slot0 = (int)(begin / a.pieces), local = (int)(begin - (long long)slot0 * a.pieces) + threadIdx.x;
+  const int slot = slot0 + local / a.pieces, piece = local % a.pieces;
+  if (slot >= a.slots) return;
+  const long long at = stream * a.stream_stride + head * a.head_stride + slot;
+  const long long to = (((long long)stream * a.heads + head) * a.slots + slot) * a.pieces + piece;
+#pragma unroll
+  for (int side = 0; side < 2; ++side) {
     float f[8];
     decode8(a.codes[side][at * a.pieces + piece], a.scales[side][at * (a.pieces / 4) + piece / 4], f);
-    store8(static_cast<T*>(a.out[side]) + i * 8, f);
+    store8(static_cast<T*>(a.out[side]) + to * 8, f);
   }
 }
 
@@ -215,6 +255,7 @@ int st_cache_append(const st_cache* c, const st_append* p, void* stream) {
   a.positions = reinterpret_cast<const long long*>(p->positions); a.starts = p->starts;
   a.rows = (int)p->rows; a.streams = c->streams; a.heads = p->heads; a.kv_heads = c->heads;
   a.head_dim = c->head_dim; a.rotary = p->rotary; a.sinks = c->sinks; a.window = c->window; a.epsilon = p->epsilon;
+  a.per_column = 1.0f / (float)c->head_dim;
   cudaStream_t s = static_cast<cudaStream_t>(stream);
   const bool four = c->type == ST_CACHE_INT4;
   if (p->mode == ST_MODE_FP32) launch_append<float, false>(a, s);
@@ -239,9 +280,7 @@ int st_cache_unpack(const st_cache* c, int mode, void* keys, void* values, void*
   a.out[0] = keys; a.out[1] = values;
   a.stream_stride = c->stream_stride; a.head_stride = c->head_stride;
   a.heads = c->heads; a.slots = c->sinks + c->window; a.pieces = c->head_dim / 8;
-  a.total = (long long)c->streams * c->heads * a.slots * a.pieces;
-  const long long need = (a.total + 255) / 256, most = 16ll * sm_count(c->device);
-  const dim3 grid((unsigned)(need < most ? need : most), 2);
+  const dim3 grid((unsigned)(((long long)a.slots * a.pieces + 255) / 256), c->heads, c->streams);
   cudaStream_t s = static_cast<cudaStream_t>(stream);
   if (mode == ST_MODE_FP32) k_cache_unpack<float><<<grid, 256, 0, s>>>(a);
   else if (mode == ST_MODE_FP16) k_cache_unpack<__half><<<grid, 256, 0, s>>>(a);
