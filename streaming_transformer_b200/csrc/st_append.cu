@@ -17,9 +17,6 @@
 namespace st {
 namespace {
 
-#ifndef X_MINB
-#define X_MINB 5
-#endif
 constexpr int kAppendThreads = 256;
 constexpr int kMaxPairs = ST_CACHE_MAX_HEAD_DIM / 2;
 
@@ -49,7 +46,7 @@ struct Raw8 {
 constexpr int kAhead = 3;  // rows a group of lanes loads ahead of their use
 
 template <typename T, int LANES, bool INT4>
-__global__ void __launch_bounds__(kAppendThreads, X_MINB) k_cache_append(const AppendArgs a) {
+__global__ void __launch_bounds__(kAppendThreads, 5) k_cache_append(const AppendArgs a) {
   __shared__ alignas(16) float2 turn[kMaxPairs];
   __shared__ int sh_slot;
   const int row = blockIdx.x, tid = threadIdx.x;

@@ -104,10 +104,11 @@ __device__ __forceinline__ unsigned encode8(const float (&f)[8], unsigned mask, 
   const float s = __bfloat162float(s16), l = __bfloat162float(l16);
   unsigned codes = 0;
   if (s > 0.f) {
+    // 1.5 * 2^23 + c is c rounded to the nearest integer, ties to even, in the sum's low bits
 #pragma unroll
     for (int i = 0; i < 8; ++i) {
-      const float c = rintf(__fdiv_rn(__fsub_rn(f[i], l), s));
-      codes |= (unsigned)fminf(fmaxf(c, 0.f), 15.f) << (4 * i);
+      const float c = fminf(fmaxf(__fdiv_rn(__fsub_rn(f[i], l), s), 0.f), 15.f);
+      codes |= (__float_as_uint(__fadd_rn(c, 12582912.f)) & 15u) << (4 * i);
     }
   }
   *pair = (unsigned)__bfloat16_as_ushort(s16) | ((unsigned)__bfloat16_as_ushort(l16) << 16);
