@@ -309,7 +309,8 @@ typedef struct {
  * rows == streams) at positions positions[s], positions[s] + 1, ... A stream at
  * a negative position is idle: its cache stays, and its rows of q_out and k_out
  * become 0. Rows before starts[0] or behind the last stream's are left as they
- * were. Of a stream's new rows only those still in the window, or at a sink
+ * were. q_out may be q itself and k_out k itself; beyond that nothing written
+ * may overlap anything read. Positions stay below 2^53. Of a stream's new rows only those still in the window, or at a sink
  * position, are inserted. Sums and angles are fp32 or wider; each output is
  * rounded once (4-bit rows are quantised from the fp32 values). */
 typedef struct {
@@ -317,8 +318,8 @@ typedef struct {
   int heads;                /* query heads */
   int64_t rows;             /* rows of q, k, v, up to 2^31 - 1 */
   st_rows q, k, v;
-  st_rows q_out;            /* normed and rotated queries; may be q itself */
-  st_rows k_out;            /* the same of the keys, or data NULL; may be k itself */
+  st_rows q_out;            /* normed and rotated queries */
+  st_rows k_out;            /* the same of the keys, or data NULL */
   const float *q_gain, *k_gain; /* [head_dim], or NULL */
   float epsilon;            /* >= 0 */
   int rotary;               /* rotated pairs, 0 .. head_dim / 2 */
@@ -332,7 +333,7 @@ int st_cache_append(const st_cache* cache, const st_append* args, void* stream);
  * the slots 0 .. min(position + 1, sinks + window) - 1 of key head
  * h / (heads / cache heads), position being that of the newest inserted row.
  * Slots past those are not looked at, whatever they hold. A negative position
- * gives a row of zeros.
+ * gives a row of zeros. out may be q itself.
  * `workspace` holds the partial results of a split over the slots:
  * st_cache_attention_workspace() bytes (0 for some shapes; then NULL will do),
  * on a 256-byte boundary. Calls that may overlap need workspaces of their own. */
@@ -356,14 +357,16 @@ int st_cache_unpack(const st_cache* cache, int mode, void* keys, void* values, v
  * sequence sees that sequence's rows j <= i with i - j < window or j < sinks.
  * Sequence s is rows starts[s] .. starts[s + 1] - 1 (starts NULL: one
  * sequence, all rows). Rows outside every sequence are not read into any
- * result and their outputs are left as they were. */
+ * result and their outputs are left as they were. A value that is not finite
+ * reaches the rows that see it and no other; such tiles are done twice, the
+ * second time slowly. out may not overlap q, k or v. */
 typedef struct {
   int device;
   int mode;                 /* st_mode of q, k, v and out */
   int heads, kv_heads;      /* heads a multiple of kv_heads */
   int head_dim;             /* a multiple of 8 up to 256 */
   int sequences;
-  int64_t rows;             /* up to 2^31 - 1 */
+  int64_t rows;             /* up to 2^30 */
   int window, sinks;        /* window >= 1, sinks >= 0 */
   float scale;
   st_rows q, k, v, out;

@@ -69,7 +69,7 @@ def new_cache(streams: int, heads: int, window: int, head_dim: int, *, sinks: in
     """An empty cache: (keys, values, key_scales, value_scales), zeroed. ``mode``
     is "fp32", "mixed" (fp16), "bf16" or "int4"; the scales are None unless "int4"."""
     rows = (int(streams), int(heads), int(sinks) + int(window))
-    if min(rows) < 1 or sinks < 0 or window < 1 or head_dim < 8 or head_dim % (GROUP if mode == "int4" else 8):
+    if min(rows) < 1 or sinks < 0 or window < 1 or not 8 <= head_dim <= 256 or head_dim % (GROUP if mode == "int4" else 8):
         _refuse("invalid cache dimensions")
     if mode == "int4":
         def scales():
@@ -116,7 +116,7 @@ def cache_attention(q, keys, values, positions, *, key_scales=None, value_scales
     q [streams, heads, head_dim], heads a multiple of the cache's;
     ``positions`` int64 [streams], the position of each stream's newest inserted
     row (negative: a row of zeros). Every slot up to min(position + 1, slots)
-    is seen. ``scale`` defaults to head_dim ** -0.5."""
+    is seen. ``scale`` defaults to head_dim ** -0.5; ``out`` may be q."""
     return _native.attend(q, keys, values, positions, key_scales, value_scales, scale, out)
 
 
@@ -135,5 +135,5 @@ def window_attention(q, k, v, *, window: int, sinks: int = 0, starts=None, scale
     multiple of the key heads; ``starts`` int32 [sequences + 1], or None for one
     sequence. Row i of a sequence sees that sequence's rows j <= i with
     i - j < window or j < sinks. Rows of no sequence are left as they were in
-    ``out``, and undefined in a fresh tensor."""
+    ``out``, which may not overlap an input, and undefined in a fresh tensor."""
     return _native.window(q, k, v, window, sinks, starts, scale, out)

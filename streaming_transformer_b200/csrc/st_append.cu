@@ -99,7 +99,7 @@ __global__ void __launch_bounds__(kAppendThreads, 5) k_cache_append(const Append
     // inserted: sink positions, and those the stream's last `window` rows hold
     const long long newest = p0 + (last - 1 - first);
     int slot = -1;
-    if (!idle) {
+    if (!idle && position >= 0) {  // a sum past 2^63 is not inserted
       if (position < a.sinks) slot = (int)position;
       else if (position > newest - a.window) slot = a.sinks + (int)((position - a.sinks) % a.window);
     }

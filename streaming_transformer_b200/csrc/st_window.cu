@@ -946,7 +946,7 @@ extern "C" int st_window_attention(const st_window* p, void* stream) {
     return cache_fail(ST_ERR_INVALID, "query heads are a multiple of the key heads, up to 65535");
   if (p->head_dim < 8 || p->head_dim > ST_CACHE_MAX_HEAD_DIM || p->head_dim % 8)
     return cache_fail(ST_ERR_INVALID, "head_dim is a multiple of 8 up to 256");
-  if (p->rows < 0 || p->rows > INT32_MAX) return cache_fail(ST_ERR_INVALID, "rows are 0 to 2^31 - 1");
+  if (p->rows < 0 || p->rows > (1 << 30)) return cache_fail(ST_ERR_INVALID, "rows are 0 to 2^30");
   if (p->window < 1 || p->sinks < 0) return cache_fail(ST_ERR_INVALID, "window is at least 1 and sinks at least 0");
   if (p->starts ? p->sequences < 0 : p->sequences != 1)
     return cache_fail(ST_ERR_INVALID, "without starts there is one sequence");
@@ -958,6 +958,8 @@ extern "C" int st_window_attention(const st_window* p, void* stream) {
       (rc = check_rows(p->v, "v", p->mode, p->rows, p->kv_heads, p->head_dim, false)) != ST_OK ||
       (rc = check_rows(p->out, "out", p->mode, p->rows, p->heads, p->head_dim, true)) != ST_OK)
     return rc;
+  if (p->out.data == p->q.data || p->out.data == p->k.data || p->out.data == p->v.data)
+    return cache_fail(ST_ERR_INVALID, "out may not be an input");
   DeviceScope scope(p->device);
   if (scope.status() != ST_OK) return scope.status();
   WindowArgs a{};

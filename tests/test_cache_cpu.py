@@ -88,7 +88,7 @@ def attend(**change):
 def window(**change):
     a = Window()
     a.mode, a.heads, a.kv_heads, a.head_dim, a.sequences, a.rows, a.window, a.sinks, a.scale = 2, 4, 2, 64, 1, 10, 5, 1, 0.125
-    a.q, a.k, a.v, a.out = rows(4), rows(2), rows(2), rows(4)
+    a.q, a.k, a.v, a.out = rows(4), rows(2), rows(2), Rows(2 * P, 256, 64)
     for k, v in change.items():
         setattr(a, k, v)
     return a
@@ -165,7 +165,7 @@ def test_attention_arguments_that_are_refused(change, match):
 
 @pytest.mark.parametrize("change,match", [
     (dict(device=-1), "device"), (dict(mode=4), "row mode"), (dict(heads=3), "multiple of the key heads"), (dict(kv_heads=0), "key heads"),
-    (dict(head_dim=68), "multiple of 8"), (dict(head_dim=512), "up to 256"), (dict(rows=2 ** 31), "rows are"),
+    (dict(head_dim=68), "multiple of 8"), (dict(head_dim=512), "up to 256"), (dict(rows=2 ** 30 + 1), "rows are"), (dict(out=rows(4)), "may not be an input"),
     (dict(window=0), "window"), (dict(sinks=-1), "sinks"), (dict(sequences=2), "one sequence"),
     (dict(sequences=-1, starts=P), "one sequence"), (dict(scale=float("nan")), "scale"), (dict(q=Rows(P + 8, 256, 64)), "q: must start"),
     (dict(k=Rows(P, 128, 4)), "k: strides must be"), (dict(out=Rows(P, 256, 32)), "out: strides let"),
@@ -191,6 +191,6 @@ def test_new_cache_shapes_and_refusals():
     assert k.shape == v.shape == (2, 3, 7, 32) and ks.shape == vs.shape == (2, 3, 7, 2, 2)
     k, v, ks, vs = ops.new_cache(1, 1, 1, 8, mode="fp32", device="cpu")
     assert k.shape == (1, 1, 1, 8) and ks is None and vs is None
-    for bad in (dict(window=0), dict(streams=0), dict(head_dim=12), dict(head_dim=80, mode="int4"), dict(sinks=-1), dict(mode="int8")):
+    for bad in (dict(window=0), dict(streams=0), dict(head_dim=12), dict(head_dim=264), dict(head_dim=80, mode="int4"), dict(sinks=-1), dict(mode="int8")):
         with pytest.raises(StreamError):
             ops.new_cache(**{**dict(streams=1, heads=1, window=4, head_dim=64, device="cpu"), **bad})

@@ -70,6 +70,9 @@ APPEND = [
     ("int4", 4, 2, 32, 5, 0, [1, 9], 2, 16, False),
     ("int4", 6, 2, 96, 11, 1, [12, 12], 2, 40, True),
     ("int4", 2, 1, 256, 4, 0, [5], 1, 128, True),
+    ("int4", 3, 3, 224, 9, 1, [14], 1, 112, True),
+    ("bf16", 2, 1, 200, 12, 2, None, 3, 51, True),
+    ("mixed", 40, 20, 128, 7, 1, None, 5, 64, True),       # more rows than a CTA's lanes hold at a time
 ]
 
 
@@ -225,6 +228,15 @@ ATTEND = [
     ("int4", "bf16", 9, 1, 32, 65, [64, 3]),
     ("int4", "bf16", 20, 1, 256, 95, [94, 47]),
     ("int4", "bf16", 16, 1, 128, 30000, [29999]),
+    ("bf16", None, 6, 2, 72, 100, [99, 31]),
+    ("mixed", None, 3, 1, 136, 61, [60, 15]),
+    ("bf16", None, 1, 1, 200, 40, [39]),
+    ("bf16", None, 5, 5, 8, 33, [32, 5]),
+    ("int4", "bf16", 4, 2, 160, 70, [69, 16]),
+    ("int4", "mixed", 2, 2, 192, 35, [34]),
+    ("int4", "bf16", 12, 1, 224, 130, [129, 64]),
+    ("int4", "bf16", 3, 3, 32, 3000, [2999]),
+    ("fp32", None, 5, 5, 24, 4100, [4099, 77]),
 ]
 
 
@@ -249,7 +261,7 @@ def test_cache_attention_matches_the_definition(case):
     cache, held = filled_cache(g, len(at), kv, slots, dim, 0, mode)
     q = normal(g, len(at), heads, dim, dtype=dtype)
     positions = torch.tensor(at, dtype=torch.int64, device="cuda")
-    for scale in (None, 0.7):
+    for scale in (None, 0.7, -0.2, 0.0):
         got = ops.cache_attention(q, *cache[:2], positions, scale=scale, **scales_of(cache))
         want, bound = attend_reference(q, held, at, dim ** -0.5 if scale is None else scale, dtype)
         ref.check(got, want, bound, f"scale {scale}")
@@ -313,6 +325,49 @@ def test_large_and_equal_logits(mode):
     want = torch.stack([values[0, 0, 0::2].double().mean(0), values[0, 0, 1::2].double().mean(0)])[None]
     size = torch.stack([values[0, 0, 0::2].double().abs().mean(0), values[0, 0, 1::2].double().abs().mean(0)])[None]
     ref.check(got, want, (2 * ref.unit(dtype) + 200 * ref.F) * size + ref.TINY[dtype])
+
+
+@pytest.mark.parametrize("rows", ["mixed", "bf16"])
+@pytest.mark.parametrize("q_size,k_size,v_size", [(1e4, 1e-4, 1.0), (1e-4, 1e3, 1e-9), (3.0, 1.0, 1e4), (2.0 ** -14, 1.0, 1.0), (0.0, 1.0, 1.0)])
+def test_four_bit_attention_over_a_range_of_sizes(rows, q_size, k_size, v_size):
+    # queries are scaled by a power of two and values' scales folded into the weights: neither may lose small or large ones
+    g = generator(21)
+    dtype = TYPES[rows]
+    packed, scales, held = [], [], []
+    for size in (k_size, v_size):
+        codes, s, low = ref.quantise(normal(g, 2, 2, 90, 64) * size)
+        packed.append(ref.pack(codes))
+        scales.append(torch.stack([s, low], -1))
+        held.append(ref.unpack(packed[-1], scales[-1]))
+        held.append((15 * s.double() + low.double().abs()).repeat_interleave(32, -1))
+    held = (held[0], held[2], held[1], held[3])
+    q = (normal(g, 2, 4, 64) * q_size).to(dtype)
+    q[:, :, :8] *= 2.0 ** -10                       # and columns far below the largest
+    at = [89, 40]
+    got = ops.cache_attention(q, *packed, torch.tensor(at, device="cuda"), key_scales=scales[0], value_scales=scales[1])
+    want, bound = attend_reference(q, held, at, 0.125, dtype)
+    ref.check(got, want, bound)
+
+
+def test_cache_attention_in_place():
+    g = generator(22)
+    for mode, slots in (("bf16", 100), ("bf16", 5000), ("fp32", 100)):
+        dtype = TYPES[mode]
+        cache, _ = filled_cache(g, 2, 2, slots, 64, 0, mode)
+        q = normal(g, 2, 8, 64, dtype=dtype)
+        at = torch.tensor([slots - 1, 40], device="cuda")
+        want = ops.cache_attention(q, *cache[:2], at)
+        assert ops.cache_attention(q, *cache[:2], at, out=q) is q
+        assert torch.equal(q, want)
+
+
+def test_append_past_the_last_position_stays_in_bounds():
+    guard = torch.zeros(3, 2, 8, 64, dtype=torch.bfloat16, device="cuda")
+    keys, values = guard[1:2], torch.zeros_like(guard)[1:2]
+    x = torch.ones(4, 2, 64, dtype=torch.bfloat16, device="cuda")
+    at = torch.tensor([2 ** 63 - 2], device="cuda")
+    ops.cache_append(x, x, x, keys, values, at, ops.rotation_frequencies(64), starts=starts_of([4]))
+    assert not guard[0].any() and not guard[2].any()
 
 
 def test_cache_attention_over_strided_and_broadcast_caches():
@@ -403,7 +458,7 @@ def test_window_attention_matches_the_definition(case):
             x[n - 3:] = float("inf")
     starts = starts_of(sizes, before) if sizes else None
     edges = starts.tolist() if sizes else [0, n]
-    for scale in (None, 0.3):
+    for scale in (None, 0.3, -0.2, 0.0):
         out = torch.full((n, heads, dim), 7.0, dtype=dtype, device="cuda")
         ops.window_attention(q, k, v, window=window, sinks=sinks, starts=starts, scale=scale, out=out)
         assert (out[:edges[0]] == 7).all() and (out[edges[-1]:] == 7).all(), "rows of no sequence"
@@ -443,6 +498,53 @@ def test_window_attention_of_strided_rows(mode):
     ops.window_attention(q, shared, v, window=50, sinks=3, out=out.transpose(0, 1))
     for a, b, want, bound in window_reference(q, shared, v, [0, n], 50, 3, 0.125, dtype):
         ref.check(out.transpose(0, 1)[a:b], want, bound)
+
+
+@pytest.mark.parametrize("mode", ["fp32", "bf16"])
+def test_window_attention_of_one_repeated_key_row(mode):
+    # a row stride of 0: every position has the same key and value, so every row is that value, to one rounding of it
+    # and the weights' (u(T) each) and sums'
+    g = generator(23)
+    dtype = TYPES[mode]
+    k, v = (normal(g, 1, 2, 64, dtype=dtype).expand(300, -1, -1) for _ in range(2))
+    got = ops.window_attention(normal(g, 300, 2, 64, dtype=dtype), k, v, window=100, sinks=2)
+    ref.check(got, v.double(), v.double().abs() * (2 * ref.unit(dtype) + 300 * ref.F) + ref.TINY[dtype])
+
+
+@pytest.mark.parametrize("mode", ["fp32", "mixed", "bf16"])
+def test_many_short_and_skipped_key_tiles(mode):
+    # long gaps between a tile's sinks and its window: key tiles that one of a CTA's two query tiles needs and the
+    # other does not, for an odd and an even number of heads a key head
+    g = generator(24)
+    dtype = TYPES[mode]
+    for heads, kv, dim in ((3, 3, 64), (4, 2, 64), (3, 1, 128), (4, 1, 128)):
+        sizes = [700, 1, 390, 133]
+        n = sum(sizes)
+        q, k, v = (normal(g, n, h, dim, dtype=dtype) for h in (heads, kv, kv))
+        for window, sinks in ((20, 150), (3, 1), (129, 70)):
+            got = ops.window_attention(q, k, v, window=window, sinks=sinks, starts=starts_of(sizes))
+            for a, b, want, bound in window_reference(q, k, v, starts_of(sizes).tolist(), window, sinks, dim ** -0.5, dtype):
+                ref.check(got[a:b], want, bound, f"{heads} heads, window {window}, rows {a}..{b}")
+
+
+def test_a_captured_backlog_replays_with_other_starts():
+    g = generator(25)
+    n, window, sinks = 400, 90, 3
+    q, k, v = (normal(g, n, h, 64, dtype=torch.bfloat16) for h in (4, 2, 2))
+    starts = starts_of([100, 300, 0])
+    ops.window_attention(q, k, v, window=window, sinks=sinks, starts=starts)
+    graph, side = torch.cuda.CUDAGraph(), torch.cuda.Stream()
+    side.wait_stream(torch.cuda.current_stream())
+    with torch.cuda.stream(side), torch.cuda.graph(graph, stream=side):
+        out = ops.window_attention(q, k, v, window=window, sinks=sinks, starts=starts)
+    torch.cuda.current_stream().wait_stream(side)
+    for sizes in ([300, 40, 60], [1, 1, 398]):
+        starts.copy_(starts_of(sizes))
+        q.copy_(normal(g, *q.shape))
+        graph.replay()
+        assert torch.equal(out, ops.window_attention(q, k, v, window=window, sinks=sinks, starts=starts))
+        for a, b, want, bound in window_reference(q, k, v, starts.tolist(), window, sinks, 0.125, torch.bfloat16):
+            ref.check(out[a:b], want, bound)
 
 
 # ---------------------------------------------------------------- together
