@@ -608,7 +608,7 @@ __global__ void __launch_bounds__(kAttendThreads) k_attend_fp32(const AttendArgs
   const long long row0 = stream * a.stream_stride + kv * a.head_stride;
   const float* kp = static_cast<const float*>(a.keys) + row0 * a.head_dim + lane * 8;
   const float* vp = static_cast<const float*>(a.values) + row0 * a.head_dim + lane * 8;
-  constexpr int U = 2;   // slots a group loads before it uses them
+  constexpr int U = GT == 1 ? 4 : 2;   // slots a group loads before it uses them; 4 at GT 2: 31 -> 40 us at 256 streams
   for (int base = first; base < last; base += kGroups * U) {
     float k[U][8] = {}, v[U][8] = {};
 #pragma unroll
@@ -735,13 +735,17 @@ int heads_per_block(const st_cache* c, int heads) {
   return group <= 8 || c->head_dim > 128 ? 8 : 16;
 }
 
-// CTAs that share the slots of one key head: one for each SM while each still
-// has 64 slots (a tile a warp), and up to 12 for each SM while each has 512, so
-// that streams of uneven lengths even out. Measured (us): see the launch below.
+// CTAs that share the slots of one key head. One for each SM while each still has
+// 64 slots, if that makes at least 6 of them (the join costs 1.5 us: one stream of
+// 16 heads, 260 slots, takes 4.6 us whole and 5.2 in 4 parts, with 504 slots 6.2
+// whole and 5.2 in 7); up to 12 for each SM while each has 512, so that streams of
+// uneven lengths even out (6, 8 and 12 for each SM: 64, 60 and 61 us at fp16, 129,
+// 123 and 117 at 4 bits; one stream of 131076 slots 88, 92 and 93).
 int splits_of(const st_cache* c, int heads) {
   const int per = heads_per_block(c, heads), group = heads / c->heads, slots = c->sinks + c->window;
   const long long ctas = (long long)c->streams * c->heads * ((group + per - 1) / per), sms = sm_count(c->device);
-  const long long fill = std::min<long long>(sms / ctas, slots / 64);
+  long long fill = std::min<long long>(sms / ctas, slots / 64);
+  if (fill < 6) fill = 1;
   const long long even = std::min<long long>(12 * sms / ctas, slots / 512);
   return (int)std::min<long long>(std::max<long long>({fill, even, 1}), kMaxSplits);
 }

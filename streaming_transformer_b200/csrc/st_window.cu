@@ -124,10 +124,10 @@ __global__ void __launch_bounds__(kWindowThreads) k_window_rows(const WindowArgs
 // ---------------------------------------------------------------- tcgen05
 constexpr int kTileRows = 128;      // query rows of a CTA: TMEM lanes
 constexpr int kBlockRows = 32;      // key rows of one copy
-constexpr int kWaitTries = 1 << 26;  // about two seconds
+constexpr int kWaitTries = 1 << 26;  // a second or two
 
 // Whether a phase of `bar` completed within the limit. It polls: a try_wait that suspends the thread costs more to
-// wake from than most of these waits last (8192 rows, window 4096: XXX us with it).
+// wake from than most of these waits last (8192 rows, window 4096: 641 us with it, 557 without).
 __device__ __forceinline__ bool wait_phase(unsigned long long* bar, unsigned parity) {
 #pragma unroll 1
   for (int i = 0; i < kWaitTries; ++i)
@@ -701,15 +701,17 @@ __global__ void __launch_bounds__(Tiles<DP>::kThreads, DP == 64 ? 2 : 1)
 // ---------------------------------------------------------------- fp32 tiles
 // 32 query rows of one head by 128 threads; thread (ty, tx) of 8 x 16 has rows
 // 4 ty .. + 3 of everything, keys tx + 16 i of a 64-key tile in S, columns
-// 64 i + 4 tx .. + 3 of O. 16 multiply-adds for each 32 bytes read from shared
+// 64 i + 4 tx .. + 3 of O: 16 multiply-adds for each 32 bytes read from shared
 // memory, rows padded by 16 bytes against bank conflicts. Key rows of the next
-// tile load under the second product, value rows under the first.
-constexpr int kFp32Rows = 32, kFp32Keys = 64, kFp32Threads = 128;
+// tile load under the second product, value rows under the first. 64 query rows
+// (8 a thread) read less and were slower, with half the warps an SM (2500 rows,
+// window 300, 32 heads of 64: 269 us against 226, a third of the fp32 rate).
+constexpr int kFp32Keys = 64, kFp32Threads = 128, kRowsEach = 4;
 
 template <int DP>
 struct Fp32Tiles {
-  static constexpr int kRow = DP + 4, kPRow = kFp32Keys + 4;
-  static constexpr int kFloats = (kFp32Rows + 2 * kFp32Keys) * kRow + kFp32Rows * kPRow;
+  static constexpr int kRows = 8 * kRowsEach, kRow = DP + 4, kPRow = kFp32Keys + 4;
+  static constexpr int kFloats = (kRows + 2 * kFp32Keys) * kRow + kRows * kPRow;
   static constexpr int kSmem = kFloats * 4;
 };
 
@@ -720,73 +722,79 @@ __device__ __forceinline__ void copy16(float* dst, const float* src, bool in) {
 template <int DP>
 __global__ void __launch_bounds__(kFp32Threads) k_window_fp32(const WindowArgs a) {
   using G = Fp32Tiles<DP>;
+  constexpr int RT = kRowsEach;
   extern __shared__ float4 dynamic[];
   float* sq = reinterpret_cast<float*>(dynamic);
-  float *sk = sq + kFp32Rows * G::kRow, *sv = sk + kFp32Keys * G::kRow, *sp = sv + kFp32Keys * G::kRow;
+  float *sk = sq + G::kRows * G::kRow, *sv = sk + kFp32Keys * G::kRow, *sp = sv + kFp32Keys * G::kRow;
   __shared__ int sh_slow;
   const int h = blockIdx.x % a.heads, tile = gridDim.x / a.heads - 1 - blockIdx.x / a.heads, kv = h / (a.heads / a.kv_heads);
   TileKeys keys;
-  if (!tile_keys(a, (long long)tile * kFp32Rows, kFp32Rows, keys)) return;
+  if (!tile_keys(a, (long long)tile * G::kRows, G::kRows, keys)) return;
   const int ty = threadIdx.x / 16, tx = threadIdx.x % 16;
   if (threadIdx.x == 0) sh_slow = 0;
-  // rows of a block beyond the tile's last, and columns past head_dim, are zeros
-  auto copy_rows = [&](float* dst, const void* src, long long row_stride, long long head, int block0) {
+  // A thread copies one column piece of every kStep-th row. Rows past the input, blocks past the tile's last and
+  // columns past head_dim are zeros.
+  constexpr int kPieces = DP / 4, kStep = kFp32Threads / kPieces;
+  const int piece = threadIdx.x % kPieces * 4, my_row = threadIdx.x / kPieces;
+  const bool on = piece < a.head_dim;
+  auto copy_rows = [&](float* dst, const float* src, long long stride, long long row, int count, int most) {
+    const float* p = src + (row + my_row) * stride + piece;
+    dst += my_row * G::kRow + piece;
+#pragma unroll
+    for (int r = my_row; r < count; r += kStep, dst += kStep * G::kRow, p += kStep * stride) {
+      const bool in = on && r < most;
+      copy16(dst, in ? p : src, in);
+    }
+  };
+  auto copy_tile = [&](float* dst, const void* src, long long stride, long long head, int block0) {
     const float* p = static_cast<const float*>(src) + head;
-    for (int e = threadIdx.x; e < kFp32Keys * (DP / 4); e += kFp32Threads) {
-      const int r = e / (DP / 4), c = e % (DP / 4), block = block0 + r / kBlockRows;
-      const int row = block < keys.blocks ? keys.base(block) + r % kBlockRows : a.rows;
-      const bool in = row < a.rows && c * 4 < a.head_dim;
-      copy16(dst + r * G::kRow + c * 4, p + (in ? row * row_stride + c * 4 : 0), in);
+#pragma unroll
+    for (int b = 0; b < 2; ++b) {
+      const int block = block0 + b, row = block < keys.blocks ? keys.base(block) : 0;
+      copy_rows(dst + b * kBlockRows * G::kRow, p, stride, row, kBlockRows,
+                block < keys.blocks ? min(kBlockRows, a.rows - row) : 0);
     }
     asm volatile("cp.async.commit_group;" ::: "memory");
   };
-  {
-    const float* p = static_cast<const float*>(a.q) + h * a.q_head;
-    for (int e = threadIdx.x; e < kFp32Rows * (DP / 4); e += kFp32Threads) {
-      const int r = e / (DP / 4), c = e % (DP / 4);
-      const long long row = (long long)tile * kFp32Rows + r;
-      const bool in = row < a.rows && c * 4 < a.head_dim;
-      copy16(sq + r * G::kRow + c * 4, p + (in ? row * a.q_row + c * 4 : 0), in);
-    }
-  }
-  copy_rows(sk, a.k, a.k_row, kv * a.k_head, 0);
-  copy_rows(sv, a.v, a.v_row, kv * a.v_head, 0);
+  copy_rows(sq, static_cast<const float*>(a.q) + h * a.q_head, a.q_row, (long long)tile * G::kRows, G::kRows,
+            (int)min((long long)G::kRows, a.rows - (long long)tile * G::kRows));
+  copy_tile(sk, a.k, a.k_row, kv * a.k_head, 0);
+  copy_tile(sv, a.v, a.v_row, kv * a.v_head, 0);
 
-  RowLimits limits[4];
+  RowLimits limits[RT];
 #pragma unroll
-  for (int r = 0; r < 4; ++r) limits[r].set(a, keys, tile * kFp32Rows + ty * 4 + r);
+  for (int r = 0; r < RT; ++r) limits[r].set(a, keys, tile * G::kRows + ty * RT + r);
   const int all_low = common_low(a, keys.r1);
   const float c = a.scale * 1.4426950408889634f;
-  float o[4][DP / 64][4] = {}, m[4], l[4] = {};
+  float o[RT][DP / 64][4] = {}, m[RT], l[RT] = {};
 #pragma unroll
-  for (int r = 0; r < 4; ++r) m[r] = -INFINITY;
+  for (int r = 0; r < RT; ++r) m[r] = -INFINITY;
   for (int b0 = 0; b0 < keys.blocks; b0 += 2) {
     const bool more = b0 + 2 < keys.blocks;
     const bool plain = b0 >= keys.sink_blocks && b0 + 1 < keys.blocks && keys.base(b0) >= all_low &&
                        keys.base(b0 + 1) + kBlockRows - 1 <= keys.r0;
     asm volatile("cp.async.wait_group 1;" ::: "memory");  // queries and keys; the values may still be on their way
     __syncthreads();
-    float s[4][4] = {};
+    float s[RT][4] = {};
 #pragma unroll 4
     for (int d = 0; d < DP; d += 4) {
-      float4 q[4], k[4];
+      float4 k[4];
 #pragma unroll
-      for (int i = 0; i < 4; ++i) {
-        q[i] = *reinterpret_cast<const float4*>(sq + (ty * 4 + i) * G::kRow + d);
-        k[i] = *reinterpret_cast<const float4*>(sk + (tx + 16 * i) * G::kRow + d);
-      }
+      for (int i = 0; i < 4; ++i) k[i] = *reinterpret_cast<const float4*>(sk + (tx + 16 * i) * G::kRow + d);
 #pragma unroll
-      for (int r = 0; r < 4; ++r)
+      for (int r = 0; r < RT; ++r) {
+        const float4 q = *reinterpret_cast<const float4*>(sq + (ty * RT + r) * G::kRow + d);
 #pragma unroll
         for (int i = 0; i < 4; ++i) {
-          s[r][i] = fmaf(q[r].x, k[i].x, s[r][i]);
-          s[r][i] = fmaf(q[r].y, k[i].y, s[r][i]);
-          s[r][i] = fmaf(q[r].z, k[i].z, s[r][i]);
-          s[r][i] = fmaf(q[r].w, k[i].w, s[r][i]);
+          s[r][i] = fmaf(q.x, k[i].x, s[r][i]);
+          s[r][i] = fmaf(q.y, k[i].y, s[r][i]);
+          s[r][i] = fmaf(q.z, k[i].z, s[r][i]);
+          s[r][i] = fmaf(q.w, k[i].w, s[r][i]);
         }
+      }
     }
 #pragma unroll
-    for (int r = 0; r < 4; ++r) {
+    for (int r = 0; r < RT; ++r) {
       const unsigned b[2] = {plain ? ~0u : limits[r].bits(keys, b0), plain ? ~0u : limits[r].bits(keys, b0 + 1)};
       float top = m[r];
 #pragma unroll
@@ -803,7 +811,7 @@ __global__ void __launch_bounds__(kFp32Threads) k_window_fp32(const WindowArgs a
       for (int i = 0; i < 4; ++i) {
         s[r][i] = exp2_fast(s[r][i] - ref);
         l[r] += s[r][i];
-        sp[(ty * 4 + r) * G::kPRow + tx + 16 * i] = s[r][i];
+        sp[(ty * RT + r) * G::kPRow + tx + 16 * i] = s[r][i];
       }
 #pragma unroll
       for (int i = 0; i < DP / 64; ++i)
@@ -811,36 +819,40 @@ __global__ void __launch_bounds__(kFp32Threads) k_window_fp32(const WindowArgs a
         for (int e = 0; e < 4; ++e) o[r][i][e] *= keep;
     }
     __syncthreads();  // everybody is done with the keys
-    if (more) copy_rows(sk, a.k, a.k_row, kv * a.k_head, b0 + 2);
+    if (more) copy_tile(sk, a.k, a.k_row, kv * a.k_head, b0 + 2);
     if (more) asm volatile("cp.async.wait_group 1;" ::: "memory");
     else asm volatile("cp.async.wait_group 0;" ::: "memory");
     __syncthreads();  // values and weights are there
 #pragma unroll 2
     for (int j = 0; j < kFp32Keys; j += 4) {
-      float4 p[4];
-#pragma unroll
-      for (int r = 0; r < 4; ++r) p[r] = *reinterpret_cast<const float4*>(sp + (ty * 4 + r) * G::kPRow + j);
+      float4 v[4][DP / 64];
 #pragma unroll
       for (int e = 0; e < 4; ++e)
 #pragma unroll
-        for (int i = 0; i < DP / 64; ++i) {
-          const float4 v = *reinterpret_cast<const float4*>(sv + (j + e) * G::kRow + i * 64 + tx * 4);
+        for (int i = 0; i < DP / 64; ++i)
+          v[e][i] = *reinterpret_cast<const float4*>(sv + (j + e) * G::kRow + i * 64 + tx * 4);
 #pragma unroll
-          for (int r = 0; r < 4; ++r) {
-            const float w = e == 0 ? p[r].x : e == 1 ? p[r].y : e == 2 ? p[r].z : p[r].w;
-            o[r][i][0] = fmaf(w, v.x, o[r][i][0]);
-            o[r][i][1] = fmaf(w, v.y, o[r][i][1]);
-            o[r][i][2] = fmaf(w, v.z, o[r][i][2]);
-            o[r][i][3] = fmaf(w, v.w, o[r][i][3]);
+      for (int r = 0; r < RT; ++r) {
+        const float4 p = *reinterpret_cast<const float4*>(sp + (ty * RT + r) * G::kPRow + j);
+#pragma unroll
+        for (int e = 0; e < 4; ++e) {
+          const float w = e == 0 ? p.x : e == 1 ? p.y : e == 2 ? p.z : p.w;
+#pragma unroll
+          for (int i = 0; i < DP / 64; ++i) {
+            o[r][i][0] = fmaf(w, v[e][i].x, o[r][i][0]);
+            o[r][i][1] = fmaf(w, v[e][i].y, o[r][i][1]);
+            o[r][i][2] = fmaf(w, v[e][i].z, o[r][i][2]);
+            o[r][i][3] = fmaf(w, v[e][i].w, o[r][i][3]);
           }
         }
+      }
     }
     __syncthreads();  // everybody is done with the values and weights
-    if (more) copy_rows(sv, a.v, a.v_row, kv * a.v_head, b0 + 2);
+    if (more) copy_tile(sv, a.v, a.v_row, kv * a.v_head, b0 + 2);
   }
   bool odd = false;  // a result that is not finite
 #pragma unroll
-  for (int r = 0; r < 4; ++r) {
+  for (int r = 0; r < RT; ++r) {
 #pragma unroll
     for (int d = 1; d < 16; d *= 2) l[r] += __shfl_xor_sync(0xffffffffu, l[r], d);
     if (limits[r].start < 0) continue;
@@ -914,11 +926,11 @@ bool encode_rows(CUtensorMap* map, const st_rows& r, int mode, long long rows, i
 
 template <int DP>
 cudaError_t launch_fp32(const WindowArgs& a, cudaStream_t s) {
-  const cudaError_t e =
-      cudaFuncSetAttribute(k_window_fp32<DP>, cudaFuncAttributeMaxDynamicSharedMemorySize, Fp32Tiles<DP>::kSmem);
+  using G = Fp32Tiles<DP>;
+  const cudaError_t e = cudaFuncSetAttribute(k_window_fp32<DP>, cudaFuncAttributeMaxDynamicSharedMemorySize, G::kSmem);
   if (e != cudaSuccess) return e;
-  const unsigned tiles = (unsigned)((a.rows + kFp32Rows - 1ll) / kFp32Rows);
-  k_window_fp32<DP><<<tiles * a.heads, kFp32Threads, Fp32Tiles<DP>::kSmem, s>>>(a);
+  const unsigned tiles = (unsigned)((a.rows + G::kRows - 1ll) / G::kRows);
+  k_window_fp32<DP><<<tiles * a.heads, kFp32Threads, G::kSmem, s>>>(a);
   return cudaSuccess;
 }
 
@@ -972,7 +984,7 @@ extern "C" int st_window_attention(const st_window* p, void* stream) {
   a.heads = p->heads; a.kv_heads = p->kv_heads; a.head_dim = p->head_dim;
   a.window = p->window; a.sinks = p->sinks; a.scale = p->scale;
   cudaStream_t s = static_cast<cudaStream_t>(stream);
-  if (p->mode == ST_MODE_FP32 && p->head_dim <= 128 && (p->rows + kFp32Rows - 1) / kFp32Rows * p->heads <= INT32_MAX) {
+  if (p->mode == ST_MODE_FP32 && p->head_dim <= 128 && (p->rows + 31) / 32 * p->heads <= INT32_MAX) {
     if ((rc = cache_cuda(p->head_dim <= 64 ? launch_fp32<64>(a, s) : launch_fp32<128>(a, s), "window attention: ")) != ST_OK) {
       cudaGetLastError();  // reported here, so not left pending
       return rc;
