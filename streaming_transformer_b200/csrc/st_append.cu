@@ -56,11 +56,13 @@ __global__ void __launch_bounds__(kAppendThreads, 5) k_cache_append(const Append
   const bool on = col < a.head_dim;
   const int tasks = a.heads + 2 * a.kv_heads;
   // task: a query head, then the key heads, then the value heads
+  const T* const q_row = static_cast<const T*>(a.q) + row * a.q_row + col;
+  const T* const k_row = static_cast<const T*>(a.k) + row * a.k_row + col;
+  const T* const v_row = static_cast<const T*>(a.v) + row * a.v_row + col;
   auto source = [&](int task) {
     const int k = task - a.heads, v = k - a.kv_heads;
-    return k < 0   ? static_cast<const T*>(a.q) + row * a.q_row + task * a.q_head + col
-           : v < 0 ? static_cast<const T*>(a.k) + row * a.k_row + k * a.k_head + col
-                   : static_cast<const T*>(a.v) + row * a.v_row + v * a.v_head + col;
+    const long long stride = k < 0 ? a.q_head : v < 0 ? a.k_head : a.v_head;
+    return (k < 0 ? q_row : v < 0 ? k_row : v_row) + (k < 0 ? task : v < 0 ? k : v) * stride;
   };
   Raw8<T> ahead[kAhead];
 #pragma unroll

@@ -104,11 +104,24 @@ __device__ __forceinline__ unsigned encode8(const float (&f)[8], unsigned mask, 
   const float s = __bfloat162float(s16), l = __bfloat162float(l16);
   unsigned codes = 0;
   if (s > 0.f) {
-    // 1.5 * 2^23 + c is c rounded to the nearest integer, ties to even, in the sum's low bits
+    // The code is the quotient, correctly rounded, to the nearest integer (ties to even; 1.5 * 2^23 + c has it in its
+    // low bits). Multiplying by the reciprocal is off by 2^-19 at most here, so only a quotient within 2^-17 of a half
+    // needs the division; the lanes that have one do all their 8 again.
+    const float inverse = __frcp_rn(s);
+    float edge = 0.f;
 #pragma unroll
     for (int i = 0; i < 8; ++i) {
-      const float c = fminf(fmaxf(__fdiv_rn(__fsub_rn(f[i], l), s), 0.f), 15.f);
-      codes |= (__float_as_uint(__fadd_rn(c, 12582912.f)) & 15u) << (4 * i);
+      const float c = fminf(fmaxf(__fmul_rn(__fsub_rn(f[i], l), inverse), 0.f), 15.f);
+      const float n = __fadd_rn(c, 12582912.f);
+      edge = fmaxf(edge, fabsf(__fsub_rn(c, __fsub_rn(n, 12582912.f))));
+      codes |= (__float_as_uint(n) & 15u) << (4 * i);
+    }
+    if (edge > 0.5f - 0x1p-17f || s < 0x1p-126f) {  // (a scale below the normal numbers may have no reciprocal)
+      codes = 0;
+      for (int i = 0; i < 8; ++i) {
+        const float c = fminf(fmaxf(__fdiv_rn(__fsub_rn(f[i], l), s), 0.f), 15.f);
+        codes |= (__float_as_uint(__fadd_rn(c, 12582912.f)) & 15u) << (4 * i);
+      }
     }
   }
   *pair = (unsigned)__bfloat16_as_ushort(s16) | ((unsigned)__bfloat16_as_ushort(l16) << 16);

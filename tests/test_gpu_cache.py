@@ -166,6 +166,7 @@ def test_four_bit_groups_at_their_limits():
     # pass-through rows (no norm, no rotation): the stored words follow the definition, group by group
     dim, inf, nan = 32 * 8, float("inf"), float("nan")
     x = torch.zeros(1, 1, dim)
+    x[..., :32] = torch.linspace(-1e-38, 1e-38, 32)       # the scale is below bf16's normal numbers
     x[..., 32:64] = 3.0                                   # constant: scale 0
     x[..., 64:96] = torch.linspace(-1e-40, 1e-40, 32)     # the range underflows bf16's normal numbers
     x[..., 96:128] = torch.linspace(-3e38, 3e38, 32)      # the range overflows fp32
