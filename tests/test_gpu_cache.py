@@ -409,6 +409,28 @@ def test_offsets_past_32_bits():
     ref.check(got, want, bound)
 
 
+@pytest.mark.parametrize("mode", ["fp32", "mixed", "bf16"])
+def test_attention_over_a_snapshot_of_the_runtime_matches_its_step(mode):
+    # a snapshot's layer is a cache without sinks: the same q over it gives the attention that the step traced
+    import numpy as np
+
+    from policy import check_state
+    from streaming_transformer_b200 import Backend, ModelConfig, Runtime, RuntimeOptions, synthetic
+
+    c = ModelConfig(2, 256, 4, 128, 40, 32, 1e-5)
+    events = synthetic.make_events(57, 32, seed=12)
+    with Runtime(synthetic.make_model(c, mode, seed=11), RuntimeOptions(backend=Backend.CUDA, blocks=0)) as rt:
+        for e in events[:56]:          # past one full ring revolution
+            rt.step(e)
+        trace, snap = rt.trace_step(events[56]), rt.snapshot()
+    positions = torch.tensor([snap.position - 1], dtype=torch.int64, device="cuda")
+    for layer in range(c.layers):
+        keys, values = (torch.from_numpy(np.ascontiguousarray(x[layer])).to(TYPES[mode])[None].cuda() for x in (snap.keys, snap.values))
+        q = torch.from_numpy(trace[f"layers.{layer}.q"]).to(TYPES[mode]).view(1, c.heads, c.head_dim).cuda()
+        got = ops.cache_attention(q, keys, values, positions).float().cpu().numpy().reshape(1, 1, -1)
+        check_state(got, trace[f"layers.{layer}.attention"][None, None, :], mode, f"layer {layer}")
+
+
 # ---------------------------------------------------------------- attention of packed sequences
 
 WINDOW = [
