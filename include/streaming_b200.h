@@ -269,7 +269,7 @@ const char* st_attention_static_error(void);
  * bf16((max - min) * (1/15)) and code = rint((x - lowest) / scale) clamped to
  * 0..15 (0 where the scale is 0). A group with a non-finite value, or whose
  * max - min or bf16(min) is not finite, reads back as NaN. Attention takes
- * value scales from 2^-56 to 2^56 (or 0).
+ * value scales from 2^-56 to 2^56 (or 0) and queries below 2^120.
  *
  * All pointers are device memory of `device`, rows start on 16-byte
  * boundaries, and work is queued on `stream` (a cudaStream_t) without waiting.
@@ -340,7 +340,7 @@ int st_cache_append(const st_cache* cache, const st_append* args, void* stream);
 typedef struct {
   int mode;                 /* st_mode of q and out: the cache's type, or fp16/bf16 for INT4 */
   int heads;                /* query heads, a multiple of the cache's */
-  float scale;              /* usually 1 / sqrt(head_dim) */
+  float scale;              /* usually 1 / sqrt(head_dim); within +-2^64 */
   st_rows q, out;           /* [streams][heads][head_dim] */
   const int64_t* positions; /* [streams] */
   void* workspace;
@@ -368,7 +368,7 @@ typedef struct {
   int sequences;
   int64_t rows;             /* up to 2^30 */
   int window, sinks;        /* window >= 1, sinks >= 0 */
-  float scale;
+  float scale;              /* within +-2^64 */
   st_rows q, k, v, out;
   const int32_t* starts;    /* [sequences + 1] non-decreasing within 0 .. rows, or NULL */
 } st_window;

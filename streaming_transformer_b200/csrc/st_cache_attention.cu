@@ -24,9 +24,9 @@
 // piece of P into the B operand of the second product.
 //
 // That holds 4 (head_dim 128) to 2 (64) KB in flight a warp, in registers. 4-bit
-// rows are too short for it: they go through a ring in shared memory, a few
-// stages of 16 or 32 slots for each warp, filled by 16-byte cp.async (zeros past
-// the last slot). Rows there are an odd number of 16-byte units apart, so that
+// rows are too short for it: they go through a ring in shared memory, two stages
+// of 16 or 32 slots for each warp, filled by 16-byte cp.async (zeros past the last
+// slot). Rows there are an odd number of 16-byte units apart, so that
 // neither product's reads meet in a bank.
 //
 // 4-bit rows: the codes enter the products as they are. A nibble in the low
@@ -41,8 +41,9 @@
 // takes scales from 2^-56 to 2^56). Codes are 0..15 where the values lie about
 // 0, so that rounding would count double; the fp32 sum beside the product takes
 // p * (lowest + 7.5 scale) - 7.5 * (the rounded weight), which leaves the error
-// with the code's distance from 7.5. Turning codes into 16-bit values first took 1.7 times the
-// instructions, which bound the kernel, and rounded each value once more.
+// with the code's distance from 7.5. Turning codes into 16-bit values first took
+// 1.7 times the instructions, which bound the kernel (256 Large streams, 516
+// slots: 58 us, now 48), and rounded each value once more.
 //
 // Softmax statistics are fp32: a running maximum per head (in units of log2),
 // the sum of unrounded weights, and output sums. Weights are rounded to the 16
@@ -73,7 +74,8 @@ struct AttendArgs {
   const unsigned* key_scales; const unsigned* value_scales;
   long long stream_stride, head_stride;  // cache rows
   const long long* positions;
-  float* parts;   // [stream][head][split]{m, l}, then [stream][head][split][head_dim]
+  float* parts;   // [stream][head][split]{m, l}, then from `sums_at` on [stream][head][split][head_dim]
+  long long sums_at;  // floats, a multiple of 4
   int streams, heads, kv_heads, group, head_dim, slots, splits, blocks;  // blocks of query heads a key head
   float scale2;   // scale * log2(e)
 };
@@ -138,7 +140,7 @@ __device__ __forceinline__ void put_result(const AttendArgs& a, int stream, int 
   }
   const long long at = ((long long)stream * a.heads + h) * a.splits + split;
   if (d == 0) reinterpret_cast<float2*>(a.parts)[at] = make_float2(m, l);
-  a.parts[(long long)a.streams * a.heads * a.splits * 2 + at * a.head_dim + d] = o;
+  a.parts[a.sums_at + at * a.head_dim + d] = o;
 }
 
 __device__ __forceinline__ void let_next_kernel_start() { asm volatile("griddepcontrol.launch_dependents;"); }
@@ -170,7 +172,7 @@ struct AttendSmem {
 // 64 DB, so that row offsets are constants and no column is checked; ONE: one
 // query head a key head, so that the odd columns of S^T are not computed on.
 template <typename T, int DB, int NT, bool INT4, bool FULL, bool ONE>
-__global__ void __launch_bounds__(kAttendThreads, DB * NT == 1 ? (INT4 ? 5 : 6) : INT4 && DB == 2 && NT == 1 ? 3 : 1)
+__global__ void __launch_bounds__(kAttendThreads, DB * NT == 1 ? (INT4 ? 7 : 6) : INT4 && DB == 2 && NT == 1 ? 3 : 1)
     k_attend_mma(const AttendArgs a) {
   constexpr int J = 2 * DB;   // 16-bit: 16-byte pieces of a key row a lane holds
   using Smem = AttendSmem<DB, NT, INT4>;
@@ -684,7 +686,7 @@ __global__ void __launch_bounds__(32 * kMergeWarps) k_merge(const AttendArgs a) 
   const int seen = slots_seen(a.positions[stream], a.slots);
   const long long at = ((long long)stream * a.heads + h) * a.splits;
   const float2* ml = reinterpret_cast<const float2*>(a.parts) + at;
-  const float4* part = reinterpret_cast<const float4*>(a.parts + (long long)a.streams * a.heads * a.splits * 2 + at * a.head_dim);
+  const float4* part = reinterpret_cast<const float4*>(a.parts + a.sums_at + at * a.head_dim);
   const int quads = a.head_dim / 4;
   wait_for_previous_kernel();
   float top = -INFINITY, sum = 0.f;
@@ -799,8 +801,12 @@ int check_heads(const st_cache* c, int heads) {
              ? cache_fail(ST_ERR_INVALID, "query heads are a multiple of the cache's heads, up to 65535") : ST_OK;
 }
 
+// Floats of the parts' statistics, up to the 16 bytes on which their sums start.
+long long statistics_floats(const st_cache* c, int heads, int splits) {
+  return ((long long)c->streams * heads * splits * 2 + 3) / 4 * 4;
+}
 size_t workspace_bytes(const st_cache* c, int heads, int splits) {
-  return splits == 1 ? 0 : (size_t)c->streams * heads * splits * (2 + c->head_dim) * sizeof(float);
+  return splits == 1 ? 0 : (statistics_floats(c, heads, splits) + (size_t)c->streams * heads * splits * c->head_dim) * sizeof(float);
 }
 
 }  // namespace
@@ -830,7 +836,7 @@ int st_cache_attention(const st_cache* c, const st_attend* p, void* stream) {
       (rc = check_rows(p->out, "out", p->mode, c->streams, p->heads, c->head_dim, true)) != ST_OK)
     return rc;
   if (!p->positions) return cache_fail(ST_ERR_INVALID, "null positions");
-  if (!(p->scale > -1.0e38f && p->scale < 1.0e38f)) return cache_fail(ST_ERR_INVALID, "scale must be finite");
+  if (!(fabsf(p->scale) <= 0x1p64f)) return cache_fail(ST_ERR_INVALID, "scale must be within 2^64");
   DeviceScope scope(c->device);
   if (scope.status() != ST_OK) return scope.status();
   const int splits = splits_of(c, p->heads);
@@ -848,6 +854,7 @@ int st_cache_attention(const st_cache* c, const st_attend* p, void* stream) {
   a.stream_stride = c->stream_stride; a.head_stride = c->head_stride;
   a.positions = reinterpret_cast<const long long*>(p->positions);
   a.parts = static_cast<float*>(p->workspace);
+  a.sums_at = statistics_floats(c, p->heads, splits);
   a.streams = c->streams; a.heads = p->heads; a.kv_heads = c->heads; a.group = p->heads / c->heads;
   a.head_dim = c->head_dim; a.slots = c->sinks + c->window; a.splits = splits;
   a.blocks = (a.group + per - 1) / per;

@@ -962,7 +962,7 @@ extern "C" int st_window_attention(const st_window* p, void* stream) {
   if (p->window < 1 || p->sinks < 0) return cache_fail(ST_ERR_INVALID, "window is at least 1 and sinks at least 0");
   if (p->starts ? p->sequences < 0 : p->sequences != 1)
     return cache_fail(ST_ERR_INVALID, "without starts there is one sequence");
-  if (!(p->scale > -3.0e38f && p->scale < 3.0e38f)) return cache_fail(ST_ERR_INVALID, "scale must be finite");
+  if (!(fabsf(p->scale) <= 0x1p64f)) return cache_fail(ST_ERR_INVALID, "scale must be within 2^64");
   if (p->rows == 0 || p->sequences == 0) return ST_OK;
   int rc;
   if ((rc = check_rows(p->q, "q", p->mode, p->rows, p->heads, p->head_dim, false)) != ST_OK ||

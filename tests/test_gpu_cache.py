@@ -238,6 +238,10 @@ ATTEND = [
     ("int4", "bf16", 12, 1, 224, 130, [129, 64]),
     ("int4", "bf16", 3, 3, 32, 3000, [2999]),
     ("fp32", None, 5, 5, 24, 4100, [4099, 77]),
+    ("bf16", None, 1, 1, 64, 500, [499]),          # 7 parts of one head: an odd number of statistics ahead of the sums
+    ("fp32", None, 1, 1, 32, 450, [449]),
+    ("int4", "bf16", 1, 1, 64, 460, [459, 100, 7]),
+    ("mixed", None, 3, 3, 128, 450, [449]),
 ]
 
 
