@@ -56,7 +56,9 @@ struct WindowArgs {
 };
 
 // The sequence that owns `row`, as its first row; -1 outside every sequence.
-__device__ int sequence_start(const WindowArgs& a, int row) {
+// `end`, if given: the first row behind that sequence.
+__device__ int sequence_start(const WindowArgs& a, int row, int* end = nullptr) {
+  if (end) *end = a.rows;
   if (!a.starts) return 0;
   int lo = 0, hi = a.sequences;  // the first sequence that ends behind the row
   while (lo < hi) {
@@ -65,6 +67,7 @@ __device__ int sequence_start(const WindowArgs& a, int row) {
     else hi = mid;
   }
   if (lo == a.sequences) return -1;
+  if (end) *end = clamp_row(a.starts[lo + 1], a.rows);
   const int first = clamp_row(a.starts[lo], a.rows);
   return first <= row ? first : -1;
 }
@@ -290,6 +293,7 @@ __device__ __forceinline__ unsigned bit_range(int lo, int hi) {
 struct TileKeys {
   int r0, r1;              // first and last row inside a sequence
   int start;               // first row of r0's sequence
+  bool one;                // r1 is in that sequence too
   int sink_end;            // sinks walked apart: rows start .. sink_end - 1
   int low;                 // first row of the window blocks
   int sink_blocks, blocks;
@@ -306,7 +310,9 @@ __device__ __forceinline__ bool tile_keys(const WindowArgs& a, long long first, 
     t.r1 = min(t.r1, clamp_row(a.starts[a.sequences], a.rows) - 1);
   }
   if (t.r0 > t.r1) return false;
-  t.start = sequence_start(a, t.r0);
+  int end;
+  t.start = sequence_start(a, t.r0, &end);
+  t.one = end > t.r1;
   if (t.start < 0) t.start = t.r0;  // only with starts that decrease
   t.low = (int)max((long long)t.start, (long long)t.r0 - a.window + 1);
   t.sink_end = (int)min((long long)t.low, (long long)t.start + a.sinks);
@@ -320,7 +326,7 @@ struct RowLimits {
   int row, start, low, sink_last;  // start -1: none
   __device__ void set(const WindowArgs& a, const TileKeys& t, int r) {
     row = r;
-    start = r >= t.r0 && r <= t.r1 ? sequence_start(a, r) : -1;
+    start = r < t.r0 || r > t.r1 ? -1 : t.one ? t.start : sequence_start(a, r);
     low = (int)max((long long)start, (long long)r - a.window + 1);
     sink_last = (int)min((long long)r, (long long)start + a.sinks - 1);
   }
@@ -332,8 +338,8 @@ struct RowLimits {
   }
 };
 // First row that is inside the window of every row up to r1 of r1's sequence.
-__device__ __forceinline__ int common_low(const WindowArgs& a, int r1) {
-  return (int)max((long long)sequence_start(a, r1), (long long)r1 - a.window + 1);
+__device__ __forceinline__ int common_low(const WindowArgs& a, const TileKeys& t, int r1) {
+  return (int)max((long long)(t.one ? t.start : sequence_start(a, r1)), (long long)r1 - a.window + 1);
 }
 
 // One of a CTA's two tiles: which key blocks any of its rows can see, and which all of them do.
@@ -347,10 +353,10 @@ struct SubTile {
     r1 = (int)min((long long)t.r1, first + kTileRows - 1);
     any = r0 <= r1;
     if (!any) return;
-    start = max(sequence_start(a, r0), 0);
+    start = t.one ? t.start : max(sequence_start(a, r0), 0);
     low = (int)max((long long)start, (long long)r0 - a.window + 1);
     sink_end = (int)min((long long)r0, (long long)start + a.sinks);
-    all_low = common_low(a, r1);
+    all_low = common_low(a, t, r1);
   }
   __device__ bool needs(const TileKeys& t, int b0, int nb) const {
     if (!any) return false;
@@ -656,29 +662,42 @@ __global__ void __launch_bounds__(Tiles<DP>::kThreads, DP == 64 ? 2 : 1)
     if (ok && n > 0) ok = wait(&o_full[side], n - 1);
     tc_fence_after();
     const bool good = __all_sync(0xffffffffu, ok && n > 0);
-    if (good || inside) {
-      bool odd = false;  // a result that is not finite
-      T* to = static_cast<T*>(a.out) + row * a.o_row + h * a.o_head;
+    T* const out = static_cast<T*>(a.out) + h * a.o_head;
+    if (good) {
+      // through this tile's place of the queries, which are done with: a row a thread in, whole lines out (16-byte
+      // pieces straight from the threads, each to a line of its own, took a quarter of a CTA's time). Pieces are
+      // exchanged by row, so that neither way meets in a bank.
+      constexpr int kPieces = DP / 8, kRowBytes = DP * 2;
+      unsigned char* mine = sq + side * G::kQBytes + (warp & 3) * 32 * kRowBytes;
+      const float inv = 1.f / l;
+      float finite = 0.f;  // NaN once a result is not finite
 #pragma unroll
       for (int d = 0; d < DP; d += 32) {
         float o[32];
-        if (good) tmem_ld32(my_o + d, o);
-        const float inv = good ? 1.f / l : NAN;
-        if (inside)
+        tmem_ld32(my_o + d, o);
 #pragma unroll
-          for (int e = 0; e < 32; e += 8) {
-            if (d + e < a.head_dim) {
-              float r[8];
+        for (int e = 0; e < 32; e += 8) {
+          float r[8];
 #pragma unroll
-              for (int w = 0; w < 8; ++w) {
-                r[w] = good ? o[e + w] * inv : NAN;
-                odd |= !(fabsf(r[w]) < INFINITY);
-              }
-              store8(to + d + e, r);
-            }
+          for (int w = 0; w < 8; ++w) {
+            r[w] = o[e + w] * inv;
+            if (d + e < a.head_dim) finite = fmaf(r[w], 0.f, finite);
           }
+          store8(reinterpret_cast<T*>(mine + lane * kRowBytes + (((d + e) / 8) ^ (lane & 7)) * 16), r);
+        }
       }
-      if (odd) sh_slow = 1;
+      if (inside && finite != finite) sh_slow = 1;
+      const unsigned rows_inside = __ballot_sync(0xffffffffu, inside);
+      __syncwarp();
+#pragma unroll
+      for (int i = 0; i < kPieces; ++i) {
+        const int r = i * (32 / kPieces) + lane / kPieces, piece = lane % kPieces;
+        if ((rows_inside >> r & 1u) && piece * 8 < a.head_dim)
+          *reinterpret_cast<uint4*>(out + (row - lane + r) * a.o_row + piece * 8) =
+              *reinterpret_cast<const uint4*>(mine + r * kRowBytes + (piece ^ (r & 7)) * 16);
+      }
+    } else if (inside) {
+      for (int d = 0; d < a.head_dim; ++d) out[row * a.o_row + d] = static_cast<T>(NAN);
     }
     tc_fence_before();
   }
@@ -764,7 +783,7 @@ __global__ void __launch_bounds__(kFp32Threads) k_window_fp32(const WindowArgs a
   RowLimits limits[RT];
 #pragma unroll
   for (int r = 0; r < RT; ++r) limits[r].set(a, keys, tile * G::kRows + ty * RT + r);
-  const int all_low = common_low(a, keys.r1);
+  const int all_low = common_low(a, keys, keys.r1);
   const float c = a.scale * 1.4426950408889634f;
   float o[RT][DP / 64][4] = {}, m[RT], l[RT] = {};
 #pragma unroll
