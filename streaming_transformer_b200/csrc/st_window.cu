@@ -9,7 +9,8 @@
 //
 // k_window_tiles. A CTA takes two tiles of 128 query rows, one TMEM lane a row,
 // that share their keys: two heads of one key head, or where a key head has an
-// odd number of them two neighbouring tiles of one head. Rows may belong to
+// odd number of them two neighbouring tiles of one head (up to 64 columns one
+// tile then, see launch_tiles). Rows may belong to
 // several sequences: the keys that are needed are those from the first row's
 // window on, which covers every sequence that begins behind it, and the sinks of
 // the first row's sequence. They are walked in blocks of 32 rows (sinks first,
@@ -20,7 +21,7 @@
 // While the four warps of one tile are in their exponentials, the products of
 // the other run, and the copies of the next key tile: with one tile a CTA and
 // room for one key tile, the waits for its copy and for the products set the pace
-// (8192 rows, window 4096, 32 heads of 128: 529 us, now 467, 0.53 of the measured
+// (8192 rows, window 4096, 32 heads of 128: 529 us, now 465, 0.53 of the measured
 // dense rate; what bounds it is the chain S, softmax, O of each query tile, 3700
 // cycles a key tile where exponentials and products take 2050 each). O is rescaled only when a row's maximum
 // has grown by more than 2^8 since the last time; P then stays below 2^8, which
@@ -138,19 +139,21 @@ __device__ __forceinline__ bool wait_phase(unsigned long long* bar, unsigned par
   return false;
 }
 
-// DP: columns, padded to 64 or 128 with zeros by the copies. Key tiles are DP rows: S and O take DP TMEM columns each
-// for each tile, so that one CTA of 128 columns or two of 64 fill an SM's TMEM.
-template <int DP>
+// DP: columns, padded to 64 or 128 with zeros by the copies; SUBS: query tiles of a CTA. Key tiles are DP rows: S and O
+// take DP TMEM columns each for each query tile, so that one CTA of 128 columns, or two (four of one query tile) of 64,
+// fill an SM's TMEM.
+template <int DP, int SUBS>
 struct Tiles {
   static constexpr int kKeys = DP, kBlocks = kKeys / kBlockRows, kPanels = DP / 64;
   static constexpr int kQBytes = kPanels * kTileRows * 128, kKvBytes = kPanels * kKeys * 128;
   // 4 warps of rows for each tile, one that copies, one that issues products; at 128 columns two more, which make the
   // last four a warpgroup that hands registers to the others
-  static constexpr int kThreads = DP == 128 ? 384 : 320;
+  static constexpr int kCopyWarp = 4 * SUBS, kIssueWarp = kCopyWarp + 1;
+  static constexpr int kThreads = DP == 128 ? 384 : kIssueWarp * 32 + 32, kCtas = 128 / DP * 2 / SUBS;
   // One ring for K and V tiles in the order of their use: two are being read, the others are on their way. With two
   // slots each (one ahead) the products waited for the copies.
-  static constexpr int kSlots = DP == 64 ? 8 : 5;
-  static constexpr int kSmem = 2 * kQBytes + kSlots * kKvBytes + 1024;
+  static constexpr int kSlots = DP == 128 ? 5 : 4 * SUBS;
+  static constexpr int kSmem = SUBS * kQBytes + kSlots * kKvBytes + 1024;
 };
 
 struct TileMaps {
@@ -369,33 +372,33 @@ struct SubTile {
   }
 };
 
-template <typename T, int DP>
-__global__ void __launch_bounds__(Tiles<DP>::kThreads, DP == 64 ? 2 : 1)
+template <typename T, int DP, int SUBS>
+__global__ void __launch_bounds__(Tiles<DP, SUBS>::kThreads, Tiles<DP, SUBS>::kCtas)
     k_window_tiles(const WindowArgs a, const __grid_constant__ TileMaps maps) {
-  using G = Tiles<DP>;
+  using G = Tiles<DP, SUBS>;
   extern __shared__ unsigned char raw[];
-  __shared__ unsigned long long q_full, full[G::kSlots], free[G::kSlots], s_full[2], p_full[2], o_full[2];
+  __shared__ unsigned long long q_full, full[G::kSlots], free[G::kSlots], s_full[SUBS], p_full[SUBS], o_full[SUBS];
   __shared__ unsigned tmem_base;
   __shared__ int sh_slow, sh_dead;
   const int warp = threadIdx.x >> 5;
-  // the pair: two heads of one tile of rows, or two tiles of one head; those with most keys first
-  const bool two_heads = (a.heads / a.kv_heads) % 2 == 0;
-  const int per_row = two_heads ? a.heads / 2 : a.heads;
+  // one query tile, or two: two heads of one tile of rows, or two tiles of one head; those with most keys first
+  const bool two_heads = SUBS == 2 && (a.heads / a.kv_heads) % 2 == 0;
+  const int per_row = two_heads ? a.heads / 2 : a.heads, row_tiles = two_heads ? 1 : SUBS;
   const int h0 = two_heads ? blockIdx.x % per_row * 2 : blockIdx.x % per_row;
-  const long long pair_row = (long long)(gridDim.x / per_row - 1 - blockIdx.x / per_row) * (two_heads ? 1 : 2) * kTileRows;
+  const long long pair_row = (long long)(gridDim.x / per_row - 1 - blockIdx.x / per_row) * row_tiles * kTileRows;
   auto head_of = [&](int s) { return two_heads ? h0 + s : h0; };
   auto first_row = [&](int s) { return pair_row + (two_heads ? 0 : s * kTileRows); };
   TileKeys keys;
-  if (!tile_keys(a, pair_row, (two_heads ? 1 : 2) * kTileRows, keys)) return;
+  if (!tile_keys(a, pair_row, row_tiles * kTileRows, keys)) return;
   unsigned char* smem = raw + ((1024u - (smem_addr(raw) & 1023u)) & 1023u);
-  unsigned char *sq = smem, *ring = sq + 2 * G::kQBytes;  // ring item 2 i: K of key tile i, 2 i + 1: V
+  unsigned char *sq = smem, *ring = sq + SUBS * G::kQBytes;  // ring item 2 i: K of key tile i, 2 i + 1: V
   if (threadIdx.x == 0) {
     mbar_init(&q_full, 1);
     for (int s = 0; s < G::kSlots; ++s) {
       mbar_init(&full[s], 1);
       mbar_init(&free[s], 1);
     }
-    for (int s = 0; s < 2; ++s) {
+    for (int s = 0; s < SUBS; ++s) {
       mbar_init(&s_full[s], 1);
       mbar_init(&p_full[s], 4);
       mbar_init(&o_full[s], 1);
@@ -403,8 +406,8 @@ __global__ void __launch_bounds__(Tiles<DP>::kThreads, DP == 64 ? 2 : 1)
     fence_mbar_init();
     sh_slow = sh_dead = 0;
   }
-  if (warp == 9) {
-    tmem_alloc(&tmem_base, 4 * DP);
+  if (warp == G::kIssueWarp) {
+    tmem_alloc(&tmem_base, 2 * SUBS * DP);
     tmem_relinquish();
   }
   tc_fence_before();
@@ -420,18 +423,18 @@ __global__ void __launch_bounds__(Tiles<DP>::kThreads, DP == 64 ? 2 : 1)
     return false;
   };
 
-  if (warp >= 8) {
+  if (warp >= G::kCopyWarp) {
     // 384 threads start with 168 registers each: 2 * 128 * 208 + 128 * 88 is as many
     if constexpr (DP == 128) asm volatile("setmaxnreg.dec.sync.aligned.u32 88;");
     // Both warps run as a whole, and one lane issues: what an instruction takes then stays in uniform registers. The
     // products' issue is on the critical path (by one lane alone, with descriptors built for each, 8192 rows, window
     // 4096: 557 us, so 489).
-    if (warp == 8) {
+    if (warp == G::kCopyWarp) {
       const bool lead = elect_one();
       const int kv = h0 / (a.heads / a.kv_heads);
       if (lead) {
-        mbar_expect_tx(&q_full, 2 * G::kQBytes);
-        for (int s = 0; s < 2; ++s)
+        mbar_expect_tx(&q_full, SUBS * G::kQBytes);
+        for (int s = 0; s < SUBS; ++s)
           for (int p = 0; p < G::kPanels; ++p)
             copy_box(sq + s * G::kQBytes + p * kTileRows * 128, &maps.q, p * 64, head_of(s), (int)first_row(s), &q_full);
       }
@@ -455,16 +458,16 @@ __global__ void __launch_bounds__(Tiles<DP>::kThreads, DP == 64 ? 2 : 1)
         wait_phase(&q_full, 0);
         for (int i = max(0, item - G::kSlots); i < item; ++i) wait_phase(&full[i % G::kSlots], (i / G::kSlots) & 1);
       }
-    } else if (warp == 9) {
+    } else if (warp == G::kIssueWarp) {
       const bool lead = elect_one();
-      SubTile sub[2];
-      for (int s = 0; s < 2; ++s) sub[s].set(a, keys, first_row(s));
+      SubTile sub[SUBS];
+      for (int s = 0; s < SUBS; ++s) sub[s].set(a, keys, first_row(s));
       const int ksteps = (a.head_dim + 15) / 16;
       const unsigned idesc_s = umma_idesc<T>(kTileRows, G::kKeys);
       const unsigned idesc_o = umma_idesc<T>(kTileRows, ksteps * 16) | (1u << 16);  // V: N contiguous
       const unsigned long long dq = swizzled_desc(sq, 0), dk = swizzled_desc(ring, 0), dv = swizzled_desc(ring, G::kKeys * 128);
       constexpr unsigned kSlotStep = G::kKvBytes >> 4;
-      int done[2] = {0, 0};  // second products issued
+      int done[SUBS] = {};  // second products issued
       auto needs = [&](int s, int i) {
         return i < tiles && sub[s].needs(keys, i * G::kBlocks, min(G::kBlocks, keys.blocks - i * G::kBlocks));
       };
@@ -493,7 +496,7 @@ __global__ void __launch_bounds__(Tiles<DP>::kThreads, DP == 64 ? 2 : 1)
 #pragma unroll
           for (int e = 0; e < G::kBlocks * 2; ++e)
             if (e < nb * 2)
-              umma_f16_ts(tmem + (2 + s) * DP, tmem + s * DP + e * 8, v + e * (2048 >> 4), idesc_o, e > 0 || done[s] > 0);
+              umma_f16_ts(tmem + (SUBS + s) * DP, tmem + s * DP + e * 8, v + e * (2048 >> 4), idesc_o, e > 0 || done[s] > 0);
           umma_commit(&o_full[s]);
         }
         __syncwarp();
@@ -512,15 +515,16 @@ __global__ void __launch_bounds__(Tiles<DP>::kThreads, DP == 64 ? 2 : 1)
         __syncwarp();
       };
       int nb = min(G::kBlocks, keys.blocks);
-      bool need0 = needs(0, 0), need1 = needs(1, 0);
+      constexpr int kLast = SUBS - 1;
+      bool need0 = needs(0, 0), need1 = kLast && needs(kLast, 0);  // one query tile: the second is never needed
       bool ok = wait(&q_full, 0) && here();
       if (ok) {
         const int k = advance();
-        ok = (!need0 || first_product(0, k, nb)) && (!need1 || first_product(1, k, nb));
+        ok = (!need0 || first_product(0, k, nb)) && (!need1 || first_product(kLast, k, nb));
         if (ok) release(k);
       }
       for (int i = 0; i < tiles && ok; ++i) {
-        const bool next0 = needs(0, i + 1), next1 = needs(1, i + 1), more = i + 1 < tiles;
+        const bool next0 = needs(0, i + 1), next1 = kLast && needs(kLast, i + 1), more = i + 1 < tiles;
         const int next_nb = min(G::kBlocks, keys.blocks - (i + 1) * G::kBlocks);
         if (!(ok = here())) break;
         const int v = advance();
@@ -531,10 +535,10 @@ __global__ void __launch_bounds__(Tiles<DP>::kThreads, DP == 64 ? 2 : 1)
           k = advance();
           if (next0 && !(ok = first_product(0, k, next_nb))) break;
         }
-        if (need1 && !(ok = second_product(1, v, nb))) break;
+        if (need1 && !(ok = second_product(kLast, v, nb))) break;
         release(v);
         if (more) {
-          if (next1 && !(ok = first_product(1, k, next_nb))) break;
+          if (next1 && !(ok = first_product(kLast, k, next_nb))) break;
           release(k);
         }
         need0 = next0;
@@ -549,7 +553,7 @@ __global__ void __launch_bounds__(Tiles<DP>::kThreads, DP == 64 ? 2 : 1)
     sub.set(a, keys, first_row(side));
     const long long row = first_row(side) + (threadIdx.x & 127);
     const unsigned lanes = (unsigned)((warp & 3) * 32) << 16;
-    const unsigned my_s = tmem + side * DP + lanes, my_o = tmem + (2 + side) * DP + lanes;
+    const unsigned my_s = tmem + side * DP + lanes, my_o = tmem + (SUBS + side) * DP + lanes;
     RowLimits limits;
     limits.set(a, keys, (int)min(row, (long long)INT32_MAX));
     const bool inside = limits.start >= 0;
@@ -664,9 +668,9 @@ __global__ void __launch_bounds__(Tiles<DP>::kThreads, DP == 64 ? 2 : 1)
     const bool good = __all_sync(0xffffffffu, ok && n > 0);
     T* const out = static_cast<T*>(a.out) + h * a.o_head;
     if (good) {
-      // through this tile's place of the queries, which are done with: a row a thread in, whole lines out (16-byte
-      // pieces straight from the threads, each to a line of its own, took a quarter of a CTA's time). Pieces are
-      // exchanged by row, so that neither way meets in a bank.
+      // through this tile's place of the queries, which are done with: a row a thread in, whole lines out (8192
+      // rows, window 512: 147 us, with 16-byte pieces straight from the threads, each to a line of its own, 151). Pieces
+      // are exchanged by row, so that neither way meets in a bank.
       constexpr int kPieces = DP / 8, kRowBytes = DP * 2;
       unsigned char* mine = sq + side * G::kQBytes + (warp & 3) * 32 * kRowBytes;
       const float inv = 1.f / l;
@@ -703,8 +707,8 @@ __global__ void __launch_bounds__(Tiles<DP>::kThreads, DP == 64 ? 2 : 1)
   }
   __syncthreads();
   tc_fence_after();
-  if (warp == 9) tmem_dealloc(tmem, 4 * DP);
-  if (sh_slow && !sh_dead && warp < 8) {
+  if (warp == G::kIssueWarp) tmem_dealloc(tmem, 2 * SUBS * DP);
+  if (sh_slow && !sh_dead && warp < G::kCopyWarp) {
     constexpr int kLanes = DP / 8;
     const int side = warp >> 2;
     SubTile sub;
@@ -953,15 +957,26 @@ cudaError_t launch_fp32(const WindowArgs& a, cudaStream_t s) {
   return cudaSuccess;
 }
 
-template <typename T, int DP>
+template <typename T, int DP, int SUBS>
 cudaError_t launch_tiles(const WindowArgs& a, const TileMaps& maps, cudaStream_t s) {
+  using G = Tiles<DP, SUBS>;
   const cudaError_t e =
-      cudaFuncSetAttribute(k_window_tiles<T, DP>, cudaFuncAttributeMaxDynamicSharedMemorySize, Tiles<DP>::kSmem);
+      cudaFuncSetAttribute(k_window_tiles<T, DP, SUBS>, cudaFuncAttributeMaxDynamicSharedMemorySize, G::kSmem);
   if (e != cudaSuccess) return e;
   const unsigned tiles = (unsigned)((a.rows + kTileRows - 1ll) / kTileRows);
-  const unsigned ctas = a.heads / a.kv_heads % 2 == 0 ? tiles * (a.heads / 2) : (tiles + 1) / 2 * a.heads;
-  k_window_tiles<T, DP><<<ctas, Tiles<DP>::kThreads, Tiles<DP>::kSmem, s>>>(a, maps);
+  const unsigned ctas =
+      SUBS == 2 && a.heads / a.kv_heads % 2 == 0 ? tiles * (a.heads / 2) : (tiles + SUBS - 1) / SUBS * a.heads;
+  k_window_tiles<T, DP, SUBS><<<ctas, G::kThreads, G::kSmem, s>>>(a, maps);
   return cudaSuccess;
+}
+
+// Up to 64 columns four CTAs of one query tile fit an SM. That is faster where no two heads share their keys (16 uneven
+// backlogs, 16 heads of 64, window 256: 41.0 us, with two tiles a CTA 42.6; 200 rows 8.9 and 10.0) and slower where
+// they do, as the keys then come twice (4 key heads of 16: 41.0 and 39.2; 8192 rows, 8 of 32, window 512: 97 and 94).
+template <typename T>
+cudaError_t launch_tiles(const WindowArgs& a, const TileMaps& maps, cudaStream_t s) {
+  if (a.head_dim > 64) return launch_tiles<T, 128, 2>(a, maps, s);
+  return a.heads / a.kv_heads % 2 == 0 ? launch_tiles<T, 64, 2>(a, maps, s) : launch_tiles<T, 64, 1>(a, maps, s);
 }
 
 }  // namespace
@@ -1017,10 +1032,7 @@ extern "C" int st_window_attention(const st_window* p, void* stream) {
                      encode_rows(&maps.k, p->k, p->mode, p->rows, p->kv_heads, p->head_dim, kBlockRows) &&
                      encode_rows(&maps.v, p->v, p->mode, p->rows, p->kv_heads, p->head_dim, kBlockRows);
   if (tiles) {
-    const bool half = p->mode == ST_MODE_FP16, small = p->head_dim <= 64;
-    const cudaError_t e = half ? (small ? launch_tiles<__half, 64>(a, maps, s) : launch_tiles<__half, 128>(a, maps, s))
-                               : (small ? launch_tiles<__nv_bfloat16, 64>(a, maps, s)
-                                        : launch_tiles<__nv_bfloat16, 128>(a, maps, s));
+    const cudaError_t e = p->mode == ST_MODE_FP16 ? launch_tiles<__half>(a, maps, s) : launch_tiles<__nv_bfloat16>(a, maps, s);
     if (e != cudaSuccess) {
       cudaGetLastError();  // reported here, so not left pending
       return cache_cuda(e, "window attention: ");
