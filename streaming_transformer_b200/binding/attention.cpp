@@ -77,6 +77,12 @@ void no_gradient(std::initializer_list<const at::Tensor*> tensors) {
     if (t && t->requires_grad()) refuse("there is no backward pass: detach the inputs or call under torch.no_grad()");
 }
 
+// Counts a write, so that a backward pass which saved the old values of one of these raises, as for torch's own.
+void written(std::initializer_list<const at::Tensor*> tensors) {
+  for (const at::Tensor* t : tensors)
+    if (t && !t->is_inference()) t->unsafeGetTensorImpl()->bump_version();
+}
+
 void placed(const at::Tensor& t, const char* name, c10::Device device, at::ScalarType type) {
   if (t.device() != device || t.scalar_type() != type) {
     std::ostringstream o;
@@ -204,14 +210,18 @@ PyObject* do_append(PyObject* const* o) {
   st_append a{};
   a.mode = row_mode(q, "q");
   a.heads = heads_of(q, "[rows, heads, head_dim]");
-  no_gradient({&q, &k, &v, q_gain, k_gain, given});
+  no_gradient({&q, &k, &v, &keys, &values, q_gain, k_gain, given});
   const int64_t rows = a.rows = q.size(0);
   a.q = rows_of(q, "q", device, type, rows, a.heads, c.head_dim);
   a.k = rows_of(k, "k", device, type, rows, c.heads, c.head_dim);
   a.v = rows_of(v, "v", device, type, rows, c.heads, c.head_dim);
   at::Tensor out = given ? *given : fresh({rows, a.heads, c.head_dim}, type, device), turned;
   a.q_out = rows_of(out, "out", device, type, rows, a.heads, c.head_dim);
-  const bool both = PyObject_IsTrue(o[14]) == 1;
+  const int both = PyObject_IsTrue(o[14]);
+  if (both < 0) {
+    PyErr_Clear();
+    refuse("rotated_keys: expected True or False");
+  }
   if (both) {
     turned = fresh({rows, c.heads, c.head_dim}, type, device);
     a.k_out = rows_of(turned, "k", device, type, rows, c.heads, c.head_dim);
@@ -226,6 +236,7 @@ PyObject* do_append(PyObject* const* o) {
   a.positions = static_cast<const int64_t*>(values_of(positions, "positions", device, at::kLong, c.streams));
   if (starts) a.starts = static_cast<const int32_t*>(values_of(*starts, "starts", device, at::kInt, c.streams + 1));
   check(st_cache_append(&c, &a, stream_of(device)));
+  written({&keys, &values, key_scales, value_scales, given});
   PyObject* first = THPVariable_Wrap(std::move(out));
   if (!both || !first) return first;
   PyObject* second = THPVariable_Wrap(std::move(turned));
@@ -260,6 +271,7 @@ PyObject* do_attend(PyObject* const* o) {
     a.workspace = work.data_ptr();
   }
   check(st_cache_attention(&c, &a, stream_of(device)));
+  written({given});
   return THPVariable_Wrap(std::move(out));
 }
 
@@ -315,6 +327,7 @@ PyObject* do_window(PyObject* const* o) {
     a.starts = static_cast<const int32_t*>(values_of(*starts, "starts", device, at::kInt, a.sequences + 1));
   }
   check(st_window_attention(&a, stream_of(device)));
+  written({given});
   return THPVariable_Wrap(std::move(out));
 }
 

@@ -730,3 +730,32 @@ def test_empty_calls():
     assert (out == 5).all()
     ops.cache_append(one, one, one, keys, values, at, f, starts=starts, out=out)
     assert (out == 5).all() and not keys.any()
+
+
+def test_writes_are_seen_by_gradients():
+    """A cache that takes part in a gradient is refused, and a tensor that a backward pass saved counts its writes."""
+    keys, values, _, _ = ops.new_cache(2, 2, 8, 64, mode="fp32")
+    at = torch.zeros(2, dtype=torch.int64, device="cuda")
+    q, kv = torch.ones(2, 2, 64, device="cuda"), torch.ones(2, 2, 64, device="cuda")
+    f = ops.rotation_frequencies(64)
+    for side in (keys, values):
+        side.requires_grad_()
+        with pytest.raises(StreamError, match="backward"):
+            ops.cache_append(q, kv, kv, keys, values, at, f)
+        side.requires_grad_(False)
+    with pytest.raises(StreamError, match="rotated_keys"):
+        ops.cache_append(q, kv, kv, keys, values, at, f, rotated_keys=kv)
+    w = torch.ones(2, 2, 8, 64, device="cuda", requires_grad=True)
+    loss = (w * keys).sum()
+    ops.cache_append(q, kv, kv, keys, values, at, f)
+    with pytest.raises(RuntimeError, match="modified by an inplace operation"):
+        loss.backward()
+    for call in (lambda out: ops.cache_append(q, kv, kv, keys, values, at, f, out=out),
+                 lambda out: ops.cache_attention(q, keys, values, at, out=out),
+                 lambda out: ops.window_attention(q, kv, kv, window=3, out=out)):
+        out = torch.empty_like(q)
+        before = out._version
+        call(out)
+        assert out._version == before + 1
+    with torch.inference_mode():
+        ops.cache_attention(q, keys, values, at, out=torch.empty_like(q))
