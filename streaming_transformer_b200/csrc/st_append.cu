@@ -73,10 +73,13 @@ __global__ void __launch_bounds__(kAppendThreads, 5) k_cache_append(const Append
   // the stream that owns this row: the number of streams that end at or before it
   int stream = row, first = row, last = row + 1;
   if (a.starts) {
-    int ended = 0;
-    for (int base = 0; base < a.streams; base += kAppendThreads) {
-      const int s = base + tid;
-      ended += __syncthreads_count(s < a.streams && a.starts[s + 1] <= row);
+    // by 256 at a time: the last stream of each stretch, then the stretch that the row is in
+    const int stretch = (a.streams + kAppendThreads - 1) / kAppendThreads;  // at most 256
+    const int end = tid * stretch + stretch - 1;
+    int ended = __syncthreads_count(end < a.streams && a.starts[end + 1] <= row);
+    if (stretch > 1) {
+      const int s = ended * stretch + tid;
+      ended = ended * stretch + __syncthreads_count(tid < stretch && s < a.streams && a.starts[s + 1] <= row);
     }
     stream = ended;
     if (stream >= a.streams) return;  // behind the last stream

@@ -73,6 +73,8 @@ APPEND = [
     ("int4", 3, 3, 224, 9, 1, [14], 1, 112, True),
     ("bf16", 2, 1, 200, 12, 2, None, 3, 51, True),
     ("mixed", 40, 20, 128, 7, 1, None, 5, 64, True),       # more rows than a CTA's lanes hold at a time
+    ("mixed", 2, 1, 16, 3, 1, [0, 2, 1] * 200, 600, 8, True),          # more streams than a CTA has threads
+    ("fp32", 1, 1, 8, 2, 0, [0] * 255 + [1, 0, 3], 258, 4, True),
 ]
 
 
