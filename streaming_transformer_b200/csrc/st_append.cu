@@ -17,7 +17,6 @@
 namespace st {
 namespace {
 
-constexpr int kAppendThreads = 256;
 constexpr int kMaxPairs = ST_CACHE_MAX_HEAD_DIM / 2;
 
 struct AppendArgs {
@@ -45,12 +44,15 @@ struct Raw8 {
 };
 constexpr int kAhead = 3;  // rows a group of lanes loads ahead of their use
 
-template <typename T, int LANES, bool INT4>
-__global__ void __launch_bounds__(kAppendThreads, 5) k_cache_append(const AppendArgs a) {
+template <typename T, int LANES, bool INT4, int THREADS>
+__global__ void __launch_bounds__(THREADS, 1280 / THREADS) k_cache_append(const AppendArgs a) {
   __shared__ alignas(16) float2 turn[kMaxPairs];
-  __shared__ int sh_slot;
+  __shared__ alignas(16) float gains[2][ST_CACHE_MAX_HEAD_DIM];
+  __shared__ long long sh_position;
+  __shared__ int sh_stream, sh_first, sh_last, sh_slot;
   const int row = blockIdx.x, tid = threadIdx.x;
-  constexpr int kGroups = kAppendThreads / LANES;
+  constexpr int kGroups = THREADS / LANES;
+  static_assert(kMaxPairs <= THREADS && ST_CACHE_MAX_HEAD_DIM / 2 <= THREADS, "a thread for each pair, and for each 4 gains");
   const int lane = tid % LANES, col = lane * 8;
   const unsigned mask = LANES == 32 ? 0xffffffffu : ((1u << LANES) - 1u) << ((tid & 31) / LANES * LANES);
   const bool on = col < a.head_dim;
@@ -70,37 +72,58 @@ __global__ void __launch_bounds__(kAppendThreads, 5) k_cache_append(const Append
     const int task = tid / LANES + u * kGroups;
     if (on && task < tasks) ahead[u].load(source(task));
   }
-  // the stream that owns this row: the number of streams that end at or before it
+  // What else the row needs is loaded beside them, each value by the thread that may use it, so that the CTA waits for
+  // memory once.
+  const double frequency = tid < a.rotary ? a.frequencies[tid] : 0.0;
+  const int side = tid >= a.head_dim / 4, gain_col = (tid - side * (a.head_dim / 4)) * 4;
+  const float* const gain = side ? a.k_gain : a.q_gain;
+  const bool has_gain = gain && gain_col < a.head_dim;
+  float4 gain4;
+  if (has_gain) gain4 = *reinterpret_cast<const float4*>(gain + gain_col);
+  // the stream that owns this row
   int stream = row, first = row, last = row + 1;
+  long long p0;
   if (a.starts) {
-    // by 256 at a time: the last stream of each stretch, then the stretch that the row is in
-    const int stretch = (a.streams + kAppendThreads - 1) / kAppendThreads;  // at most 256
-    const int end = tid * stretch + stretch - 1;
-    int ended = __syncthreads_count(end < a.streams && a.starts[end + 1] <= row);
-    if (stretch > 1) {
-      const int s = ended * stretch + tid;
-      ended = ended * stretch + __syncthreads_count(tid < stretch && s < a.streams && a.starts[s + 1] <= row);
+    // one of the first THREADS, or of the stretch of so many that lies behind all that end at or before this row
+    int base = 0, span = a.streams;
+    while (span > THREADS) {
+      span = (span + THREADS - 1) / THREADS;
+      const int end = base + tid * span + span - 1;
+      base += __syncthreads_count(end < a.streams && a.starts[end + 1] <= row) * span;
     }
-    stream = ended;
-    if (stream >= a.streams) return;  // behind the last stream
-    first = clamp_row(a.starts[stream], a.rows);
-    last = clamp_row(a.starts[stream + 1], a.rows);
-    if (row < first || row >= last) return;  // before the first stream
+    const int s = base + tid;
+    bool mine = false;
+    if (tid < span && s < a.streams) {
+      const int from = a.starts[s], to = a.starts[s + 1];
+      const long long position = a.positions[s];
+      mine = from <= row && row < to;
+      if (mine) {
+        sh_stream = s;
+        sh_first = clamp_row(from, a.rows);
+        sh_last = clamp_row(to, a.rows);
+        sh_position = position;
+      }
+    }
+    if (!__syncthreads_or(mine)) return;  // a row of no stream
+    stream = sh_stream;
+    first = sh_first;
+    last = sh_last;
+    p0 = sh_position;
+  } else {
+    p0 = a.positions[row];
   }
-  const long long p0 = a.positions[stream];
   const bool idle = p0 < 0;
   const long long position = p0 + (row - first);
-  for (int p = tid; p < (a.rotary + 3) / 4 * 4; p += kAppendThreads) {  // a lane's 4 pairs: those past the last turn by 0
-    if (p >= a.rotary) {
-      turn[p] = make_float2(1.f, 0.f);
-      continue;
-    }
-    const double t = (double)position * a.frequencies[p] * 0.15915494309189533577;  // 1 / (2 pi)
+  if (has_gain) *reinterpret_cast<float4*>(&gains[side][gain_col]) = gain4;
+  if (tid < a.rotary) {
+    const double t = (double)position * frequency * 0.15915494309189533577;  // 1 / (2 pi)
     float s, c;
     sincospif(2.f * (float)(t - rint(t)), &s, &c);
-    turn[p] = make_float2(c, s);
+    turn[tid] = make_float2(c, s);
+  } else if (tid < (a.rotary + 3) / 4 * 4) {
+    turn[tid] = make_float2(1.f, 0.f);  // a lane's 4 pairs: those past the last turn by 0
   }
-  if (tid == kAppendThreads - 1) {  // in a warp that has no pairs, mostly
+  if (tid == THREADS - 1) {  // in a warp that has no pairs, mostly
     // inserted: sink positions, and those the stream's last `window` rows hold
     const long long newest = p0 + (last - 1 - first);
     int slot = -1;
@@ -123,8 +146,7 @@ __global__ void __launch_bounds__(kAppendThreads, 5) k_cache_append(const Append
       if (on && !idle) load8(reinterpret_cast<const T*>(ahead[u].u), f);
       if (on && task + kAhead * kGroups < tasks) ahead[u].load(source(task + kAhead * kGroups));
       if (!is_v && !idle) {
-        const float* gain = is_q ? a.q_gain : a.k_gain;
-        if (gain) {
+        if (is_q ? a.q_gain : a.k_gain) {
           float sum = 0.f;
 #pragma unroll
           for (int i = 0; i < 8; ++i) sum = fmaf(f[i], f[i], sum);
@@ -133,7 +155,7 @@ __global__ void __launch_bounds__(kAppendThreads, 5) k_cache_append(const Append
           const float scale = rsqrtf(fmaf(sum, a.per_column, a.epsilon));
           if (on) {
             float g[8];
-            load8(gain + col, g);
+            load8(&gains[!is_q][col], g);
 #pragma unroll
             for (int i = 0; i < 8; ++i) f[i] = f[i] * scale * g[i];
           }
@@ -172,16 +194,25 @@ __global__ void __launch_bounds__(kAppendThreads, 5) k_cache_append(const Append
   }
 }
 
-template <typename T, bool INT4>
+// Rows that are resident all at once, 5 CTAs on each of 148 SMs, have 256 threads each: fewer heads one after another
+// (16 heads of 64, 256 rows: 2.8 us, with 128 threads 3.2; 700: 4.0 and 4.1). More rows have 128, as a CTA's threads
+// wait together for what it does once (1000 rows: 4.5 us, with 256 threads 5.4; 3000: 11.3 and 13.5).
+constexpr int kFewRows = 5 * 148;
+
+template <typename T, bool INT4, int THREADS>
 void launch_append(const AppendArgs& a, cudaStream_t s) {
   switch (lanes_per_row(a.head_dim)) {
-    case 1: if constexpr (!INT4) k_cache_append<T, 1, INT4><<<a.rows, kAppendThreads, 0, s>>>(a); break;
-    case 2: if constexpr (!INT4) k_cache_append<T, 2, INT4><<<a.rows, kAppendThreads, 0, s>>>(a); break;
-    case 4: k_cache_append<T, 4, INT4><<<a.rows, kAppendThreads, 0, s>>>(a); break;
-    case 8: k_cache_append<T, 8, INT4><<<a.rows, kAppendThreads, 0, s>>>(a); break;
-    case 16: k_cache_append<T, 16, INT4><<<a.rows, kAppendThreads, 0, s>>>(a); break;
-    default: k_cache_append<T, 32, INT4><<<a.rows, kAppendThreads, 0, s>>>(a); break;
+    case 1: if constexpr (!INT4) k_cache_append<T, 1, INT4, THREADS><<<a.rows, THREADS, 0, s>>>(a); break;
+    case 2: if constexpr (!INT4) k_cache_append<T, 2, INT4, THREADS><<<a.rows, THREADS, 0, s>>>(a); break;
+    case 4: k_cache_append<T, 4, INT4, THREADS><<<a.rows, THREADS, 0, s>>>(a); break;
+    case 8: k_cache_append<T, 8, INT4, THREADS><<<a.rows, THREADS, 0, s>>>(a); break;
+    case 16: k_cache_append<T, 16, INT4, THREADS><<<a.rows, THREADS, 0, s>>>(a); break;
+    default: k_cache_append<T, 32, INT4, THREADS><<<a.rows, THREADS, 0, s>>>(a); break;
   }
+}
+template <typename T, bool INT4>
+void launch_append(const AppendArgs& a, cudaStream_t s) {
+  a.rows <= kFewRows ? launch_append<T, INT4, 256>(a, s) : launch_append<T, INT4, 128>(a, s);
 }
 
 struct UnpackArgs {

@@ -75,6 +75,12 @@ APPEND = [
     ("mixed", 40, 20, 128, 7, 1, None, 5, 64, True),       # more rows than a CTA's lanes hold at a time
     ("mixed", 2, 1, 16, 3, 1, [0, 2, 1] * 200, 600, 8, True),          # more streams than a CTA has threads
     ("fp32", 1, 1, 8, 2, 0, [0] * 255 + [1, 0, 3], 258, 4, True),
+    # more rows than are resident at once: CTAs of 128 threads
+    ("fp32", 3, 1, 40, 7, 2, [300, 0, 461], 3, 20, True),
+    ("mixed", 20, 2, 128, 33, 1, [5, 800], 2, 64, True),
+    ("bf16", 2, 1, 256, 9, 4, None, 750, 128, True),
+    ("bf16", 5, 5, 16, 2, 0, [0, 2, 1] * 300, 900, 8, True),
+    ("int4", 4, 2, 64, 19, 2, [790, 3], 2, 32, True),
 ]
 
 
