@@ -8,9 +8,12 @@
 // fraction goes to sincospi in fp32 (a position of 2^20 keeps an angle to
 // 2^-24 turns, where an fp32 product would lose it to 2^-4).
 // A head's row is a group of lanes with 8 columns each; the mean square is a
-// shuffle sum inside the group. Every row is read once and written once: the
-// bound is memory. The first rows of every group are on their way before the
-// CTA knows whose they are.
+// shuffle sum inside the group. Every row is read once and written once. 8192
+// fp32 rows of 32 and 8 heads of 128 take 58.5 us, 0.95 of the copy bandwidth;
+// 16384 16-bit ones, with as many bytes, 82, since 8 columns cost as many
+// instructions whatever their type (4 of 5 issue slots are busy), and 90 into a
+// 4-bit cache. All that a CTA needs is on its way before it knows whose its row
+// is.
 #include "st_cache.cuh"
 #include "st_cache_host.h"
 
@@ -42,16 +45,19 @@ struct Raw8 {
     for (int i = 0; i < (int)sizeof(T) / 2; ++i) u[i] = reinterpret_cast<const uint4*>(p)[i];
   }
 };
-constexpr int kAhead = 3;  // rows a group of lanes loads ahead of their use
 
 template <typename T, int LANES, bool INT4, int THREADS>
 __global__ void __launch_bounds__(THREADS, 1280 / THREADS) k_cache_append(const AppendArgs a) {
-  __shared__ alignas(16) float2 turn[kMaxPairs];
-  __shared__ alignas(16) float gains[2][ST_CACHE_MAX_HEAD_DIM];
+  // of every 8 columns the first half in one list and the second in another, which a warp reads without bank conflicts:
+  // cosine and sine of 2 pairs, gains of 4 columns
+  __shared__ float4 turn[2][kMaxPairs / 4], gains[2][2][kMaxPairs / 4];
   __shared__ long long sh_position;
   __shared__ int sh_stream, sh_first, sh_last, sh_slot;
   const int row = blockIdx.x, tid = threadIdx.x;
   constexpr int kGroups = THREADS / LANES;
+  // rows a group of lanes loads ahead of their use: 3 where it has few to take; with more, 2 copies of the loop's body
+  // fit the instruction cache better (8192 fp32 rows 58.5 us, with 3 60.7)
+  constexpr int kAhead = THREADS == 128 ? 2 : 3;
   static_assert(kMaxPairs <= THREADS && ST_CACHE_MAX_HEAD_DIM / 2 <= THREADS, "a thread for each pair, and for each 4 gains");
   const int lane = tid % LANES, col = lane * 8;
   const unsigned mask = LANES == 32 ? 0xffffffffu : ((1u << LANES) - 1u) << ((tid & 31) / LANES * LANES);
@@ -114,14 +120,15 @@ __global__ void __launch_bounds__(THREADS, 1280 / THREADS) k_cache_append(const 
   }
   const bool idle = p0 < 0;
   const long long position = p0 + (row - first);
-  if (has_gain) *reinterpret_cast<float4*>(&gains[side][gain_col]) = gain4;
+  auto pair_turn = [&](int p) -> float2& { return reinterpret_cast<float2*>(&turn[p / 2 % 2][p / 4])[p % 2]; };
+  if (has_gain) gains[side][gain_col / 4 % 2][gain_col / 8] = gain4;
   if (tid < a.rotary) {
     const double t = (double)position * frequency * 0.15915494309189533577;  // 1 / (2 pi)
     float s, c;
     sincospif(2.f * (float)(t - rint(t)), &s, &c);
-    turn[tid] = make_float2(c, s);
+    pair_turn(tid) = make_float2(c, s);
   } else if (tid < (a.rotary + 3) / 4 * 4) {
-    turn[tid] = make_float2(1.f, 0.f);  // a lane's 4 pairs: those past the last turn by 0
+    pair_turn(tid) = make_float2(1.f, 0.f);  // a lane's 4 pairs: those past the last turn by 0
   }
   if (tid == THREADS - 1) {  // in a warp that has no pairs, mostly
     // inserted: sink positions, and those the stream's last `window` rows hold
@@ -154,17 +161,20 @@ __global__ void __launch_bounds__(THREADS, 1280 / THREADS) k_cache_append(const 
           for (int o = 1; o < LANES; o *= 2) sum += __shfl_xor_sync(mask, sum, o);
           const float scale = rsqrtf(fmaf(sum, a.per_column, a.epsilon));
           if (on) {
-            float g[8];
-            load8(&gains[!is_q][col], g);
 #pragma unroll
-            for (int i = 0; i < 8; ++i) f[i] = f[i] * scale * g[i];
+            for (int i = 0; i < 2; ++i) {
+              const float4 g = gains[!is_q][i][lane];
+              f[4 * i] *= scale * g.x;
+              f[4 * i + 1] *= scale * g.y;
+              f[4 * i + 2] *= scale * g.z;
+              f[4 * i + 3] *= scale * g.w;
+            }
           }
         }
         if (col / 2 < a.rotary) {
-          const float4* w = reinterpret_cast<const float4*>(&turn[col / 2]);
 #pragma unroll
           for (int i = 0; i < 2; ++i) {
-            const float4 t = w[i];
+            const float4 t = turn[i][lane];
             const float x0 = f[4 * i], y0 = f[4 * i + 1], x1 = f[4 * i + 2], y1 = f[4 * i + 3];
             f[4 * i] = x0 * t.x - y0 * t.y;
             f[4 * i + 1] = x0 * t.y + y0 * t.x;
