@@ -310,9 +310,10 @@ typedef struct {
  * a negative position is idle: its cache stays, and its rows of q_out and k_out
  * become 0. Rows before starts[0] or behind the last stream's are left as they
  * were. q_out may be q itself and k_out k itself; beyond that nothing written
- * may overlap anything read. Positions stay below 2^53. Of a stream's new rows only those still in the window, or at a sink
- * position, are inserted. Sums and angles are fp32 or wider; each output is
- * rounded once (4-bit rows are quantised from the fp32 values). */
+ * may overlap anything read. Positions stay below 2^53, head strides of rows
+ * below 2^31 times 16 bytes. Of a stream's new rows only those still in the
+ * window, or at a sink position, are inserted. Sums and angles are fp32 or wider;
+ * each output is rounded once (4-bit rows are quantised from the fp32 values). */
 typedef struct {
   int mode;                 /* st_mode of q, k, v, q_out, k_out: the cache's type, or fp16/bf16 for INT4 */
   int heads;                /* query heads */

@@ -10,8 +10,8 @@
 // A head's row is a group of lanes with 8 columns each; the mean square is a
 // shuffle sum inside the group. Every row is read once and written once. 8192
 // fp32 rows of 32 and 8 heads of 128 take 58.5 us, 0.95 of the copy bandwidth;
-// 16384 16-bit ones, with as many bytes, 82, since 8 columns cost as many
-// instructions whatever their type (4 of 5 issue slots are busy), and 90 into a
+// 16384 16-bit ones, with as many bytes, 79, since 8 columns cost as many
+// instructions whatever their type (4 of 5 issue slots are busy), and 87 into a
 // 4-bit cache. All that a CTA needs is on its way before it knows whose its row
 // is.
 #include "st_cache.cuh"
@@ -24,7 +24,10 @@ constexpr int kMaxPairs = ST_CACHE_MAX_HEAD_DIM / 2;
 
 struct AppendArgs {
   void* q; void* k; void* v; void* q_out; void* k_out;
-  long long q_row, q_head, k_row, k_head, v_row, v_head, qo_row, qo_head, ko_row, ko_head;  // elements
+  long long q_row, k_row, v_row, qo_row, ko_row;  // elements
+  // pieces of 16 bytes: a head's address is then one multiply-add of 32 bits (16384 16-bit rows: 82.3 us from 64-bit
+  // strides, 79.3)
+  int q_head, k_head, v_head, qo_head, ko_head;
   void* keys; void* values;
   unsigned* key_scales; unsigned* value_scales;
   long long stream_stride, head_stride;  // cache rows
@@ -40,9 +43,9 @@ struct AppendArgs {
 template <typename T>
 struct Raw8 {
   uint4 u[sizeof(T) / 2];
-  __device__ __forceinline__ void load(const T* p) {
+  __device__ __forceinline__ void load(const uint4* p) {
 #pragma unroll
-    for (int i = 0; i < (int)sizeof(T) / 2; ++i) u[i] = reinterpret_cast<const uint4*>(p)[i];
+    for (int i = 0; i < (int)sizeof(T) / 2; ++i) u[i] = p[i];
   }
 };
 
@@ -64,13 +67,17 @@ __global__ void __launch_bounds__(THREADS, 1280 / THREADS) k_cache_append(const 
   const bool on = col < a.head_dim;
   const int tasks = a.heads + 2 * a.kv_heads;
   // task: a query head, then the key heads, then the value heads
-  const T* const q_row = static_cast<const T*>(a.q) + row * a.q_row + col;
-  const T* const k_row = static_cast<const T*>(a.k) + row * a.k_row + col;
-  const T* const v_row = static_cast<const T*>(a.v) + row * a.v_row + col;
+  auto at_row = [&](const void* rows, long long stride) {  // this thread's columns of head 0
+    return reinterpret_cast<const uint4*>(static_cast<const T*>(rows) + row * stride + col);
+  };
+  const uint4 *const q_row = at_row(a.q, a.q_row), *const k_row = at_row(a.k, a.k_row), *const v_row = at_row(a.v, a.v_row);
   auto source = [&](int task) {
     const int k = task - a.heads, v = k - a.kv_heads;
-    const long long stride = k < 0 ? a.q_head : v < 0 ? a.k_head : a.v_head;
-    return (k < 0 ? q_row : v < 0 ? k_row : v_row) + (k < 0 ? task : v < 0 ? k : v) * stride;
+    const int stride = k < 0 ? a.q_head : v < 0 ? a.k_head : a.v_head;
+    return (k < 0 ? q_row : v < 0 ? k_row : v_row) + (long long)(k < 0 ? task : v < 0 ? k : v) * stride;
+  };
+  auto result = [&](void* rows, long long row_stride, int head, int stride) {
+    return reinterpret_cast<T*>(const_cast<uint4*>(at_row(rows, row_stride)) + (long long)head * stride);
   };
   Raw8<T> ahead[kAhead];
 #pragma unroll
@@ -184,10 +191,10 @@ __global__ void __launch_bounds__(THREADS, 1280 / THREADS) k_cache_append(const 
         }
       }
       if (is_q) {
-        if (on) store8(static_cast<T*>(a.q_out) + row * a.qo_row + head * a.qo_head + col, f);
+        if (on) store8(result(a.q_out, a.qo_row, head, a.qo_head), f);
         continue;
       }
-      if (!is_v && a.k_out && on) store8(static_cast<T*>(a.k_out) + row * a.ko_row + head * a.ko_head + col, f);
+      if (!is_v && a.k_out && on) store8(result(a.k_out, a.ko_row, head, a.ko_head), f);
       if (slot < 0) continue;
       const long long at = stream * a.stream_stride + head * a.head_stride + slot;
       if (INT4) {
@@ -282,15 +289,22 @@ int st_cache_append(const st_cache* c, const st_append* p, void* stream) {
     return cache_fail(ST_ERR_INVALID, "rotary is 0 to head_dim / 2, with a frequency for each");
   for (const float* g : {p->q_gain, p->k_gain})
     if (reinterpret_cast<uintptr_t>(g) % 16) return cache_fail(ST_ERR_INVALID, "gains must start on a 16-byte boundary");
-  DeviceScope scope(c->device);
-  if (scope.status() != ST_OK) return scope.status();
   AppendArgs a{};
   a.q = p->q.data; a.k = p->k.data; a.v = p->v.data; a.q_out = p->q_out.data; a.k_out = p->k_out.data;
-  a.q_row = p->q.row_stride; a.q_head = p->q.head_stride;
-  a.k_row = p->k.row_stride; a.k_head = p->k.head_stride;
-  a.v_row = p->v.row_stride; a.v_head = p->v.head_stride;
-  a.qo_row = p->q_out.row_stride; a.qo_head = p->q_out.head_stride;
-  a.ko_row = p->k_out.row_stride; a.ko_head = p->k_out.head_stride;
+  const int per = p->mode == ST_MODE_FP32 ? 4 : 8;
+  const struct { const st_rows* rows; int heads; long long* row; int* head; const char* name; } sides[] = {
+      {&p->q, p->heads, &a.q_row, &a.q_head, "q"}, {&p->k, c->heads, &a.k_row, &a.k_head, "k"},
+      {&p->v, c->heads, &a.v_row, &a.v_head, "v"}, {&p->q_out, p->heads, &a.qo_row, &a.qo_head, "q_out"},
+      {&p->k_out, c->heads, &a.ko_row, &a.ko_head, "k_out"}};
+  for (const auto& x : sides) {
+    if (!x.rows->data) continue;  // no k_out
+    const long long stride = x.heads > 1 ? x.rows->head_stride / per : 0;
+    if (stride > INT32_MAX) return cache_fail(ST_ERR_INVALID, ": head strides are up to 2^31 - 1 times 16 bytes", x.name);
+    *x.row = x.rows->row_stride;
+    *x.head = (int)stride;
+  }
+  DeviceScope scope(c->device);
+  if (scope.status() != ST_OK) return scope.status();
   a.keys = c->keys; a.values = c->values;
   a.key_scales = static_cast<unsigned*>(c->key_scales); a.value_scales = static_cast<unsigned*>(c->value_scales);
   a.stream_stride = c->stream_stride; a.head_stride = c->head_stride;

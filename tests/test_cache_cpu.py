@@ -127,6 +127,7 @@ def test_cache_descriptors_that_are_refused(change, match):
     (dict(positions=None), "null positions"), (dict(epsilon=-1e-6), "epsilon"), (dict(epsilon=float("nan")), "epsilon"),
     (dict(epsilon=float("inf")), "epsilon"), (dict(rotary=33), "rotary"), (dict(rotary=-1), "rotary"),
     (dict(frequencies=None), "rotary"), (dict(q_gain=P + 4), "gains"),
+    (dict(q=Rows(P, 256, 2 ** 34)), "q: head strides"), (dict(k_out=Rows(P, 128, 2 ** 34)), "k_out: head strides"),
 ], ids=lambda v: str(v))
 def test_append_arguments_that_are_refused(change, match):
     refused(entry_points().st_cache_append(cache(), append(**change), None), match)
