@@ -66,6 +66,18 @@ __device__ __forceinline__ void store8(T* p, const float (&f)[8]) {
                                             pack2(p, f[6], f[7]));
 }
 
+__device__ __forceinline__ float max3(float a, float b, float c) {
+  float y;
+  asm("max.f32 %0, %1, %2, %3;" : "=f"(y) : "f"(a), "f"(b), "f"(c));
+  return y;
+}
+// The least of three, NaN if one is.
+__device__ __forceinline__ float min3_nan(float a, float b, float c) {
+  float y;
+  asm("min.NaN.f32 %0, %1, %2, %3;" : "=f"(y) : "f"(a), "f"(b), "f"(c));
+  return y;
+}
+
 // ---- 4-bit rows: {scale, lowest} of a group as one word, scale in the low half
 __device__ __forceinline__ float group_scale(unsigned pair) { return __uint_as_float(pair << 16); }
 __device__ __forceinline__ float group_lowest(unsigned pair) { return __uint_as_float(pair & 0xffff0000u); }
@@ -80,18 +92,16 @@ __device__ __forceinline__ void decode8(unsigned codes, unsigned pair, float (&f
 // and the group's {scale, lowest}. All 4 lanes of the group call it together;
 // `mask` names the lanes of the warp that do.
 __device__ __forceinline__ unsigned encode8(const float (&f)[8], unsigned mask, unsigned* pair) {
-  float low = f[0], high = f[0];
-  bool bad = false;  // fminf and fmaxf drop a NaN, so it is looked for
+  float low = min3_nan(f[0], f[1], f[2]), high = max3(f[0], f[1], f[2]);  // a NaN in `low` makes the range one
 #pragma unroll
-  for (int i = 0; i < 8; ++i) {
-    low = fminf(low, f[i]);
-    high = fmaxf(high, f[i]);
-    bad |= f[i] != f[i];
+  for (int i = 3; i < 8; i += 2) {
+    low = min3_nan(low, f[i], f[i < 7 ? i + 1 : i]);
+    high = max3(high, f[i], f[i < 7 ? i + 1 : i]);
   }
-  if (bad) low = -INFINITY;  // makes the range non-finite
 #pragma unroll
   for (int o = 1; o < 4; o *= 2) {
-    low = fminf(low, __shfl_xor_sync(mask, low, o));
+    const float other = __shfl_xor_sync(mask, low, o);
+    low = min3_nan(low, other, other);
     high = fmaxf(high, __shfl_xor_sync(mask, high, o));
   }
   const float range = __fsub_rn(high, low);

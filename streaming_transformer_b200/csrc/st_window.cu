@@ -259,11 +259,6 @@ __device__ __forceinline__ float exp2_fast(float x) {
   return y;
 }
 
-__device__ __forceinline__ float max3(float a, float b, float c) {
-  float y;
-  asm("max.f32 %0, %1, %2, %3;" : "=f"(y) : "f"(a), "f"(b), "f"(c));
-  return y;
-}
 // Two fp32 operations in one instruction.
 __device__ __forceinline__ float2 fma2(float2 a, float2 b, float2 c) {
   unsigned long long x, y, z, d;
