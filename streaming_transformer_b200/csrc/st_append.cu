@@ -8,12 +8,12 @@
 // fraction goes to sincospi in fp32 (a position of 2^20 keeps an angle to
 // 2^-24 turns, where an fp32 product would lose it to 2^-4).
 // A head's row is a group of lanes with 8 columns each; the mean square is a
-// shuffle sum inside the group. Every row is read once and written once. 8192
-// fp32 rows of 32 and 8 heads of 128 take 58.5 us, 0.95 of the copy bandwidth;
-// 16384 16-bit ones, with as many bytes, 79, since 8 columns cost as many
-// instructions whatever their type (4 of 5 issue slots are busy), and 87 into a
-// 4-bit cache. All that a CTA needs is on its way before it knows whose its row
-// is.
+// shuffle sum inside the group. Every row that a result or a slot needs is read
+// once and written once. 8192 fp32 rows of 32 and 8 heads of 128 take 57.7 us,
+// 0.97 of the copy bandwidth. 16-bit rows are bound by instructions, as 8 columns
+// cost as many whatever their type: 16384 take 79 us if all are inserted, and 65.5
+// with 8 streams of 2048 and a window of 512 (72 into 4-bit rows).
+// All that a CTA needs is on its way before it knows whose its row is.
 #include "st_cache.cuh"
 #include "st_cache_host.h"
 
@@ -42,7 +42,7 @@ struct AppendArgs {
 // 8 columns as they were loaded.
 template <typename T>
 struct Raw8 {
-  uint4 u[sizeof(T) / 2];
+  uint4 u[sizeof(T) / 2] = {};
   __device__ __forceinline__ void load(const uint4* p) {
 #pragma unroll
     for (int i = 0; i < (int)sizeof(T) / 2; ++i) u[i] = p[i];
@@ -58,9 +58,9 @@ __global__ void __launch_bounds__(THREADS, 1280 / THREADS) k_cache_append(const 
   __shared__ int sh_stream, sh_first, sh_last, sh_slot;
   const int row = blockIdx.x, tid = threadIdx.x;
   constexpr int kGroups = THREADS / LANES;
-  // rows a group of lanes loads ahead of their use: 3 where it has few to take; with more, 2 copies of the loop's body
-  // fit the instruction cache better (8192 fp32 rows 58.5 us, with 3 60.7)
-  constexpr int kAhead = THREADS == 128 ? 2 : 3;
+  // Rows a group of lanes loads ahead of their use, and copies of the loop's body. With 3 the instruction cache misses
+  // (8192 fp32 rows 58.5 us, with 3 60.7) or registers run short (256 fp32 rows 3.4 and 3.9).
+  constexpr int kAhead = 2;
   static_assert(kMaxPairs <= THREADS && ST_CACHE_MAX_HEAD_DIM / 2 <= THREADS, "a thread for each pair, and for each 4 gains");
   const int lane = tid % LANES, col = lane * 8;
   const unsigned mask = LANES == 32 ? 0xffffffffu : ((1u << LANES) - 1u) << ((tid & 31) / LANES * LANES);
@@ -125,7 +125,13 @@ __global__ void __launch_bounds__(THREADS, 1280 / THREADS) k_cache_append(const 
   } else {
     p0 = a.positions[row];
   }
-  const bool idle = p0 < 0;
+  if (p0 < 0) {  // idle
+    const float zeros[8] = {};
+    for (int task = tid / LANES; on && task < a.heads + (a.k_out ? a.kv_heads : 0); task += kGroups)
+      store8(task < a.heads ? result(a.q_out, a.qo_row, task, a.qo_head)
+                            : result(a.k_out, a.ko_row, task - a.heads, a.ko_head), zeros);
+    return;
+  }
   const long long position = p0 + (row - first);
   auto pair_turn = [&](int p) -> float2& { return reinterpret_cast<float2*>(&turn[p / 2 % 2][p / 4])[p % 2]; };
   if (has_gain) gains[side][gain_col / 4 % 2][gain_col / 8] = gain4;
@@ -134,14 +140,12 @@ __global__ void __launch_bounds__(THREADS, 1280 / THREADS) k_cache_append(const 
     float s, c;
     sincospif(2.f * (float)(t - rint(t)), &s, &c);
     pair_turn(tid) = make_float2(c, s);
-  } else if (tid < (a.rotary + 3) / 4 * 4) {
-    pair_turn(tid) = make_float2(1.f, 0.f);  // a lane's 4 pairs: those past the last turn by 0
   }
   if (tid == THREADS - 1) {  // in a warp that has no pairs, mostly
     // inserted: sink positions, and those the stream's last `window` rows hold
     const long long newest = p0 + (last - 1 - first);
     int slot = -1;
-    if (!idle && position >= 0) {  // a sum past 2^63 is not inserted
+    if (position >= 0) {  // a sum past 2^63 is not inserted
       if (position < a.sinks) slot = (int)position;
       else if (position > newest - a.window) slot = a.sinks + (int)((position - a.sinks) % a.window);
     }
@@ -149,17 +153,20 @@ __global__ void __launch_bounds__(THREADS, 1280 / THREADS) k_cache_append(const 
   }
   __syncthreads();
   const int slot = sh_slot;
-  for (int first = tid / LANES; first < tasks; first += kAhead * kGroups) {
+  // A row that is not inserted has no use for its values, nor for keys that are not asked for (16384 rows, a quarter of
+  // them inserted: 65.5 us, with the loads 79.3, of which conditions that this loop no longer has took 2).
+  const int end = slot >= 0 ? tasks : a.heads + (a.k_out ? a.kv_heads : 0), turns = a.rotary - col / 2;
+  for (int next = tid / LANES; next < end; next += kAhead * kGroups) {
 #pragma unroll
     for (int u = 0; u < kAhead; ++u) {
-      const int task = first + u * kGroups;
-      if (task >= tasks) break;
+      const int task = next + u * kGroups;
+      if (task >= end) break;
       const bool is_q = task < a.heads, is_v = task >= a.heads + a.kv_heads;
       const int head = is_q ? task : is_v ? task - a.heads - a.kv_heads : task - a.heads;
-      float f[8] = {};
-      if (on && !idle) load8(reinterpret_cast<const T*>(ahead[u].u), f);
-      if (on && task + kAhead * kGroups < tasks) ahead[u].load(source(task + kAhead * kGroups));
-      if (!is_v && !idle) {
+      float f[8];  // zeros past head_dim
+      load8(reinterpret_cast<const T*>(ahead[u].u), f);
+      if (on && task + kAhead * kGroups < end) ahead[u].load(source(task + kAhead * kGroups));
+      if (!is_v) {
         if (is_q ? a.q_gain : a.k_gain) {
           float sum = 0.f;
 #pragma unroll
@@ -167,27 +174,31 @@ __global__ void __launch_bounds__(THREADS, 1280 / THREADS) k_cache_append(const 
 #pragma unroll
           for (int o = 1; o < LANES; o *= 2) sum += __shfl_xor_sync(mask, sum, o);
           const float scale = rsqrtf(fmaf(sum, a.per_column, a.epsilon));
-          if (on) {
 #pragma unroll
-            for (int i = 0; i < 2; ++i) {
-              const float4 g = gains[!is_q][i][lane];
-              f[4 * i] *= scale * g.x;
-              f[4 * i + 1] *= scale * g.y;
-              f[4 * i + 2] *= scale * g.z;
-              f[4 * i + 3] *= scale * g.w;
-            }
+          for (int i = 0; i < 2; ++i) {
+            const float4 g = gains[!is_q][i][lane];
+            f[4 * i] *= scale * g.x;
+            f[4 * i + 1] *= scale * g.y;
+            f[4 * i + 2] *= scale * g.z;
+            f[4 * i + 3] *= scale * g.w;
           }
         }
-        if (col / 2 < a.rotary) {
+        auto rotate = [&](int pair, float c, float s) {
+          const float x = f[2 * pair], y = f[2 * pair + 1];
+          f[2 * pair] = x * c - y * s;
+          f[2 * pair + 1] = x * s + y * c;
+        };
+        if (turns >= 4) {
 #pragma unroll
           for (int i = 0; i < 2; ++i) {
             const float4 t = turn[i][lane];
-            const float x0 = f[4 * i], y0 = f[4 * i + 1], x1 = f[4 * i + 2], y1 = f[4 * i + 3];
-            f[4 * i] = x0 * t.x - y0 * t.y;
-            f[4 * i + 1] = x0 * t.y + y0 * t.x;
-            f[4 * i + 2] = x1 * t.z - y1 * t.w;
-            f[4 * i + 3] = x1 * t.w + y1 * t.z;
+            rotate(2 * i, t.x, t.y);
+            rotate(2 * i + 1, t.z, t.w);
           }
+        } else if (turns > 0) {  // the lane where the rotated columns end
+#pragma unroll
+          for (int i = 0; i < 3; ++i)
+            if (i < turns) rotate(i, pair_turn(col / 2 + i).x, pair_turn(col / 2 + i).y);
         }
       }
       if (is_q) {

@@ -767,3 +767,21 @@ def test_writes_are_seen_by_gradients():
         assert out._version == before + 1
     with torch.inference_mode():
         ops.cache_attention(q, keys, values, at, out=torch.empty_like(q))
+
+
+def test_columns_past_the_rotation_pass():
+    """Whatever they hold: a lane that has the last rotated pair does not touch the pair beside it."""
+    g = generator(41)
+    f = ops.rotation_frequencies(40)
+    for pairs in (0, 1, 3, 4, 13, 20):
+        q, k, v = (normal(g, 2, 2, 40, dtype=torch.float32) for _ in range(3))
+        for x in (q, k):
+            x[:, 0, 2 * pairs:] = float("inf")
+            x[:, 1, 2 * pairs + 1::2] = float("-inf")
+        keys, values, _, _ = ops.new_cache(2, 2, 4, 40, mode="fp32")
+        at = torch.tensor([5, 2], device="cuda")
+        out = ops.cache_append(q, k, v, keys, values, at, f[:pairs])
+        held = torch.stack([keys[0, :, 1], keys[1, :, 2]])
+        for x, y in ((q, out), (k, held)):
+            assert torch.equal(x[..., 2 * pairs:], y[..., 2 * pairs:])
+            assert torch.isfinite(y[..., :2 * pairs]).all()
