@@ -717,18 +717,18 @@ __global__ void __launch_bounds__(Tiles<DP, SUBS>::kThreads, Tiles<DP, SUBS>::kC
 }
 
 // ---------------------------------------------------------------- fp32 tiles
-// 32 query rows of one head by 128 threads; thread (ty, tx) of 8 x 16 has rows
-// 4 ty .. + 3 of everything, keys tx + 16 i of a 64-key tile in S, columns
-// 64 i + 4 tx .. + 3 of O: 16 multiply-adds for each 32 bytes read from shared
-// memory, rows padded by 16 bytes against bank conflicts. Key rows of the next
-// tile load under the second product, value rows under the first. 64 query rows
-// (8 a thread) read less and were slower, with half the warps an SM (2500 rows,
-// window 300, 32 heads of 64: 269 us against 226, a third of the fp32 rate).
-constexpr int kFp32Keys = 64, kFp32Threads = 128, kRowsEach = 4;
+// 8 RT query rows of one head by 128 threads; thread (ty, tx) of 8 x 16 has rows
+// RT ty .. + RT - 1 of everything, keys tx + 16 i of a 64-key tile in S, columns
+// 64 i + 4 tx .. + 3 of O. With RT = 4 that is 16 multiply-adds for each 32 bytes
+// read from shared memory; rows are padded by 16 bytes against bank conflicts. Key
+// rows of the next tile load under the second product, value rows under the first.
+// RT = 8 reads less and was slower, with half the warps an SM (2500 rows, window
+// 300, 32 heads of 64: 269 us against 226, a third of the fp32 rate).
+constexpr int kFp32Keys = 64, kFp32Threads = 128;
 
-template <int DP>
+template <int DP, int RT>
 struct Fp32Tiles {
-  static constexpr int kRows = 8 * kRowsEach, kRow = DP + 4, kPRow = kFp32Keys + 4;
+  static constexpr int kRows = 8 * RT, kRow = DP + 4, kPRow = kFp32Keys + 4;
   static constexpr int kFloats = (kRows + 2 * kFp32Keys) * kRow + kRows * kPRow;
   static constexpr int kSmem = kFloats * 4;
 };
@@ -737,10 +737,9 @@ __device__ __forceinline__ void copy16(float* dst, const float* src, bool in) {
   asm volatile("cp.async.cg.shared.global [%0], [%1], 16, %2;" ::"r"(smem_addr(dst)), "l"(src), "r"(in ? 16 : 0) : "memory");
 }
 
-template <int DP>
+template <int DP, int RT>
 __global__ void __launch_bounds__(kFp32Threads) k_window_fp32(const WindowArgs a) {
-  using G = Fp32Tiles<DP>;
-  constexpr int RT = kRowsEach;
+  using G = Fp32Tiles<DP, RT>;
   extern __shared__ float4 dynamic[];
   float* sq = reinterpret_cast<float*>(dynamic);
   float *sk = sq + G::kRows * G::kRow, *sv = sk + kFp32Keys * G::kRow, *sp = sv + kFp32Keys * G::kRow;
@@ -942,14 +941,24 @@ bool encode_rows(CUtensorMap* map, const st_rows& r, int mode, long long rows, i
                           CU_TENSOR_MAP_L2_PROMOTION_L2_256B, CU_TENSOR_MAP_FLOAT_OOB_FILL_NONE) == CUDA_SUCCESS;
 }
 
-template <int DP>
+template <int DP, int RT>
 cudaError_t launch_fp32(const WindowArgs& a, cudaStream_t s) {
-  using G = Fp32Tiles<DP>;
-  const cudaError_t e = cudaFuncSetAttribute(k_window_fp32<DP>, cudaFuncAttributeMaxDynamicSharedMemorySize, G::kSmem);
+  using G = Fp32Tiles<DP, RT>;
+  const cudaError_t e = cudaFuncSetAttribute(k_window_fp32<DP, RT>, cudaFuncAttributeMaxDynamicSharedMemorySize, G::kSmem);
   if (e != cudaSuccess) return e;
   const unsigned tiles = (unsigned)((a.rows + G::kRows - 1ll) / G::kRows);
-  k_window_fp32<DP><<<tiles * a.heads, kFp32Threads, G::kSmem, s>>>(a);
+  k_window_fp32<DP, RT><<<tiles * a.heads, kFp32Threads, G::kSmem, s>>>(a);
   return cudaSuccess;
+}
+// Few rows are dealt to more CTAs, 1 or 2 a thread: as long as those of 1 find an SM each, and those of 2 a place (4
+// heads of 64, window 64: 201 rows 6.6 us with 1, 7.7 with 2, 10.9 with 4; 400 rows 9.0, 7.7, 10.9; 1400 rows 17.1,
+// 13.8, 14.8; 2000 rows 25.1, 16.4, 15.0. Of 128: 400 rows 15.4, 11.4, 16.0; 1000 rows 36.9, 17.5, 16.3).
+template <int DP>
+cudaError_t launch_fp32(const WindowArgs& a, cudaStream_t s) {
+  constexpr long long kSms = 148;
+  if ((a.rows + 7ll) / 8 * a.heads <= kSms) return launch_fp32<DP, 1>(a, s);
+  if ((a.rows + 15ll) / 16 * a.heads <= kSms * (DP == 64 ? 3 : 1)) return launch_fp32<DP, 2>(a, s);
+  return launch_fp32<DP, 4>(a, s);
 }
 
 template <typename T, int DP, int SUBS>

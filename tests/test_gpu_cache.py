@@ -451,6 +451,12 @@ WINDOW = [
     ("fp32", 6, 2, 40, 17, 0, [1, 0, 130, 33]),
     ("fp32", 2, 1, 256, 1000, 4, [70, 65]),
     ("fp32", 3, 3, 8, 1, 1, [40]),
+    # rows and heads for each size of the fp32 tiles
+    ("fp32", 8, 2, 64, 100, 3, [300, 77]),
+    ("fp32", 16, 16, 24, 70, 2, [600]),
+    ("fp32", 6, 3, 96, 50, 1, [300, 1]),
+    ("fp32", 8, 1, 128, 90, 4, [500, 3]),
+    ("fp32", 1, 1, 128, 40, 2, [90]),
     ("mixed", 4, 4, 64, 100, 4, [301]),
     ("mixed", 7, 1, 80, 60, 1, [129, 127, 128, 1, 1, 300]),
     ("mixed", 2, 2, 128, 5, 200, [400, 3]),
@@ -501,14 +507,14 @@ def test_window_attention_matches_the_definition(case):
             ref.check(out[a:b], want, bound, f"rows {a}..{b}")
 
 
-@pytest.mark.parametrize("mode", ["fp32", "mixed", "bf16"])
+@pytest.mark.parametrize("mode,heads", [("fp32", 2), ("fp32", 6), ("fp32", 20), ("mixed", 2), ("bf16", 2), ("bf16", 4)])
 @pytest.mark.parametrize("where", [140, 200, 259])
-def test_non_finite_rows_reach_those_that_see_them_only(mode, where):
+def test_non_finite_rows_reach_those_that_see_them_only(mode, heads, where):
     g = generator(14)
     dtype = TYPES[mode]
     n, window = 420, 70
     sizes = [260, 160]
-    q, k, v = (normal(g, n, 2, 64, dtype=dtype) for _ in range(3))
+    q, k, v = (normal(g, n, h, 64, dtype=dtype) for h in (heads, 2, 2))
     v[where, 0] = float("nan")
     k[where, 1] = float("nan")
     out = ops.window_attention(q, k, v, window=window, sinks=1, starts=starts_of(sizes))
