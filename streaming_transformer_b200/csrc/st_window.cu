@@ -5,7 +5,7 @@
 // k_window_fp32: fp32 rows of up to 128 columns, tiled for the fp32 units (there
 // is no fp32 tensor product). k_window_rows: a few lanes walk the keys that one
 // query row of one head sees; it serves the rest (wider rows, 16-bit rows with a
-// scale that is not positive).
+// scale that is not positive, calls of a few rows).
 //
 // k_window_tiles. A CTA takes two tiles of 128 query rows, one TMEM lane a row,
 // that share their keys: two heads of one key head, or where a key head has an
@@ -1022,7 +1022,10 @@ extern "C" int st_window_attention(const st_window* p, void* stream) {
   a.heads = p->heads; a.kv_heads = p->kv_heads; a.head_dim = p->head_dim;
   a.window = p->window; a.sinks = p->sinks; a.scale = p->scale;
   cudaStream_t s = static_cast<cudaStream_t>(stream);
-  if (p->mode == ST_MODE_FP32 && p->head_dim <= 128 && (p->rows + 31) / 32 * p->heads <= INT32_MAX) {
+  // So few rows see so few keys that walking them one by one ends before a tile has been set up (bf16, 1 row: 2.2 us,
+  // in tiles 4.6 at 64 columns and 6.3 at 128; 4 rows: 3.2 to 3.6, and 4.6 and 6.6; 16: 7.6 to 7.9, and 4.9 and 6.7).
+  const bool few = p->rows <= 6;
+  if (!few && p->mode == ST_MODE_FP32 && p->head_dim <= 128 && (p->rows + 31) / 32 * p->heads <= INT32_MAX) {
     if ((rc = cache_cuda(p->head_dim <= 64 ? launch_fp32<64>(a, s) : launch_fp32<128>(a, s), "window attention: ")) != ST_OK) {
       cudaGetLastError();  // reported here, so not left pending
       return rc;
@@ -1031,7 +1034,7 @@ extern "C" int st_window_attention(const st_window* p, void* stream) {
   }
   TileMaps maps;
   const long long ctas = (p->rows + kTileRows - 1) / kTileRows * p->heads;
-  const bool tiles = p->mode != ST_MODE_FP32 && p->head_dim <= 128 && p->scale > 0.f && ctas <= INT32_MAX &&
+  const bool tiles = !few && p->mode != ST_MODE_FP32 && p->head_dim <= 128 && p->scale > 0.f && ctas <= INT32_MAX &&
                      encode_rows(&maps.q, p->q, p->mode, p->rows, p->heads, p->head_dim, kTileRows) &&
                      encode_rows(&maps.k, p->k, p->mode, p->rows, p->kv_heads, p->head_dim, kBlockRows) &&
                      encode_rows(&maps.v, p->v, p->mode, p->rows, p->kv_heads, p->head_dim, kBlockRows);

@@ -791,3 +791,18 @@ def test_columns_past_the_rotation_pass():
         for x, y in ((q, out), (k, held)):
             assert torch.equal(x[..., 2 * pairs:], y[..., 2 * pairs:])
             assert torch.isfinite(y[..., :2 * pairs]).all()
+
+
+@pytest.mark.parametrize("mode", ["fp32", "mixed", "bf16"])
+@pytest.mark.parametrize("dim", [64, 128])
+@pytest.mark.parametrize("n", [1, 2, 6, 7, 8])
+def test_window_attention_of_a_few_rows(mode, dim, n):
+    g = generator(43)
+    dtype = TYPES[mode]
+    q, k, v = (normal(g, n, h, dim, dtype=dtype) for h in (4, 2, 2))
+    for sizes in (None, [n - 1, 0, 1]):
+        starts, edges = (starts_of(sizes), starts_of(sizes).tolist()) if sizes else (None, [0, n])
+        for window, sinks in ((1, 0), (3, 1), (100, 4)):
+            out = ops.window_attention(q, k, v, window=window, sinks=sinks, starts=starts)
+            for a, b, want, bound in window_reference(q, k, v, edges, window, sinks, dim ** -0.5, dtype):
+                ref.check(out[a:b], want, bound, f"window {window}, rows {a}..{b}")
