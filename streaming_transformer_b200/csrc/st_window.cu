@@ -1,16 +1,16 @@
 // st_window.cu -- causal attention of packed sequences with a sliding window
 // and sinks (st_window_attention).
 //
-// Three kernels. k_window_tiles: 16-bit rows of up to 128 columns, on tcgen05.
+// Three kernels. k_window_tiles: 16-bit rows, on tcgen05.
 // k_window_fp32: fp32 rows of up to 128 columns, tiled for the fp32 units (there
 // is no fp32 tensor product). k_window_rows: a few lanes walk the keys that one
-// query row of one head sees; it serves the rest (wider rows, 16-bit rows with a
-// scale that is not positive, calls of a few rows).
+// query row of one head sees; it serves the rest (wider fp32 rows, 16-bit rows
+// with a scale that is not positive, calls of a few rows).
 //
 // k_window_tiles. A CTA takes two tiles of 128 query rows, one TMEM lane a row,
 // that share their keys: two heads of one key head, or where a key head has an
-// odd number of them two neighbouring tiles of one head (up to 64 columns one
-// tile then, see launch_tiles). Rows may belong to
+// odd number of them two neighbouring tiles of one head (one tile: past 128 columns,
+// and then up to 64, see launch_tiles). Rows may belong to
 // several sequences: the keys that are needed are those from the first row's
 // window on, which covers every sequence that begins behind it, and the sinks of
 // the first row's sequence. They are walked in blocks of 32 rows (sinks first,
@@ -74,7 +74,9 @@ __device__ int sequence_start(const WindowArgs& a, int row, int* end = nullptr) 
 }
 
 // One query row of one head by a group of LANES lanes (`mask`: those lanes of the warp).
-template <typename T, int LANES>
+// KEYS at a time: 2 where that is all a kernel does (201 fp32 rows of 256 columns 27.5 -> 18.5 us, bf16 9 % less; 4 take
+// more registers: 17 % more), 1 where another kernel falls back on it.
+template <typename T, int LANES, int KEYS = 1>
 __device__ __forceinline__ void window_row(const WindowArgs& a, int row, int start, int h, int lane, unsigned mask) {
   const int kv = h / (a.heads / a.kv_heads);
   const bool on = lane * 8 < a.head_dim;
@@ -88,23 +90,41 @@ __device__ __forceinline__ void window_row(const WindowArgs& a, int row, int sta
   const long long sinks = (long long)start + a.sinks;                         // first row behind the sinks
   int j = start < low && a.sinks > 0 ? start : low;
   while (j <= row) {
-    float k[8] = {}, v[8] = {}, dot = 0.f;
-    if (on) {
-      load8(kp + j * a.k_row, k);
-      load8(vp + j * a.v_row, v);
+    float k[KEYS][8] = {}, v[KEYS][8] = {}, dot[KEYS] = {};
+    bool seen[KEYS];
+#pragma unroll
+    for (int u = 0; u < KEYS; ++u) {
+      seen[u] = j <= row;
+      if (seen[u] && on) {
+        load8(kp + j * a.k_row, k[u]);
+        load8(vp + j * a.v_row, v[u]);
+      }
+      ++j;
+      if (j < low && j >= sinks) j = low;
     }
 #pragma unroll
-    for (int i = 0; i < 8; ++i) dot = fmaf(q[i], k[i], dot);
+    for (int i = 0; i < 8; ++i)
 #pragma unroll
-    for (int o = 1; o < LANES; o *= 2) dot += __shfl_xor_sync(mask, dot, o);
-    const float top = fmaxf(m, dot), keep = top == -INFINITY ? 1.f : __expf(m - top);
-    const float p = __expf(dot - (top == -INFINITY ? 0.f : top));  // a NaN stays one
+      for (int u = 0; u < KEYS; ++u) dot[u] = fmaf(q[i], k[u][i], dot[u]);
+#pragma unroll
+    for (int o = 1; o < LANES; o *= 2)
+#pragma unroll
+      for (int u = 0; u < KEYS; ++u) dot[u] += __shfl_xor_sync(mask, dot[u], o);
+    float top = m;
+#pragma unroll
+    for (int u = 0; u < KEYS; ++u) top = seen[u] ? fmaxf(top, dot[u]) : top;
+    const float ref = top == -INFINITY ? 0.f : top, keep = top == -INFINITY ? 1.f : __expf(m - top);
     m = top;
-    l = fmaf(l, keep, p);
+    l *= keep;
 #pragma unroll
-    for (int i = 0; i < 8; ++i) acc[i] = fmaf(acc[i], keep, p * v[i]);
-    ++j;
-    if (j < low && j >= sinks) j = low;
+    for (int i = 0; i < 8; ++i) acc[i] *= keep;
+#pragma unroll
+    for (int u = 0; u < KEYS; ++u) {
+      const float p = seen[u] ? __expf(dot[u] - ref) : 0.f;  // a NaN stays one
+      l += p;
+#pragma unroll
+      for (int i = 0; i < 8; ++i) acc[i] = fmaf(p, v[u][i], acc[i]);
+    }
   }
 #pragma unroll
   for (int i = 0; i < 8; ++i) acc[i] /= l;
@@ -122,7 +142,7 @@ __global__ void __launch_bounds__(kWindowThreads) k_window_rows(const WindowArgs
   if (row >= a.rows) return;
   const int start = sequence_start(a, (int)row);
   if (start < 0) return;
-  window_row<T, LANES>(a, (int)row, start, blockIdx.y, threadIdx.x % LANES, row_mask<LANES>());
+  window_row<T, LANES, 2>(a, (int)row, start, blockIdx.y, threadIdx.x % LANES, row_mask<LANES>());
 }
 
 // ---------------------------------------------------------------- tcgen05
@@ -139,17 +159,18 @@ __device__ __forceinline__ bool wait_phase(unsigned long long* bar, unsigned par
   return false;
 }
 
-// DP: columns, padded to 64 or 128 with zeros by the copies; SUBS: query tiles of a CTA. Key tiles are DP rows: S and O
-// take DP TMEM columns each for each query tile, so that one CTA of 128 columns, or two (four of one query tile) of 64,
-// fill an SM's TMEM.
+// DP: columns, padded to 64, 128 or 256 with zeros by the copies; SUBS: query tiles of a CTA. S and O take DP TMEM
+// columns each for each query tile, so that one CTA of 128 or 256 columns, or two (four of one query tile) of 64, fill an
+// SM's TMEM. Key tiles are DP rows, of 256 columns 64: shared memory holds no more (2 sequences of 4000 rows, window 4000,
+// 16 heads of 256: 562 us, 619 TFLOP/s).
 template <int DP, int SUBS>
 struct Tiles {
-  static constexpr int kKeys = DP, kBlocks = kKeys / kBlockRows, kPanels = DP / 64;
+  static constexpr int kKeys = DP == 256 ? 64 : DP, kBlocks = kKeys / kBlockRows, kPanels = DP / 64;
   static constexpr int kQBytes = kPanels * kTileRows * 128, kKvBytes = kPanels * kKeys * 128;
   // 4 warps of rows for each tile, one that copies, one that issues products; at 128 columns two more, which make the
   // last four a warpgroup that hands registers to the others
   static constexpr int kCopyWarp = 4 * SUBS, kIssueWarp = kCopyWarp + 1;
-  static constexpr int kThreads = DP == 128 ? 384 : kIssueWarp * 32 + 32, kCtas = 128 / DP * 2 / SUBS;
+  static constexpr int kThreads = DP == 128 ? 384 : kIssueWarp * 32 + 32, kCtas = DP == 64 ? 4 / SUBS : 1;
   // One ring for K and V tiles in the order of their use: two are being read, the others are on their way. With two
   // slots each (one ahead) the products waited for the copies.
   static constexpr int kSlots = DP == 128 ? 5 : 4 * SUBS;
@@ -571,7 +592,7 @@ __global__ void __launch_bounds__(Tiles<DP, SUBS>::kThreads, Tiles<DP, SUBS>::kC
       }
       if (!(ok = wait(&s_full[side], n))) break;
       tc_fence_after();
-      // At 128 columns the registers hold the tile between the passes, at 64 (two CTAs an SM) it is read again.
+      // At 128 columns the registers hold the tile between the passes, else it is read again.
       constexpr bool kKeep = DP == 128;
       float x[kKeep ? 2 : 1][kKeep ? 64 : 32], tops[4] = {-INFINITY, -INFINITY, -INFINITY, -INFINITY};  // for latency
       auto mask = [&](int b, auto& y, int from) {
@@ -979,6 +1000,7 @@ cudaError_t launch_tiles(const WindowArgs& a, const TileMaps& maps, cudaStream_t
 // they do, as the keys then come twice (4 key heads of 16: 41.0 and 39.2; 8192 rows, 8 of 32, window 512: 97 and 94).
 template <typename T>
 cudaError_t launch_tiles(const WindowArgs& a, const TileMaps& maps, cudaStream_t s) {
+  if (a.head_dim > 128) return launch_tiles<T, 256, 1>(a, maps, s);
   if (a.head_dim > 64) return launch_tiles<T, 128, 2>(a, maps, s);
   return a.heads / a.kv_heads % 2 == 0 ? launch_tiles<T, 64, 2>(a, maps, s) : launch_tiles<T, 64, 1>(a, maps, s);
 }
@@ -1034,7 +1056,7 @@ extern "C" int st_window_attention(const st_window* p, void* stream) {
   }
   TileMaps maps;
   const long long ctas = (p->rows + kTileRows - 1) / kTileRows * p->heads;
-  const bool tiles = !few && p->mode != ST_MODE_FP32 && p->head_dim <= 128 && p->scale > 0.f && ctas <= INT32_MAX &&
+  const bool tiles = !few && p->mode != ST_MODE_FP32 && p->scale > 0.f && ctas <= INT32_MAX &&
                      encode_rows(&maps.q, p->q, p->mode, p->rows, p->heads, p->head_dim, kTileRows) &&
                      encode_rows(&maps.k, p->k, p->mode, p->rows, p->kv_heads, p->head_dim, kBlockRows) &&
                      encode_rows(&maps.v, p->v, p->mode, p->rows, p->kv_heads, p->head_dim, kBlockRows);

@@ -462,6 +462,10 @@ WINDOW = [
     ("mixed", 2, 2, 128, 5, 200, [400, 3]),
     ("mixed", 4, 1, 256, 33, 2, [150]),
     ("bf16", 16, 16, 64, 256, 4, [511, 257, 13]),
+    ("bf16", 8, 2, 256, 300, 5, [700, 1, 129]),
+    ("mixed", 6, 3, 136, 90, 70, [31, 400, 2]),
+    ("bf16", 2, 1, 192, 2 ** 33, 0, [260]),
+    ("bf16", 3, 3, 248, 1, 1, [128, 64]),
     ("bf16", 32, 8, 128, 500, 16, [1200]),
     ("bf16", 8, 2, 96, 1, 0, [140]),
     ("bf16", 8, 1, 128, 130, 3, [0, 0, 260, 0, 100, 0]),
@@ -507,14 +511,15 @@ def test_window_attention_matches_the_definition(case):
             ref.check(out[a:b], want, bound, f"rows {a}..{b}")
 
 
-@pytest.mark.parametrize("mode,heads", [("fp32", 2), ("fp32", 6), ("fp32", 20), ("mixed", 2), ("bf16", 2), ("bf16", 4)])
+@pytest.mark.parametrize("mode,heads,dim", [("fp32", 2, 64), ("fp32", 6, 64), ("fp32", 20, 64), ("mixed", 2, 64), ("bf16", 2, 64),
+                                            ("bf16", 4, 64), ("bf16", 4, 128), ("mixed", 2, 192)])
 @pytest.mark.parametrize("where", [140, 200, 259])
-def test_non_finite_rows_reach_those_that_see_them_only(mode, heads, where):
+def test_non_finite_rows_reach_those_that_see_them_only(mode, heads, dim, where):
     g = generator(14)
     dtype = TYPES[mode]
     n, window = 420, 70
     sizes = [260, 160]
-    q, k, v = (normal(g, n, h, 64, dtype=dtype) for h in (heads, 2, 2))
+    q, k, v = (normal(g, n, h, dim, dtype=dtype) for h in (heads, 2, 2))
     v[where, 0] = float("nan")
     k[where, 1] = float("nan")
     out = ops.window_attention(q, k, v, window=window, sinks=1, starts=starts_of(sizes))
@@ -522,7 +527,7 @@ def test_non_finite_rows_reach_those_that_see_them_only(mode, heads, where):
     hit[where:min(where + window, 260)] = True
     assert torch.isnan(out[hit]).all()
     clean = [torch.where(torch.isnan(x), 0.0, x.float()).to(dtype) for x in (k, v)]
-    for a, b, want, bound in window_reference(q, *clean, [0, 260, 420], window, 1, 0.125, dtype):
+    for a, b, want, bound in window_reference(q, *clean, [0, 260, 420], window, 1, dim ** -0.5, dtype):
         keep = ~hit[a:b]
         ref.check(out[a:b][keep], want[keep], bound[keep], f"rows {a}..{b}")
 
@@ -794,7 +799,7 @@ def test_columns_past_the_rotation_pass():
 
 
 @pytest.mark.parametrize("mode", ["fp32", "mixed", "bf16"])
-@pytest.mark.parametrize("dim", [64, 128])
+@pytest.mark.parametrize("dim", [64, 128, 256])
 @pytest.mark.parametrize("n", [1, 2, 6, 7, 8])
 def test_window_attention_of_a_few_rows(mode, dim, n):
     g = generator(43)
