@@ -28,8 +28,9 @@ A stream that starts with a backlog runs ``cache_append`` and
 Work is queued on the current stream of the tensors' device, which may be
 another device than the current one; nothing waits. Positions and starts are
 read on the device, so a captured CUDA graph replays with new ones. There is no
-backward pass: a call with an input that requires a gradient raises while
-gradients are on. Errors are ``StreamError`` with the C status, as the runtime's.
+backward pass: a call with an input (frequencies, gains and scales among them)
+or a cache that requires a gradient raises while gradients are on, and one with
+a forward-mode tangent always. Errors are ``StreamError`` with the C status, as the runtime's.
 """
 from __future__ import annotations
 

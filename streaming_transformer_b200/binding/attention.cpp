@@ -10,7 +10,7 @@
 
 #include <ATen/core/Tensor.h>
 #include <ATen/ops/empty.h>
-#include <c10/core/GradMode.h>
+#include <c10/core/AutogradState.h>
 #include <c10/cuda/CUDAStream.h>
 #include <torch/csrc/autograd/python_variable.h>
 
@@ -71,10 +71,16 @@ int row_mode(const at::Tensor& t, const char* name) {
   return mode;
 }
 
+// Refuses tensors whose derivative a call would drop: every floating-point one that it reads or writes is named here,
+// before any other check. Forward-mode tangents (there is one level, 0) count with gradients off as well.
 void no_gradient(std::initializer_list<const at::Tensor*> tensors) {
-  if (!c10::GradMode::is_enabled()) return;
-  for (const at::Tensor* t : tensors)
-    if (t && t->requires_grad()) refuse("there is no backward pass: detach the inputs or call under torch.no_grad()");
+  const c10::AutogradState& state = c10::AutogradState::get_tls_state();
+  for (const at::Tensor* t : tensors) {
+    if (!t) continue;
+    if (state.get_grad_mode() && t->requires_grad())
+      refuse("there is no backward pass: detach the inputs or call under torch.no_grad()");
+    if (state.get_fw_grad_mode() && t->_fw_grad(0).defined()) refuse("there is no forward-mode derivative: detach the inputs");
+  }
 }
 
 // Counts a write, so that a backward pass which saved the old values of one of these raises, as for torch's own.
@@ -204,13 +210,13 @@ PyObject* do_append(PyObject* const* o) {
   const at::Tensor *starts = optional_tensor(o[8], "starts"), *q_gain = optional_tensor(o[9], "q_gain"),
                    *k_gain = optional_tensor(o[10], "k_gain"), *key_scales = optional_tensor(o[12], "key_scales"),
                    *value_scales = optional_tensor(o[13], "value_scales"), *given = optional_tensor(o[15], "out");
+  no_gradient({&q, &k, &v, &keys, &values, &frequencies, q_gain, k_gain, key_scales, value_scales, given});
   const st_cache c = cache_of(keys, values, key_scales, value_scales, integer(o[7], "sinks"));
   const c10::Device device = keys.device();
   const at::ScalarType type = q.scalar_type();
   st_append a{};
   a.mode = row_mode(q, "q");
   a.heads = heads_of(q, "[rows, heads, head_dim]");
-  no_gradient({&q, &k, &v, &keys, &values, q_gain, k_gain, given});
   const int64_t rows = a.rows = q.size(0);
   a.q = rows_of(q, "q", device, type, rows, a.heads, c.head_dim);
   a.k = rows_of(k, "k", device, type, rows, c.heads, c.head_dim);
@@ -252,13 +258,13 @@ PyObject* do_attend(PyObject* const* o) {
                    &positions = tensor(o[3], "positions");
   const at::Tensor *key_scales = optional_tensor(o[4], "key_scales"), *value_scales = optional_tensor(o[5], "value_scales"),
                    *given = optional_tensor(o[7], "out");
+  no_gradient({&q, &keys, &values, key_scales, value_scales, given});
   const st_cache c = cache_of(keys, values, key_scales, value_scales, 0);
   const c10::Device device = keys.device();
   const at::ScalarType type = q.scalar_type();
   st_attend a{};
   a.mode = row_mode(q, "q");
   a.heads = heads_of(q, "[streams, heads, head_dim]");
-  no_gradient({&q, &keys, &values, given});
   a.scale = o[6] == Py_None ? (float)(1.0 / std::sqrt((double)c.head_dim)) : (float)number(o[6], "scale");
   a.q = rows_of(q, "q", device, type, c.streams, a.heads, c.head_dim);
   at::Tensor out = given ? *given : fresh({c.streams, a.heads, c.head_dim}, type, device), work;
@@ -279,6 +285,7 @@ PyObject* do_attend(PyObject* const* o) {
 PyObject* do_unpack(PyObject* const* o) {
   const at::Tensor &keys = tensor(o[0], "keys"), &values = tensor(o[1], "values");
   const at::Tensor *key_scales = optional_tensor(o[2], "key_scales"), *value_scales = optional_tensor(o[3], "value_scales");
+  no_gradient({key_scales, value_scales});
   const st_cache c = cache_of(keys, values, key_scales, value_scales, 0);
   const at::ScalarType type = tensor(o[4], "dtype").scalar_type();
   const int mode = row_mode(THPVariable_Unpack(o[4]), "dtype");
@@ -297,6 +304,7 @@ PyObject* do_unpack(PyObject* const* o) {
 PyObject* do_window(PyObject* const* o) {
   const at::Tensor &q = tensor(o[0], "q"), &k = tensor(o[1], "k"), &v = tensor(o[2], "v");
   const at::Tensor *starts = optional_tensor(o[5], "starts"), *given = optional_tensor(o[7], "out");
+  no_gradient({&q, &k, &v, given});
   if (!q.is_cuda()) refuse("q: expected a CUDA tensor, got " + q.device().str());
   const c10::Device device = q.device();
   const at::ScalarType type = q.scalar_type();
@@ -305,7 +313,6 @@ PyObject* do_window(PyObject* const* o) {
   a.mode = row_mode(q, "q");
   a.heads = heads_of(q, "[rows, heads, head_dim]");
   if (k.dim() != 3 || k.size(1) > 65535) refuse("k: expected [rows, key heads, head_dim]");
-  no_gradient({&q, &k, &v, given});
   const int64_t window = integer(o[3], "window"), sinks = integer(o[4], "sinks"), rows = a.rows = q.size(0), dim = q.size(2);
   if (window < 1 || sinks < 0) refuse("window is at least 1 and sinks at least 0");
   // no sequence is longer than the largest int: a wider window sees as much

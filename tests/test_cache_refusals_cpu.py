@@ -1,0 +1,66 @@
+"""Refusals of the window-cache operators that need no GPU: derivatives that a call
+would drop, and C arguments that a kernel could not read."""
+import pytest
+
+torch = pytest.importorskip("torch")
+
+from streaming_transformer_b200 import StreamError
+from streaming_transformer_b200 import attention as ops
+
+
+def append_arguments(four):
+    """Names to tensors of one append; None where there is none."""
+    row = torch.zeros(1, 1, 64, dtype=torch.bfloat16)
+    cache = ops.new_cache(1, 1, 4, 64, mode="int4" if four else "bf16", device="cpu")
+    return dict(zip(("keys", "values", "key_scales", "value_scales"), cache)) | dict(
+        q=row.clone(), k=row.clone(), v=row.clone(), frequencies=ops.rotation_frequencies(64, device="cpu"),
+        q_gain=torch.ones(64), k_gain=torch.ones(64), out=row.clone())
+
+
+def append(t):
+    return ops.cache_append(t["q"], t["k"], t["v"], t["keys"], t["values"], torch.zeros(1, dtype=torch.int64), t["frequencies"],
+                            q_gain=t["q_gain"], k_gain=t["k_gain"], key_scales=t["key_scales"], value_scales=t["value_scales"],
+                            out=t["out"])
+
+
+def attend(t):
+    return ops.cache_attention(t["q"], t["keys"], t["values"], torch.zeros(1, dtype=torch.int64), key_scales=t["key_scales"],
+                               value_scales=t["value_scales"], out=t["out"])
+
+
+def unpack(t):
+    return ops.unpack_cache(t["keys"], t["values"], key_scales=t["key_scales"], value_scales=t["value_scales"])
+
+
+def window(t):
+    return ops.window_attention(t["q"], t["k"], t["v"], window=2, out=t["out"])
+
+
+# every floating-point tensor of every call, with a cache of 16-bit or of 4-bit rows
+DERIVATIVES = [(append, four, name) for four in (False, True) for name in ("q", "k", "v", "frequencies", "q_gain", "k_gain", "out")]
+DERIVATIVES += [(append, False, "keys"), (append, False, "values"), (append, True, "key_scales"), (append, True, "value_scales")]
+DERIVATIVES += [(attend, False, name) for name in ("q", "keys", "values", "out")]
+DERIVATIVES += [(attend, True, name) for name in ("q", "key_scales", "value_scales", "out")]
+DERIVATIVES += [(unpack, True, "key_scales"), (unpack, True, "value_scales")]
+DERIVATIVES += [(window, False, name) for name in ("q", "k", "v", "out")]
+
+
+@pytest.mark.parametrize("call,four,name", DERIVATIVES, ids=lambda v: v.__name__ if callable(v) else str(v))
+def test_a_derivative_is_never_dropped(call, four, name):
+    t = append_arguments(four)
+    t[name].requires_grad_()
+    with pytest.raises(StreamError, match="no backward pass"):
+        call(t)
+    with torch.no_grad(), pytest.raises(StreamError, match="expected a CUDA tensor"):   # past the gradients' check
+        call(t)
+
+
+@pytest.mark.parametrize("call,four,name", DERIVATIVES, ids=lambda v: v.__name__ if callable(v) else str(v))
+def test_a_tangent_is_never_dropped(call, four, name):
+    t = append_arguments(four)
+    with torch.autograd.forward_ad.dual_level(), torch.no_grad():
+        t[name] = torch.autograd.forward_ad.make_dual(t[name], torch.ones_like(t[name]))
+        with pytest.raises(StreamError, match="no forward-mode derivative"):
+            call(t)
+    with pytest.raises(StreamError, match="expected a CUDA tensor"):
+        call(append_arguments(four))
