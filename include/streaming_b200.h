@@ -271,8 +271,9 @@ const char* st_attention_static_error(void);
  * max - min or bf16(min) is not finite, reads back as NaN. Attention takes
  * value scales from 2^-56 to 2^56 (or 0) and queries below 2^120.
  *
- * All pointers are device memory of `device`, rows start on 16-byte
- * boundaries, and work is queued on `stream` (a cudaStream_t) without waiting.
+ * All pointers are device memory of `device`, rows, scales and gains start on
+ * 16-byte boundaries, positions, starts and frequencies on those of their
+ * values, and work is queued on `stream` (a cudaStream_t) without waiting.
  * Positions and starts are read on the device, so a captured graph replays
  * with new ones. Each call returns ST_OK or an ST_ERR_* code with its message
  * in st_cache_error() (one per thread). A CUDA error already pending on the

@@ -298,6 +298,9 @@ int st_cache_append(const st_cache* c, const st_append* p, void* stream) {
   if (!(p->epsilon >= 0.f) || p->epsilon > 3.0e38f) return cache_fail(ST_ERR_INVALID, "epsilon must be finite and >= 0");
   if (p->rotary < 0 || p->rotary > c->head_dim / 2 || (p->rotary && !p->frequencies))
     return cache_fail(ST_ERR_INVALID, "rotary is 0 to head_dim / 2, with a frequency for each");
+  if ((rc = check_aligned(p->positions, "positions", 8)) != ST_OK || (rc = check_aligned(p->starts, "starts", 4)) != ST_OK ||
+      (rc = check_aligned(p->rotary ? p->frequencies : nullptr, "frequencies", 8)) != ST_OK)
+    return rc;
   for (const float* g : {p->q_gain, p->k_gain})
     if (reinterpret_cast<uintptr_t>(g) % 16) return cache_fail(ST_ERR_INVALID, "gains must start on a 16-byte boundary");
   AppendArgs a{};

@@ -836,6 +836,7 @@ int st_cache_attention(const st_cache* c, const st_attend* p, void* stream) {
       (rc = check_rows(p->out, "out", p->mode, c->streams, p->heads, c->head_dim, true)) != ST_OK)
     return rc;
   if (!p->positions) return cache_fail(ST_ERR_INVALID, "null positions");
+  if ((rc = check_aligned(p->positions, "positions", 8)) != ST_OK) return rc;
   if (!(fabsf(p->scale) <= 0x1p64f)) return cache_fail(ST_ERR_INVALID, "scale must be within 2^64");
   DeviceScope scope(c->device);
   if (scope.status() != ST_OK) return scope.status();

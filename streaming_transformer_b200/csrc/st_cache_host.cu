@@ -81,6 +81,11 @@ int check_rows(const st_rows& r, const char* name, int mode, int64_t rows, int h
   return ST_OK;
 }
 
+int check_aligned(const void* p, const char* name, unsigned bytes) {
+  return reinterpret_cast<uintptr_t>(p) % bytes == 0
+             ? ST_OK : cache_fail(ST_ERR_INVALID, " must be on a boundary of the size of its values", name);
+}
+
 DeviceScope::DeviceScope(int device) {
   int current = 0;
   if ((status_ = cache_cuda(cudaGetDevice(&current), "cudaGetDevice: ")) != ST_OK) return;

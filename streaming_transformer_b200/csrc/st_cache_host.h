@@ -23,6 +23,8 @@ inline int mode_bytes(int mode) { return mode == ST_MODE_FP32 ? 4 : 2; }
 int check_cache(const st_cache* c, bool writes);
 // Checks rows [rows][heads][head_dim] of `mode`; `writes` as above.
 int check_rows(const st_rows& r, const char* name, int mode, int64_t rows, int heads, int head_dim, bool writes);
+// Checks that `p` (NULL passes) is on a boundary of `bytes`, the size of the values that a kernel loads from it.
+int check_aligned(const void* p, const char* name, unsigned bytes);
 
 // Makes `device` current for the calls of a scope and restores the caller's;
 // status() is an ST_ERR_CUDA when the device cannot be taken or an error of an

@@ -1030,6 +1030,7 @@ extern "C" int st_window_attention(const st_window* p, void* stream) {
       (rc = check_rows(p->v, "v", p->mode, p->rows, p->kv_heads, p->head_dim, false)) != ST_OK ||
       (rc = check_rows(p->out, "out", p->mode, p->rows, p->heads, p->head_dim, true)) != ST_OK)
     return rc;
+  if ((rc = check_aligned(p->starts, "starts", 4)) != ST_OK) return rc;
   if (p->out.data == p->q.data || p->out.data == p->k.data || p->out.data == p->v.data)
     return cache_fail(ST_ERR_INVALID, "out may not be an input");
   DeviceScope scope(p->device);

@@ -4,6 +4,8 @@ import pytest
 
 torch = pytest.importorskip("torch")
 
+from test_cache_cpu import FOUR, P, append as append_struct, attend as attend_struct, cache, entry_points, refused, window as window_struct
+
 from streaming_transformer_b200 import StreamError
 from streaming_transformer_b200 import attention as ops
 
@@ -64,3 +66,21 @@ def test_a_tangent_is_never_dropped(call, four, name):
             call(t)
     with pytest.raises(StreamError, match="expected a CUDA tensor"):
         call(append_arguments(four))
+
+
+@pytest.mark.parametrize("name,by", [("positions", 4), ("positions", 1), ("starts", 2), ("frequencies", 4)])
+@pytest.mark.parametrize("four", [False, True])
+def test_misaligned_values_of_an_append_are_refused(name, by, four):
+    # a kernel's load from such an address would fault
+    change = {"starts": P, name: P + by}
+    refused(entry_points().st_cache_append(cache(**(FOUR if four else {})), append_struct(**change), None), f"{name} must be on a boundary")
+
+
+def test_misaligned_positions_and_starts_are_refused():
+    lib = entry_points()
+    for by in (1, 4):
+        refused(lib.st_cache_attention(cache(), attend_struct(positions=P + by), None), "positions must be on a boundary")
+    for by in (1, 2, 3):
+        refused(lib.st_window_attention(window_struct(starts=P + by), None), "starts must be on a boundary")
+    # frequencies that no pair uses are not read: what is refused here is the gain
+    refused(lib.st_cache_append(cache(), append_struct(rotary=0, frequencies=P + 1, q_gain=P + 4), None), "gains")
