@@ -63,7 +63,7 @@ __device__ int sequence_start(const WindowArgs& a, int row, int* end = nullptr) 
   if (!a.starts) return 0;
   int lo = 0, hi = a.sequences;  // the first sequence that ends behind the row
   while (lo < hi) {
-    const int mid = (lo + hi) / 2;
+    const int mid = lo + (hi - lo) / 2;  // the sum of both passes 2^31 from 2^30 sequences on
     if (a.starts[mid + 1] <= row) lo = mid + 1;
     else hi = mid;
   }
