@@ -87,15 +87,16 @@ int check_aligned(const void* p, const char* name, unsigned bytes) {
 }
 
 DeviceScope::DeviceScope(int device) {
+  const cudaError_t pending = cudaPeekAtLastError();
   int current = 0;
-  if ((status_ = cache_cuda(cudaGetDevice(&current), "cudaGetDevice: ")) != ST_OK) return;
-  if (current != device) {
-    if ((status_ = cache_cuda(cudaSetDevice(device), "cudaSetDevice: ")) != ST_OK) return;
-    previous_ = current;
+  status_ = cache_cuda(cudaGetDevice(&current), "cudaGetDevice: ");
+  if (status_ == ST_OK && pending != cudaSuccess)
+    status_ = cache_fail(ST_ERR_CUDA, cudaGetErrorString(pending), "an earlier CUDA error is pending: ");
+  if (status_ == ST_OK && current != device) {
+    status_ = cache_cuda(cudaSetDevice(device), "cudaSetDevice: ");
+    if (status_ == ST_OK) previous_ = current;
   }
-  const cudaError_t e = cudaPeekAtLastError();
-  if (e != cudaSuccess)
-    status_ = cache_fail(ST_ERR_CUDA, cudaGetErrorString(e), "an earlier CUDA error is pending: ");
+  if (status_ != ST_OK && pending == cudaSuccess) cudaGetLastError();  // reported here, so not left pending
 }
 
 DeviceScope::~DeviceScope() {
@@ -105,7 +106,11 @@ DeviceScope::~DeviceScope() {
 int sm_count(int device) {
   int n = g_sms[device].load(std::memory_order_relaxed);
   if (!n) {
-    if (cudaDeviceGetAttribute(&n, cudaDevAttrMultiProcessorCount, device) != cudaSuccess) return 1;
+    const bool pending = cudaPeekAtLastError() != cudaSuccess;
+    if (cudaDeviceGetAttribute(&n, cudaDevAttrMultiProcessorCount, device) != cudaSuccess) {
+      if (!pending) cudaGetLastError();  // the call that needs the device reports it
+      return 1;
+    }
     g_sms[device].store(n, std::memory_order_relaxed);
   }
   return n;
