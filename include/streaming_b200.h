@@ -314,7 +314,10 @@ typedef struct {
  * may overlap anything read. Positions stay below 2^53, head strides of rows
  * below 2^31 times 16 bytes. Of a stream's new rows only those still in the
  * window, or at a sink position, are inserted. Sums and angles are fp32 or wider;
- * each output is rounded once (4-bit rows are quantised from the fp32 values). */
+ * each output is rounded once (4-bit rows are quantised from the fp32 values).
+ * The mean square is an fp32 number: a normed row's values stay below 2^60, and
+ * where epsilon is below 2^-60 its largest is above 2^-50 (a row of zeros is
+ * 0 / 0 for an epsilon of 0). */
 typedef struct {
   int mode;                 /* st_mode of q, k, v, q_out, k_out: the cache's type, or fp16/bf16 for INT4 */
   int heads;                /* query heads */

@@ -105,7 +105,9 @@ def cache_append(q, k, v, keys, values, positions, frequencies, *, sinks: int = 
     [up to head_dim / 2]); k and v enter the cache. Returns the rotated queries
     (written to ``out`` when given, which may be q), or with ``rotated_keys``
     the pair (queries, keys). Rows of idle streams come back as 0; rows of no
-    stream are left as they were in ``out``, and undefined in a fresh tensor."""
+    stream are left as they were in ``out``, and undefined in a fresh tensor.
+    A row's mean square is an fp32 number: normed values stay below 2 ** 60, and
+    the largest of a row above 2 ** -50 where epsilon is below 2 ** -60."""
     return _native.append(q, k, v, keys, values, positions, frequencies, sinks, starts, q_gain, k_gain, epsilon,
                           key_scales, value_scales, rotated_keys, out)
 

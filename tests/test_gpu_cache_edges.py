@@ -45,3 +45,42 @@ def test_a_call_for_a_device_that_is_not_there_leaves_no_error_behind():
         assert torch.equal(ops.cache_attention(q, *cache[:2], at), want)
     lib.st_cache_attention_workspace(absent, 4, need)
     assert torch.equal(ops.cache_attention(q, *cache[:2], at), want)
+
+
+@pytest.mark.parametrize("mode", ["fp32", "bf16"])
+@pytest.mark.parametrize("dim", [8, 128, 256])
+def test_the_norm_at_the_ends_of_its_range(mode, dim):
+    # the largest and least rows whose mean square is said to be held, without an epsilon and with one
+    g = generator(53)
+    dtype = TYPES[mode]
+    exponents = [-50, -49, -40, -31, -29, 0, 30, 50, 57, 58]
+    n = len(exponents)
+    size = torch.tensor([2.0 ** e for e in exponents], dtype=torch.float64, device="cuda")[:, None, None]
+    x = torch.randn(n, 2, dim, generator=g, device="cuda", dtype=torch.float64).clamp(-3, 3)
+    x[:, :, 0] = 1.5
+    x[:, 1, 1:] *= 2.0 ** -20                    # rows that one column outweighs
+    x = (x * size).to(dtype)
+    gain = 0.5 + torch.rand(dim, generator=g, device="cuda")
+    at = torch.arange(n, device="cuda") * 1000
+    f = ops.rotation_frequencies(dim)
+    for epsilon in (0.0, 2.0 ** -80, 1e-6, 2.0 ** 122):
+        cache = ops.new_cache(n, 2, 4, dim, mode=mode)
+        q, k = ops.cache_append(x, x, x, *cache[:2], at, f, q_gain=gain, k_gain=gain, epsilon=epsilon, rotated_keys=True)
+        want, bound = ref.rotated(x, at, f, gain, torch.tensor(epsilon, dtype=torch.float32).item(), dtype)
+        ref.check(q, want, bound, f"epsilon {epsilon}")
+        assert torch.equal(q, k)
+
+
+def test_the_norm_of_rows_that_are_not_finite_or_zero():
+    x = torch.ones(4, 1, 64, device="cuda")
+    x[0, 0, 5] = float("inf")                    # x / inf: 0, and the infinite column is no number
+    x[1, 0, 7] = float("nan")
+    x[2] = 0
+    gain = torch.ones(64, device="cuda")
+    cache = ops.new_cache(4, 1, 4, 64, mode="fp32")
+    at = torch.zeros(4, dtype=torch.int64, device="cuda")
+    q = ops.cache_append(x, x, x, *cache[:2], at, ops.rotation_frequencies(64)[:0], q_gain=gain, k_gain=gain)
+    assert torch.isnan(q[0, 0, 5]) and int(torch.isnan(q[0]).sum()) == 1 and int((q[0] == 0).sum()) == 63
+    assert torch.isnan(q[1]).all() and not q[2].any() and torch.isfinite(q[3]).all()
+    q = ops.cache_append(x, x, x, *cache[:2], at, ops.rotation_frequencies(64)[:0], q_gain=gain, k_gain=gain, epsilon=0.0)
+    assert torch.isnan(q[2]).all()               # 0 / 0
