@@ -38,7 +38,9 @@
 // within one group of 32 columns, whose scale and lowest value then enter in
 // fp32: sum q k = scale * sum q c + lowest * sum q. For values the scale is
 // folded into the weight before its one rounding, to bf16 (times 2^70: its range
-// takes scales from 2^-56 to 2^56). Codes are 0..15 where the values lie about
+// takes scales from 2^-56 to 2^56). For fp16 rows, which have 3 bits more, the
+// weight is a sum of two bf16, each with a product of its own (fp16 itself has no
+// room for the scales; 256 Large streams, 516 slots: 55 us, at bf16 48). Codes are 0..15 where the values lie about
 // 0, so that rounding would count double; the fp32 sum beside the product takes
 // p * (lowest + 7.5 scale) - 7.5 * (the rounded weight), which leaves the error
 // with the code's distance from 7.5. Turning codes into 16-bit values first took
@@ -180,6 +182,7 @@ __global__ void __launch_bounds__(kAttendThreads, DB * NT == 1 ? (INT4 ? 7 : 6) 
   constexpr int X = ONE ? 1 : 2;  // query heads a lane has of each block: 8 n + 2 t + x
   using PT = typename std::conditional<INT4, __nv_bfloat16, T>::type;  // operands of the second product
   constexpr float kLift = std::is_same<PT, __half>::value ? 10.f : 0.f;
+  constexpr bool kTwo = INT4 && std::is_same<T, __half>::value;  // 4-bit: a weight is two bf16
   extern __shared__ uint4 dynamic[];
   float(*sh_o)[NT * 8][Smem::kPartRow] = reinterpret_cast<float(*)[NT * 8][Smem::kPartRow]>(dynamic);
   __shared__ float sh_m[kAttendWarps][NT * 8], sh_l[kAttendWarps][NT * 8];
@@ -421,7 +424,7 @@ __global__ void __launch_bounds__(kAttendThreads, DB * NT == 1 ? (INT4 ? 7 : 6) 
     if constexpr (!INT4)
       if (next < last) fetch_k(next);
 
-    unsigned pf[TS][NT][SW][2];
+    unsigned pf[TS][NT][SW][kTwo ? 4 : 2];
 #pragma unroll
     for (int n = 0; n < NT; ++n) {
       float p[TS][2][X], top[X];
@@ -477,9 +480,16 @@ __global__ void __launch_bounds__(kAttendThreads, DB * NT == 1 ? (INT4 ? 7 : 6) 
               const unsigned w = pack2((PT*)nullptr, p[u][r][0] * (scale * kValueLift),
                                        ONE ? 0.f : p[u][r][X - 1] * (scale * kValueLift));
               pf[u][n][j][r] = transpose8x8(w);
+              unsigned rest = 0;
+              if constexpr (kTwo) {
+                rest = pack2((PT*)nullptr, fmaf(p[u][r][0], scale * kValueLift, -group_scale(w)),
+                             ONE ? 0.f : fmaf(p[u][r][X - 1], scale * kValueLift, -group_lowest(w)));
+                pf[u][n][j][2 + r] = transpose8x8(rest);
+              }
 #pragma unroll
               for (int x = 0; x < X; ++x) {
-                const float rounded = x ? group_lowest(w) : group_scale(w);  // the halves of a word of two bf16
+                float rounded = x ? group_lowest(w) : group_scale(w);  // the halves of a word of two bf16
+                if constexpr (kTwo) rounded += x ? group_lowest(rest) : group_scale(rest);
                 olow[n][j][x] = fmaf(p[u][r][x], middle, fmaf(rounded, -7.5f / kValueLift, olow[n][j][x]));
               }
             }
@@ -506,9 +516,13 @@ __global__ void __launch_bounds__(kAttendThreads, DB * NT == 1 ? (INT4 ? 7 : 6) 
 #pragma unroll
           for (int n = 0; n < NT; ++n)
 #pragma unroll
-            for (int w = 0; w < 2; ++w)
+            for (int w = 0; w < 2; ++w) {
               mma<PT>(o[n][j / 2][2 * (j & 1) + w], c0[2 * w], c0[2 * w + 1], c1[2 * w], c1[2 * w + 1], pf[u][n][j][0],
                       pf[u][n][j][1]);
+              if constexpr (kTwo)
+                mma<PT>(o[n][j / 2][2 * (j & 1) + w], c0[2 * w], c0[2 * w + 1], c1[2 * w], c1[2 * w + 1], pf[u][n][j][2],
+                        pf[u][n][j][3]);
+            }
         }
       } else {
 #pragma unroll

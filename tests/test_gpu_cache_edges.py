@@ -84,3 +84,34 @@ def test_the_norm_of_rows_that_are_not_finite_or_zero():
     assert torch.isnan(q[1]).all() and not q[2].any() and torch.isfinite(q[3]).all()
     q = ops.cache_append(x, x, x, *cache[:2], at, ops.rotation_frequencies(64)[:0], q_gain=gain, k_gain=gain, epsilon=0.0)
     assert torch.isnan(q[2]).all()               # 0 / 0
+
+
+@pytest.mark.parametrize("heads,kv,dim", [(2, 2, 64), (4, 1, 64), (16, 1, 64), (1, 1, 96), (4, 2, 128), (16, 1, 128), (2, 1, 32),
+                                          (1, 1, 256), (3, 1, 160)])
+def test_weights_of_fp16_rows_over_four_bits_keep_the_precision_of_fp16(heads, kv, dim):
+    # Values of opposite sign at the ends of a group nearly cancel, so that what a weight loses shows. Keys are constant
+    # rows (scale 0) and queries sum to about 1, so logits are small and exact. The bound is that of the reference with
+    # a weight's rounding at 2^-16, two bf16 numbers (2^-8 twice), in place of one.
+    g = generator(54)
+    streams, slots = 40, 5
+    k_scales, v_scales = (torch.zeros(streams, kv, slots, dim // 32, 2, dtype=torch.bfloat16, device="cuda") for _ in range(2))
+    k_scales[..., 1] = normal(g, streams, kv, slots, 1, dtype=torch.bfloat16)
+    v_scales[..., 0] = 0.1328125
+    v_scales[..., 1] = -7.5 * 0.1328125
+    codes = (torch.arange(slots, device="cuda")[:, None] + torch.arange(dim, device="cuda") // 3) % 2 * 15
+    v = ref.pack(codes.to(torch.uint8)).expand(streams, kv, -1, -1).contiguous()
+    k = torch.zeros_like(v)
+    q = (1 + 0.5 * normal(g, streams, heads, dim)).mul(2 / dim).to(torch.float16)
+    at = torch.arange(streams, device="cuda") % slots
+    got = ops.cache_attention(q, k, v, at, key_scales=k_scales, value_scales=v_scales, scale=1.0)
+    group, u = heads // kv, ref.unit(torch.float16)
+    see = torch.arange(slots, device="cuda") <= at[:, None]
+    for s in range(streams):
+        qs = q[s].double().unflatten(0, (kv, group))
+        ks, vs = ref.unpack(k[s], k_scales[s]), ref.unpack(v[s], v_scales[s])
+        sizes = [(15 * x[s, ..., 0].double() + x[s, ..., 1].double().abs()).repeat_interleave(32, -1) for x in (k_scales, v_scales)]
+        mask = see[s].expand(kv, group, -1)
+        want, bound = ref.attention(qs, ks, vs, mask, 1.0, torch.float16, sizes)
+        size, _ = ref.attention(qs, ks, sizes[1], mask, 1.0, torch.float16, sizes)
+        bound = bound - (1 + u) * (ref.unit(torch.bfloat16) - 2.0 ** -16) * size
+        ref.check(got[s].unflatten(0, (kv, group)), want, bound, f"stream {s}")
