@@ -17,13 +17,15 @@ A stream that starts with a backlog runs ``cache_append`` and
 ``window_attention`` over all its events at once, then ``cache_append`` and
 ``cache_attention`` for each further one:
 
-    cache = new_cache(streams, heads, window, head_dim, sinks=4, mode="bf16")
+    keys, values, _, _ = new_cache(streams, kv_heads, window, head_dim, sinks=4, mode="bf16")
     f = rotation_frequencies(head_dim)
-    q, k = cache_append(q, k, v, *cache[:2], positions, f, sinks=4, starts=starts, rotated_keys=True)
+    q, k = cache_append(q, k, v, keys, values, positions, f, sinks=4, starts=starts, rotated_keys=True)
     out = window_attention(q, k, v, window=window, sinks=4, starts=starts)
-    ...
-    q = cache_append(q, k, v, *cache[:2], positions, f, sinks=4)
-    out = cache_attention(q, *cache[:2], positions)
+    positions += torch.where(positions >= 0, starts.diff(), 0)  # the next event's; a stream at a negative one is idle
+    # then, for each further event of every stream
+    q = cache_append(q, k, v, keys, values, positions, f, sinks=4)
+    out = cache_attention(q, keys, values, positions)
+    positions += positions >= 0
 
 Work is queued on the current stream of the tensors' device, which may be
 another device than the current one; nothing waits. Positions and starts are

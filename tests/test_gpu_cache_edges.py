@@ -1,7 +1,9 @@
 """Calls of the window-cache operators at the edges of what their documentation
 allows, against their definitions in 64 bits (tests/cache_reference.py)."""
 import ctypes
-import itertools
+import re
+import textwrap
+from pathlib import Path
 
 import pytest
 import torch
@@ -115,3 +117,45 @@ def test_weights_of_fp16_rows_over_four_bits_keep_the_precision_of_fp16(heads, k
         size, _ = ref.attention(qs, ks, sizes[1], mask, 1.0, torch.float16, sizes)
         bound = bound - (1 + u) * (ref.unit(torch.bfloat16) - 2.0 ** -16) * size
         ref.check(got[s].unflatten(0, (kv, group)), want, bound, f"stream {s}")
+
+
+def recipe(where):
+    """The documented calls: (for the backlogs, for each further event)."""
+    text = ops.__doc__ if where == "module" else (Path(__file__).parents[1] / where).read_text()
+    block = re.search(r"^ *keys, values.*= new_cache\(.*?(?=^ *```|^ *$)", text, re.M | re.S)[0]
+    backlogs, events = re.split(r"^# then.*\n", textwrap.dedent(block), flags=re.M)
+    return backlogs, events
+
+
+@pytest.mark.parametrize("where", ["module", "INTEGRATION.md"])
+def test_the_documented_calls_give_the_attention_of_each_streams_history(where):
+    # two streams with backlogs, one without, and one that stays idle
+    g = generator(55)
+    heads, kv, dim, window, sizes, more = 4, 2, 64, 24, [60, 0, 10, 0], 20
+    backlogs, events = recipe(where)
+    total = [n + more for n in sizes]
+    history = [[normal(g, n, h, dim, dtype=torch.bfloat16) for h in (heads, kv, kv)] for n in total]
+    gains = [0.5 + torch.rand(dim, generator=g, device="cuda") for _ in range(2)] if "gq" in events else [None, None]
+    names = dict(vars(ops), streams=4, kv_heads=kv, window=window, head_dim=dim, starts=starts_of(sizes), gq=gains[0], gk=gains[1],
+                 positions=torch.tensor([0, 0, 0, -1], device="cuda"))
+    names.update(zip("qkv", (torch.cat([h[i][:n] for h, n in zip(history, sizes)]) for i in range(3))))
+    exec(backlogs, names)
+    got = [[names["out"][a:b]] for a, b in zip(names["starts"].tolist(), names["starts"].tolist()[1:])]
+    for t in range(more):
+        names.update(zip("qkv", (torch.stack([h[i][n + t] for h, n in zip(history, sizes)]) for i in range(3))))
+        exec(events, names)
+        for s in range(4):
+            got[s].append(names["out"][s:s + 1])
+    assert names["positions"].tolist() == [80, 20, 30, -1]
+    assert not torch.cat(got[3]).any()
+    for s in range(3):
+        at = torch.arange(total[s], device="cuda")
+        q, k = (ref.rotated(history[s][i], at, names["f"], gains[i], 1e-6, torch.bfloat16)[0] for i in range(2))
+        for _, _, want, bound in window_reference(q, k, history[s][2], [0, total[s]], window, 4, dim ** -0.5, torch.bfloat16):
+            # the operators see q and k rounded to the type: a logit moves by at most 2 u(T) sum|q k| scale, and a
+            # weight by twice that, relative
+            products = (q.abs().sum(-1).amax() * k.abs().amax()).item() * dim ** -0.5
+            extra = 2 * 2 * 2 * (ref.unit(torch.bfloat16) + 24 * ref.F) * products * history[s][2].double().abs().amax()
+            ref.check(torch.cat(got[s]), want, bound + extra, f"stream {s}")
+            # and, as that bound is far from what happens: a norm that a wrong slot or angle would leave
+            assert (torch.cat(got[s]).double() - want).norm() < 0.02 * want.norm()
