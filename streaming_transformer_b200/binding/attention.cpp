@@ -193,11 +193,16 @@ double number(PyObject* o, const char* name) {
   }
   return v;
 }
-// An integer; one past 64 bits becomes the nearest that fits.
+// An integer of any type that is one (numpy's among them); one past 64 bits becomes the nearest that fits.
 int64_t integer(PyObject* o, const char* name) {
+  PyObject* index = PyNumber_Index(o);
+  if (!index) {
+    PyErr_Clear();
+    refuse(std::string(name) + ": expected an integer");
+  }
   int over = 0;
-  const long long v = PyLong_Check(o) ? PyLong_AsLongLongAndOverflow(o, &over) : -1;
-  if (!PyLong_Check(o)) refuse(std::string(name) + ": expected an integer");
+  const long long v = PyLong_AsLongLongAndOverflow(index, &over);
+  Py_DECREF(index);
   return over > 0 ? INT64_MAX : over < 0 ? INT64_MIN : v;
 }
 

@@ -84,3 +84,22 @@ def test_misaligned_positions_and_starts_are_refused():
         refused(lib.st_window_attention(window_struct(starts=P + by), None), "starts must be on a boundary")
     # frequencies that no pair uses are not read: what is refused here is the gain
     refused(lib.st_cache_append(cache(), append_struct(rotary=0, frequencies=P + 1, q_gain=P + 4), None), "gains")
+
+
+def test_sinks_of_any_integer_type():
+    import numpy as np
+    t = append_arguments(False)
+    positions = torch.zeros(1, dtype=torch.int64)
+
+    def call(sinks):
+        return ops.cache_append(t["q"], t["k"], t["v"], t["keys"], t["values"], positions, t["frequencies"], sinks=sinks)
+
+    for sinks in (2, np.int64(2), np.int32(0), torch.tensor(1)):
+        with pytest.raises(StreamError, match="expected a CUDA tensor"):     # past the integers' check
+            call(sinks)
+    for sinks in (1.0, np.float32(1), "1", None, torch.tensor(1.0)):
+        with pytest.raises(StreamError, match="sinks: expected an integer"):
+            call(sinks)
+    for sinks in (-1, 2 ** 70, np.int64(-3)):
+        with pytest.raises(StreamError, match="sinks.*out of range"):
+            call(sinks)

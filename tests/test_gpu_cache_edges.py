@@ -159,3 +159,12 @@ def test_the_documented_calls_give_the_attention_of_each_streams_history(where):
             ref.check(torch.cat(got[s]), want, bound + extra, f"stream {s}")
             # and, as that bound is far from what happens: a norm that a wrong slot or angle would leave
             assert (torch.cat(got[s]).double() - want).norm() < 0.02 * want.norm()
+
+
+def test_window_and_sinks_of_any_integer_type():
+    import numpy as np
+    q = normal(generator(56), 40, 2, 64, dtype=torch.bfloat16)
+    want = ops.window_attention(q, q, q, window=9, sinks=2)
+    assert torch.equal(ops.window_attention(q, q, q, window=np.int64(9), sinks=np.int32(2)), want)
+    with pytest.raises(StreamError, match="window: expected an integer"):
+        ops.window_attention(q, q, q, window=9.0)
