@@ -364,7 +364,8 @@ int st_cache_unpack(const st_cache* cache, int mode, void* keys, void* values, v
  * sequence, all rows). Rows outside every sequence are not read into any
  * result and their outputs are left as they were. A value that is not finite
  * reaches the rows that see it and no other; such tiles are done twice, the
- * second time slowly. out may not overlap q, k or v. */
+ * second time slowly. out may not overlap q, k or v; strides of 16-bit inputs
+ * are below 2^40 bytes. */
 typedef struct {
   int device;
   int mode;                 /* st_mode of q, k, v and out */

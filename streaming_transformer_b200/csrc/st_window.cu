@@ -941,9 +941,11 @@ EncodeTiled encode_tiled() {
   if (!f) {
     void* p = nullptr;
     cudaDriverEntryPointQueryResult found{};
-    if (cudaGetDriverEntryPointByVersion("cuTensorMapEncodeTiled", &p, 12000, cudaEnableDefault, &found) != cudaSuccess ||
-        found != cudaDriverEntryPointSuccess)
+    if (cudaGetDriverEntryPointByVersion("cuTensorMapEncodeTiled", &p, 12000, cudaEnableDefault, &found) != cudaSuccess) {
+      cudaGetLastError();  // the caller reports it
       return nullptr;
+    }
+    if (found != cudaDriverEntryPointSuccess) return nullptr;
     f = reinterpret_cast<EncodeTiled>(p);
     fn.store(f, std::memory_order_release);
   }
@@ -951,10 +953,11 @@ EncodeTiled encode_tiled() {
 }
 
 // [rows][heads][head_dim] as a tensor whose boxes are 64 columns of `box_rows` rows of one head. Columns past
-// head_dim and rows past `rows` read as zeros. A stride along a dimension of one element, or of 0, is never used.
+// head_dim and rows past `rows` read as zeros. A stride of 0 repeats its row or head; along a dimension of one element
+// it is never used, whatever it is.
 bool encode_rows(CUtensorMap* map, const st_rows& r, int mode, long long rows, int heads, int head_dim, int box_rows) {
   const cuuint64_t dims[3] = {(cuuint64_t)head_dim, (cuuint64_t)heads, (cuuint64_t)rows};
-  const cuuint64_t strides[2] = {(cuuint64_t)r.head_stride * 2, (cuuint64_t)r.row_stride * 2};
+  const cuuint64_t strides[2] = {(cuuint64_t)(heads > 1 ? r.head_stride : head_dim) * 2, (cuuint64_t)r.row_stride * 2};
   const cuuint32_t box[3] = {64, 1, (cuuint32_t)box_rows}, step[3] = {1, 1, 1};
   const EncodeTiled encode = encode_tiled();
   return encode && encode(map, mode == ST_MODE_FP16 ? CU_TENSOR_MAP_DATA_TYPE_FLOAT16 : CU_TENSOR_MAP_DATA_TYPE_BFLOAT16, 3,
@@ -1031,6 +1034,12 @@ extern "C" int st_window_attention(const st_window* p, void* stream) {
       (rc = check_rows(p->out, "out", p->mode, p->rows, p->heads, p->head_dim, true)) != ST_OK)
     return rc;
   if ((rc = check_aligned(p->starts, "starts", 4)) != ST_OK) return rc;
+  const struct { const st_rows* rows; int heads; const char* name; } inputs[] = {
+      {&p->q, p->heads, "q"}, {&p->k, p->kv_heads, "k"}, {&p->v, p->kv_heads, "v"}};
+  for (const auto& x : inputs)  // what a tensor map takes
+    if (p->mode != ST_MODE_FP32 && ((p->rows > 1 && x.rows->row_stride >= (int64_t)1 << 39) ||
+                                    (x.heads > 1 && x.rows->head_stride >= (int64_t)1 << 39)))
+      return cache_fail(ST_ERR_INVALID, ": strides of 16-bit rows are below 2^40 bytes", x.name);
   if (p->out.data == p->q.data || p->out.data == p->k.data || p->out.data == p->v.data)
     return cache_fail(ST_ERR_INVALID, "out may not be an input");
   DeviceScope scope(p->device);
@@ -1057,11 +1066,11 @@ extern "C" int st_window_attention(const st_window* p, void* stream) {
   }
   TileMaps maps;
   const long long ctas = (p->rows + kTileRows - 1) / kTileRows * p->heads;
-  const bool tiles = !few && p->mode != ST_MODE_FP32 && p->scale > 0.f && ctas <= INT32_MAX &&
-                     encode_rows(&maps.q, p->q, p->mode, p->rows, p->heads, p->head_dim, kTileRows) &&
-                     encode_rows(&maps.k, p->k, p->mode, p->rows, p->kv_heads, p->head_dim, kBlockRows) &&
-                     encode_rows(&maps.v, p->v, p->mode, p->rows, p->kv_heads, p->head_dim, kBlockRows);
-  if (tiles) {
+  if (!few && p->mode != ST_MODE_FP32 && p->scale > 0.f && ctas <= INT32_MAX) {
+    if (!encode_rows(&maps.q, p->q, p->mode, p->rows, p->heads, p->head_dim, kTileRows) ||
+        !encode_rows(&maps.k, p->k, p->mode, p->rows, p->kv_heads, p->head_dim, kBlockRows) ||
+        !encode_rows(&maps.v, p->v, p->mode, p->rows, p->kv_heads, p->head_dim, kBlockRows))
+      return cache_fail(ST_ERR_CUDA, "window attention: the driver takes no tensor map of the rows");
     const cudaError_t e = p->mode == ST_MODE_FP16 ? launch_tiles<__half>(a, maps, s) : launch_tiles<__nv_bfloat16>(a, maps, s);
     if (e != cudaSuccess) {
       cudaGetLastError();  // reported here, so not left pending

@@ -4,7 +4,7 @@ import pytest
 
 torch = pytest.importorskip("torch")
 
-from test_cache_cpu import FOUR, P, append as append_struct, attend as attend_struct, cache, entry_points, refused, window as window_struct
+from test_cache_cpu import FOUR, P, Rows, append as append_struct, attend as attend_struct, cache, entry_points, refused, rows, window as window_struct
 
 from streaming_transformer_b200 import StreamError
 from streaming_transformer_b200 import attention as ops
@@ -103,3 +103,14 @@ def test_sinks_of_any_integer_type():
     for sinks in (-1, 2 ** 70, np.int64(-3)):
         with pytest.raises(StreamError, match="sinks.*out of range"):
             call(sinks)
+
+
+@pytest.mark.parametrize("name", ["q", "k", "v"])
+@pytest.mark.parametrize("mode", [1, 2])
+def test_strides_that_no_tensor_map_takes_are_refused(name, mode):
+    heads = 4 if name == "q" else 2
+    for strides in ((2 ** 39, 64), (heads * 64, 2 ** 39)):
+        refused(entry_points().st_window_attention(window_struct(mode=mode, **{name: Rows(P, *strides)}), None), f"{name}: strides of 16-bit")
+    # along a dimension of one element a stride is never used: what is refused here is the next input
+    one = window_struct(mode=mode, heads=1, kv_heads=1, q=Rows(P, 64, 2 ** 40), k=rows(1), v=Rows(P, 2 ** 39, 64))
+    refused(entry_points().st_window_attention(one, None), "v: strides of 16-bit")

@@ -168,3 +168,40 @@ def test_window_and_sinks_of_any_integer_type():
     assert torch.equal(ops.window_attention(q, q, q, window=np.int64(9), sinks=np.int32(2)), want)
     with pytest.raises(StreamError, match="window: expected an integer"):
         ops.window_attention(q, q, q, window=9.0)
+
+
+@pytest.mark.parametrize("mode", ["mixed", "bf16"])
+def test_a_stride_of_a_single_head_is_never_used(mode):
+    # whatever it is, the call takes the way of its size, which the bits tell
+    g, lib = generator(57), c_calls.entry_points()
+    q, k, v = (normal(g, 200, 1, 64, dtype=TYPES[mode]) for _ in range(3))
+    want = ops.window_attention(q, k, v, window=50, scale=0.125)
+    for stride in (0, 64, 2 ** 40):
+        out = torch.empty_like(q)
+        a = c_calls.window(mode=1 if mode == "mixed" else 2, heads=1, kv_heads=1, rows=200, window=50, sinks=0, device=torch.cuda.current_device(),
+                           q=c_calls.Rows(q.data_ptr(), 64, stride), k=c_calls.Rows(k.data_ptr(), 64, stride),
+                           v=c_calls.Rows(v.data_ptr(), 64, stride), out=c_calls.Rows(out.data_ptr(), 64, 64))
+        assert lib.st_window_attention(a, torch.cuda.current_stream().cuda_stream) == 0
+        assert torch.equal(out, want), f"head stride {stride}"
+
+
+@pytest.mark.parametrize("mode", ["fp32", "mixed", "bf16"])
+@pytest.mark.parametrize("dim", [64, 72, 128, 200])
+def test_strides_of_every_order_take_the_way_of_their_size(mode, dim):
+    # heads outermost, rows with a tail, rows whose stride is no multiple of the heads', rows and heads that overlap or
+    # repeat: the same bits as of a copy in the usual order
+    g = generator(58)
+    n, heads, kv = 150, 4, 2
+    q, out = normal(g, n, heads, dim, dtype=TYPES[mode]), torch.empty(n, heads, dim, dtype=TYPES[mode], device="cuda")
+    pool = normal(g, 400000, dtype=TYPES[mode])
+    for strides in ((dim, n * dim), (kv * dim + 8, dim), (dim + 8, n * (dim + 8) + 16), (8, 16), (16, 8), (0, dim), (dim, 0), (0, 0),
+                    (kv * (dim + 8), dim + 8)):
+        k, v = (pool[8 * i:].as_strided((n, kv, dim), (*strides, 1)) for i in range(2))
+        got = ops.window_attention(q, k, v, window=40, sinks=2)
+        assert torch.equal(got, ops.window_attention(q, k.contiguous(), v.contiguous(), window=40, sinks=2)), strides
+    for strides in ((dim, n * dim), (heads * dim + 8, dim), (heads * (dim + 8), dim + 8)):
+        wide = torch.full((400000,), 7.0, dtype=TYPES[mode], device="cuda")
+        qs, to = pool.as_strided((n, heads, dim), (*strides, 1)), wide.as_strided((n, heads, dim), (*strides, 1))
+        ops.window_attention(qs, q[:, :kv], q[:, kv:], window=40, sinks=2, out=to)
+        assert torch.equal(to, ops.window_attention(qs.contiguous(), q[:, :kv], q[:, kv:], window=40, sinks=2, out=out)), strides
+        assert int((wide != 7).sum()) == int((to != 7).sum())
