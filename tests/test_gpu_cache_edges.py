@@ -11,7 +11,7 @@ import torch
 import cache_reference as ref
 from streaming_transformer_b200.runtime import StreamError
 import test_cache_cpu as c_calls
-from test_gpu_cache import TYPES, filled_cache, generator, normal, scales_of, starts_of, window_reference
+from test_gpu_cache import TYPES, attend_reference, filled_cache, generator, normal, scales_of, starts_of, window_reference
 
 pytestmark = pytest.mark.gpu
 
@@ -205,3 +205,84 @@ def test_strides_of_every_order_take_the_way_of_their_size(mode, dim):
         ops.window_attention(qs, q[:, :kv], q[:, kv:], window=40, sinks=2, out=to)
         assert torch.equal(to, ops.window_attention(qs.contiguous(), q[:, :kv], q[:, kv:], window=40, sinks=2, out=out)), strides
         assert int((wide != 7).sum()) == int((to != 7).sum())
+
+
+@pytest.mark.parametrize("outside", [1e4, float("nan")])
+@pytest.mark.parametrize("mode", ["fp32", "mixed", "bf16"])
+@pytest.mark.parametrize("dim", [8, 16, 24, 32, 40, 64, 72, 80, 96, 120, 128, 136, 160, 192, 200, 248, 256])
+def test_what_rows_of_no_sequence_hold_does_not_count(dim, mode, outside):
+    # Large finite values reach the results of the tiles if a mask misses them; values that are not finite make the tiles
+    # be done again row by row, so that each way is compared by itself.
+    g = generator(59)
+    dtype = TYPES[mode]
+    for heads, kv, window, sinks, sizes in ((2, 1, 50, 3, [130, 1, 61]), (3, 3, 200, 0, [7, 161]), (1, 1, 33, 40, [97, 33])):
+        before, n = 5, 5 + sum(sizes) + 40
+        q, k, v = (normal(g, n, h, dim, dtype=dtype) for h in (heads, kv, kv))
+        for x in (q, k, v):
+            x[:before] = outside
+            x[before + sum(sizes):] = outside
+            x[before + sum(sizes)::2] *= -1
+        starts = starts_of(sizes, before)
+        got = torch.full((n, heads, dim), 7.0, dtype=dtype, device="cuda")
+        ops.window_attention(q, k, v, window=window, sinks=sinks, starts=starts, out=got)
+        for a, b, want, bound in window_reference(q, k, v, starts.tolist(), window, sinks, dim ** -0.5, dtype):
+            ref.check(got[a:b], want, bound, f"{heads} heads, rows {a}..{b}")
+        assert (got[:before] == 7).all() and (got[before + sum(sizes):] == 7).all()
+
+
+@pytest.mark.parametrize("mode", ["fp32", "mixed", "bf16", "int4"])
+@pytest.mark.parametrize("dim", [32, 64, 96, 128, 256])
+def test_large_values_in_unseen_slots_do_not_count(mode, dim):
+    # unlike NaN, which would show at once, they would only shift a result
+    g = generator(60)
+    dtype = TYPES.get(mode, torch.bfloat16)
+    at = [0, 14, 31, 32, 77, 128]
+    cache, held = filled_cache(g, len(at), 2, 140, dim, 0, mode)
+    for s, p in enumerate(at):
+        for t in cache[2:] if mode == "int4" else cache[:2]:
+            t[s, :, p + 1:] = 1e4
+    for heads in (2, 6, 24):
+        q = normal(g, len(at), heads, dim, dtype=dtype)
+        got = ops.cache_attention(q, *cache[:2], torch.tensor(at, device="cuda"), **scales_of(cache))
+        want, bound = attend_reference(q, held, at, dim ** -0.5, dtype)
+        ref.check(got, want, bound, f"{heads} heads")
+
+
+@pytest.mark.parametrize("mode", ["fp32", "mixed", "bf16", "int4"])
+def test_a_second_backlog_enters_a_full_cache(mode):
+    # two appends of many rows, then single events: every slot holds the newest position that belongs there
+    g = generator(61)
+    dtype, kind = TYPES.get(mode, torch.bfloat16), mode
+    heads, kv, dim, window, sinks = 4, 2, 64, 19, 3
+    cache = ops.new_cache(3, kv, window, dim, sinks=sinks, mode=kind)
+    f = ops.rotation_frequencies(dim)
+    positions = torch.zeros(3, dtype=torch.int64, device="cuda")
+    keys, values = ([[] for _ in range(3)] for _ in range(2))
+    for sizes in ([30, 1, 20], [5, 44, 0], [1, 1, 1], [25, 2, 19], [1, 1, 1]):
+        starts = starts_of(sizes)
+        q, k, v = (normal(g, sum(sizes), h, dim, dtype=dtype) for h in (heads, kv, kv))
+        q, k = ops.cache_append(q, k, v, *cache[:2], positions, f, sinks=sinks, starts=starts, rotated_keys=True, **scales_of(cache))
+        for s, (a, b) in enumerate(zip(starts.tolist(), starts.tolist()[1:])):
+            keys[s] += k[a:b]
+            values[s] += v[a:b]
+        positions += starts.diff()
+        if sizes == [1, 1, 1]:
+            held = [torch.zeros(3, kv, sinks + window, dim, dtype=dtype, device="cuda") for _ in range(2)]
+            for s in range(3):
+                for t in range(len(keys[s])):
+                    if t < sinks or t >= len(keys[s]) - window:
+                        slot = t if t < sinks else sinks + (t - sinks) % window
+                        held[0][s, :, slot], held[1][s, :, slot] = keys[s][t], values[s][t]
+            at = positions - 1
+            if mode == "int4":
+                stands = [ref.unpack(cache[i], cache[2 + i]) for i in range(2)]
+                for x, h in zip(stands, held):    # the right rows: half a step of at most 10 / 15, and roundings to bf16
+                    assert (x - h.double()).abs().amax() < 0.75
+                sizes4 = [(15 * t[..., 0].double() + t[..., 1].double().abs()).repeat_interleave(32, -1) for t in cache[2:]]
+                held = (*stands, *sizes4)
+            else:
+                assert torch.equal(cache[0], held[0]) and torch.equal(cache[1], held[1])
+                held = [h.double() for h in held]
+            got = ops.cache_attention(q, *cache[:2], at, **scales_of(cache))
+            want, bound = attend_reference(q, held, at.tolist(), dim ** -0.5, dtype)
+            ref.check(got, want, bound)
