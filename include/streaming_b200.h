@@ -269,7 +269,8 @@ const char* st_attention_static_error(void);
  * bf16((max - min) * (1/15)) and code = rint((x - lowest) / scale) clamped to
  * 0..15 (0 where the scale is 0). A group with a non-finite value, or whose
  * max - min or bf16(min) is not finite, reads back as NaN. Attention takes
- * value scales from 2^-56 to 2^56 (or 0) and queries below 2^120.
+ * value scales from 2^-56 to 2^56 (or 0) and queries below 2^120; past them a
+ * result can be infinite or NaN, or below 2^-56 lose digits.
  *
  * All pointers are device memory of `device`, rows, scales and gains start on
  * 16-byte boundaries, positions, starts and frequencies on those of their
@@ -337,7 +338,9 @@ int st_cache_append(const st_cache* cache, const st_append* args, void* stream);
 /* One query row per stream over its cache: out = softmax(scale q K^T) V over
  * the slots 0 .. min(position + 1, sinks + window) - 1 of key head
  * h / (heads / cache heads), position being that of the newest inserted row.
- * Slots past those are not looked at, whatever they hold. A negative position
+ * Slots past those are not looked at, whatever they hold. The sum is fp32
+ * before its quotient, so seen values stay below 2^127 / slots, here and in
+ * st_window_attention. A negative position
  * gives a row of zeros. out may be q itself.
  * `workspace` holds the partial results of a split over the slots:
  * st_cache_attention_workspace() bytes (0 for some shapes; then NULL will do),
@@ -363,8 +366,8 @@ int st_cache_unpack(const st_cache* cache, int mode, void* keys, void* values, v
  * Sequence s is rows starts[s] .. starts[s + 1] - 1 (starts NULL: one
  * sequence, all rows). Rows outside every sequence are not read into any
  * result and their outputs are left as they were. A value that is not finite
- * reaches the rows that see it and no other; such tiles are done twice, the
- * second time slowly. out may not overlap q, k or v; strides of 16-bit inputs
+ * reaches the rows that see it and no other; tiles that load one are done twice,
+ * the second time slowly and with weights in fp32. out may not overlap q, k or v; strides of 16-bit inputs
  * are below 2^40 bytes. */
 typedef struct {
   int device;

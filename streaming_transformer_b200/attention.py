@@ -121,7 +121,9 @@ def cache_attention(q, keys, values, positions, *, key_scales=None, value_scales
     q [streams, heads, head_dim], heads a multiple of the cache's;
     ``positions`` int64 [streams], the position of each stream's newest inserted
     row (negative: a row of zeros). Every slot up to min(position + 1, slots)
-    is seen. ``scale`` defaults to head_dim ** -0.5; ``out`` may be q."""
+    is seen. ``scale`` defaults to head_dim ** -0.5; ``out`` may be q. Over a
+    4-bit cache, value scales are 0 or 2 ** -56 to 2 ** 56 and queries below
+    2 ** 120; seen values of any cache stay below 2 ** 127 / slots."""
     return _native.attend(q, keys, values, positions, key_scales, value_scales, scale, out)
 
 

@@ -286,3 +286,39 @@ def test_a_second_backlog_enters_a_full_cache(mode):
             got = ops.cache_attention(q, *cache[:2], at, **scales_of(cache))
             want, bound = attend_reference(q, held, at.tolist(), dim ** -0.5, dtype)
             ref.check(got, want, bound)
+
+
+@pytest.mark.parametrize("q_size,k_size,v_scale", [(2.0 ** 119, 2.0 ** -118, 1.0), (1.0, 1.0, 2.0 ** 56), (1.0, 1.0, 2.0 ** -56),
+                                                   (2.0 ** -100, 2.0 ** 100, 2.0 ** -20)])
+@pytest.mark.parametrize("dim,heads", [(64, 2), (64, 8), (96, 2), (128, 8), (256, 4)])
+def test_four_bit_attention_at_the_ends_of_its_range(dim, heads, q_size, k_size, v_scale):
+    g = generator(62)
+    codes, s, low = ref.quantise(normal(g, 2, 2, 90, dim) * k_size)
+    k, ks = ref.pack(codes), torch.stack([s, low], -1)
+    v = ref.pack(torch.randint(0, 16, (2, 2, 90, dim), generator=g, device="cuda").to(torch.uint8))
+    vs = torch.tensor([v_scale, -7.5 * v_scale], dtype=torch.bfloat16, device="cuda").expand(2, 2, 90, dim // 32, 2).contiguous()
+    held = [ref.unpack(k, ks), ref.unpack(v, vs)] + [(15 * x[..., 0].double() + x[..., 1].double().abs()).repeat_interleave(32, -1) for x in (ks, vs)]
+    q = normal(g, 2, heads, dim).clamp(-1.9, 1.9).mul(q_size).to(torch.bfloat16)
+    at = [89, 40]
+    got = ops.cache_attention(q, k, v, torch.tensor(at, device="cuda"), key_scales=ks, value_scales=vs)
+    want, bound = attend_reference(q, held, at, dim ** -0.5, torch.bfloat16)
+    ref.check(got, want, bound)
+    assert (got.double() - want).norm() < 0.01 * want.norm()
+
+
+@pytest.mark.parametrize("mode", ["fp32", "bf16"])
+def test_attention_of_the_largest_values(mode):
+    # every value next to 2^127 / slots: the sum stays a number
+    g = generator(63)
+    slots, dtype = 128, TYPES[mode]
+    size = 2.0 ** 127 / slots * 0.99
+    q, k = normal(g, 1, 4, 64, dtype=dtype), normal(g, 1, 2, slots, 64, dtype=dtype)
+    v = torch.full((1, 2, slots, 64), size, device="cuda").to(dtype)
+    got = ops.cache_attention(q, k, v, torch.tensor([slots - 1], device="cuda"))
+    want, bound = attend_reference(q, (k.double(), v.double()), [slots - 1], 0.125, dtype)
+    ref.check(got, want, bound)
+    q, k = normal(g, slots, 4, 64, dtype=dtype), normal(g, slots, 2, 64, dtype=dtype)
+    v = torch.full((slots, 2, 64), size, device="cuda").to(dtype)
+    got = ops.window_attention(q, k, v, window=slots)
+    for _, _, want, bound in window_reference(q, k, v, [0, slots], slots, 0, 0.125, dtype):
+        ref.check(got, want, bound)
