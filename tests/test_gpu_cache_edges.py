@@ -2,6 +2,8 @@
 allows, against their definitions in 64 bits (tests/cache_reference.py)."""
 import ctypes
 import re
+import subprocess
+import sys
 import textwrap
 from pathlib import Path
 
@@ -322,3 +324,43 @@ def test_attention_of_the_largest_values(mode):
     got = ops.window_attention(q, k, v, window=slots)
     for _, _, want, bound in window_reference(q, k, v, [0, slots], slots, 0, 0.125, dtype):
         ref.check(got, want, bound)
+
+
+FIRST_CALLS = """
+import sys
+import torch
+from streaming_transformer_b200 import attention as ops
+
+def rows(*shape):
+    return torch.arange(torch.tensor(shape).prod().item(), device="cuda").remainder(7).sub(3).view(shape).to(dtype)
+
+mode = sys.argv[1]
+dtype = {"fp32": torch.float32, "mixed": torch.float16}.get(mode, torch.bfloat16)
+cache = ops.new_cache(2, 2, 3000, 64, mode=mode)
+scales = dict(key_scales=cache[2], value_scales=cache[3])
+q, k, v = (rows(2, h, 64) for h in (4, 2, 2))
+many = [rows(300, h, 64) for h in (4, 2, 2)]
+at, f = torch.tensor([5, 2999], device="cuda"), ops.rotation_frequencies(64)
+calls = {
+    "append": lambda: ops.cache_append(q, k, v, *cache[:2], at, f, **scales),
+    "attend": lambda: ops.cache_attention(q, *cache[:2], at, **scales),
+    "unpack": lambda: ops.unpack_cache(*cache[:2], **scales)[0],
+    "window": lambda: ops.window_attention(*many, window=90),
+}
+side = torch.cuda.Stream()
+for name in ("append", "attend") + (("unpack",) if mode == "int4" else ("window",)):
+    graph = torch.cuda.CUDAGraph()
+    side.wait_stream(torch.cuda.current_stream())
+    with torch.cuda.stream(side), torch.cuda.graph(graph, stream=side):
+        out = calls[name]()
+    torch.cuda.current_stream().wait_stream(side)
+    graph.replay()
+    assert torch.equal(out, calls[name]()), name
+"""
+
+
+@pytest.mark.parametrize("mode", ["fp32", "bf16", "int4"])
+def test_a_first_call_can_be_captured(mode):
+    # in a process of its own, so that nothing has loaded the kernels before
+    done = subprocess.run([sys.executable, "-c", FIRST_CALLS, mode], cwd=Path(__file__).parents[1], capture_output=True, text=True, timeout=300)
+    assert done.returncode == 0, done.stderr[-2000:]
