@@ -9,10 +9,11 @@
 // 2^-24 turns, where an fp32 product would lose it to 2^-4).
 // A head's row is a group of lanes with 8 columns each; the mean square is a
 // shuffle sum inside the group. Every row that a result or a slot needs is read
-// once and written once. 8192 fp32 rows of 32 and 8 heads of 128 take 57.7 us,
-// 0.97 of the copy bandwidth. 16-bit rows are bound by instructions, as 8 columns
-// cost as many whatever their type: 16384 take 79 us if all are inserted, and 65.5
-// with 8 streams of 2048 and a window of 512 (72 into 4-bit rows).
+// once and written once. 8192 fp32 rows of 8 streams, 32 and 8 heads of 128, take
+// 68 us if all are inserted (window 4096), 0.90 of the copy bandwidth, and 57 with
+// a window of 512. 16-bit rows are bound by instructions, as 8 columns
+// cost as many whatever their type: 16384 take 79 to 82 us if all are inserted, and
+// 66 with a window of 512 (72 into 4-bit rows).
 // All that a CTA needs is on its way before it knows whose its row is.
 #include "st_cache.cuh"
 #include "st_cache_host.h"

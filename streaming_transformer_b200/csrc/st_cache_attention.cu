@@ -1,10 +1,11 @@
 // st_cache_attention.cu -- one query row per stream over its cache
 // (st_cache_attention).
 //
-// The bound is memory: every seen key and value row is read once, and each
+// The bound is memory: every seen key and value row has to be read, and each
 // byte of a 16-bit row meets one multiply-add per query head of its group. A
 // kernel for a head alone would read the rows once per head, so a CTA takes all
-// query heads of a key head (in blocks of 8 or 16), and 16-bit and 4-bit rows
+// query heads of a key head, up to 16 (8 past 128 columns, 4 of fp32 rows); more
+// are dealt to CTAs that each read the rows. 16-bit and 4-bit rows
 // go through mma.sync: a tile of 16 slots is only 16 x 8 x head_dim
 // multiply-adds, a few percent of what even the warp-level instruction does, and
 // its fragments load straight from global memory into the registers that feed
@@ -752,7 +753,9 @@ int heads_per_block(const st_cache* c, int heads) {
 }
 
 // CTAs that share the slots of one key head. One for each SM while each still has
-// 64 slots, if that makes at least 6 of them (the join costs 1.5 us: one stream of
+// 64 slots, if that makes at least 6 of them; whole steps are dealt, of 64 slots
+// (128 of narrow 4-bit rows), so that some parts can stay empty: 504 slots in 7
+// parts are 8 steps, 2 each for 4 of them (the join costs 1.5 us: one stream of
 // 16 heads, 260 slots, takes 4.6 us whole and 5.2 in 4 parts, with 504 slots 6.2
 // whole and 5.2 in 7); up to 12 for each SM while each has 512, so that streams of
 // uneven lengths even out (6, 8 and 12 for each SM: 64, 60 and 61 us at fp16, 129,

@@ -23,7 +23,8 @@
 // room for one key tile, the waits for its copy and for the products set the pace
 // (8192 rows, window 4096, 32 heads of 128: 529 us, now 465, 0.53 of the measured
 // dense rate; what bounds it is the chain S, softmax, O of each query tile, 3700
-// cycles a key tile where exponentials and products take 2050 each). O is rescaled only when a row's maximum
+// cycles a key tile where exponentials and products take 2050 each; the rest has
+// not been measured). O is rescaled only when a row's maximum
 // has grown by more than 2^8 since the last time; P then stays below 2^8, which
 // both 16-bit types hold, and l and O share the reference, so the quotient is
 // exact.
@@ -162,7 +163,7 @@ __device__ __forceinline__ bool wait_phase(unsigned long long* bar, unsigned par
 // DP: columns, padded to 64, 128 or 256 with zeros by the copies; SUBS: query tiles of a CTA. S and O take DP TMEM
 // columns each for each query tile, so that one CTA of 128 or 256 columns, or two (four of one query tile) of 64, fill an
 // SM's TMEM. Key tiles are DP rows, of 256 columns 64: shared memory holds no more (2 sequences of 4000 rows, window 4000,
-// 16 heads of 256: 562 us, 619 TFLOP/s).
+// 16 heads of 256: 550 us, 622 TFLOP/s).
 template <int DP, int SUBS>
 struct Tiles {
   static constexpr int kKeys = DP == 256 ? 64 : DP, kBlocks = kKeys / kBlockRows, kPanels = DP / 64;
