@@ -123,13 +123,14 @@ def test_weights_of_fp16_rows_over_four_bits_keep_the_precision_of_fp16(heads, k
 
 def recipe(where):
     """The documented calls: (for the backlogs, for each further event)."""
-    text = ops.__doc__ if where == "module" else (Path(__file__).parents[1] / where).read_text()
+    guides = (path.read_text() for path in Path(__file__).parents[1].glob("*.md"))
+    text = ops.__doc__ if where == "module" else next(text for text in guides if "= new_cache(" in text)
     block = re.search(r"^ *keys, values.*= new_cache\(.*?(?=^ *```|^ *$)", text, re.M | re.S)[0]
     backlogs, events = re.split(r"^# then.*\n", textwrap.dedent(block), flags=re.M)
     return backlogs, events
 
 
-@pytest.mark.parametrize("where", ["module", "INTEGRATION.md"])
+@pytest.mark.parametrize("where", ["module", "guide"])
 def test_the_documented_calls_give_the_attention_of_each_streams_history(where):
     # two streams with backlogs, one without, and one that stays idle
     g = generator(55)
