@@ -365,3 +365,66 @@ def test_a_first_call_can_be_captured(mode):
     # in a process of its own, so that nothing has loaded the kernels before
     done = subprocess.run([sys.executable, "-c", FIRST_CALLS, mode], cwd=Path(__file__).parents[1], capture_output=True, text=True, timeout=300)
     assert done.returncode == 0, done.stderr[-2000:]
+
+
+@pytest.mark.parametrize("mode", ["fp32", "mixed", "bf16", "int4"])
+def test_append_rotates_keys_in_place(mode):
+    # the C call's q_out and k_out may be q and k themselves
+    g, lib = generator(64), c_calls.entry_points()
+    dtype, types = TYPES.get(mode, torch.bfloat16), {"fp32": 0, "mixed": 1, "bf16": 2, "int4": 3}
+    streams, heads, kv, dim, window, sinks, sizes = 3, 6, 2, 96, 9, 2, [30, 0, 7]
+    n = sum(sizes)
+    q, k, v = (normal(g, n, h, dim, dtype=dtype) for h in (heads, kv, kv))
+    gains = [0.5 + torch.rand(dim, generator=g, device="cuda") for _ in range(2)]
+    at, starts, f = torch.tensor([3, 5, 1000], device="cuda"), starts_of(sizes), ops.rotation_frequencies(dim)
+    caches = [ops.new_cache(streams, kv, window, dim, sinks=sinks, mode=mode) for _ in range(2)]
+    want = ops.cache_append(q, k, v, *caches[0][:2], at, f, sinks=sinks, starts=starts, q_gain=gains[0], k_gain=gains[1], epsilon=1e-5,
+                            rotated_keys=True, **scales_of(caches[0]))
+    keys, values, ks, vs = caches[1]
+    slots = sinks + window
+    c = c_calls.cache(device=torch.cuda.current_device(), type=types[mode], streams=streams, heads=kv, head_dim=dim, sinks=sinks, window=window,
+                      stream_stride=kv * slots, head_stride=slots, keys=keys.data_ptr(), values=values.data_ptr(),
+                      key_scales=ks.data_ptr() if ks is not None else None, value_scales=vs.data_ptr() if vs is not None else None)
+    rows = [c_calls.Rows(x.data_ptr(), x.stride(0), dim) for x in (q, k, v)]
+    a = c_calls.append(mode=2 if mode == "int4" else types[mode], heads=heads, rows=n, q=rows[0], k=rows[1], v=rows[2], q_out=rows[0], k_out=rows[1],
+                       q_gain=gains[0].data_ptr(), k_gain=gains[1].data_ptr(), epsilon=1e-5, rotary=dim // 2, frequencies=f.data_ptr(),
+                       positions=at.data_ptr(), starts=starts.data_ptr())
+    assert lib.st_cache_append(c, a, torch.cuda.current_stream().cuda_stream) == 0
+    for x, y in zip((q, k, *caches[1]), (*want, *caches[0])):
+        assert x is None or torch.equal(x, y)
+
+
+@pytest.mark.parametrize("mode", ["fp32", "mixed", "bf16", "int4"])
+def test_append_of_rows_that_repeat_or_lie_in_another_order(mode):
+    g = generator(65)
+    dtype = TYPES.get(mode, torch.bfloat16)
+    n, heads, kv, dim = 40, 4, 2, 64
+    pool = normal(g, 100000, dtype=dtype)
+    at, starts, f = torch.tensor([7, 0], device="cuda"), starts_of([25, 15]), ops.rotation_frequencies(dim)
+    for row, head in ((0, dim), (heads * dim, 0), (0, 0), (dim, n * dim), (8, 16), (heads * dim + 24, dim)):
+        q, k, v = (pool[8 * i:].as_strided((n, h, dim), (row, head, 1)) for i, h in enumerate((heads, kv, kv)))
+        caches = [ops.new_cache(2, kv, 11, dim, sinks=1, mode=mode) for _ in range(2)]
+        results = [ops.cache_append(*x, *c[:2], at, f, sinks=1, starts=starts, rotated_keys=True, **scales_of(c))
+                   for x, c in zip(((q, k, v), [t.contiguous() for t in (q, k, v)]), caches)]
+        for x, y in zip((*results[0], *caches[0]), (*results[1], *caches[1])):
+            assert x is None or torch.equal(x, y), (row, head)
+
+
+@pytest.mark.parametrize("mode", ["fp32", "bf16"])
+@pytest.mark.parametrize("dim", [64, 128, 256])
+def test_sequences_whose_offsets_pass_32_bits(mode, dim):
+    # rows 2^24 elements apart: the last ones lie past 2^31 elements, and 2^32 bytes
+    g = generator(66)
+    n, heads, kv, apart = 150, 2, 1, 2 ** 24
+    buffer = torch.empty(n * apart, dtype=TYPES[mode], device="cuda")
+    q, k, v, out = (buffer[4096 * i:].as_strided((n, h, dim), (apart, dim, 1)) for i, h in enumerate((heads, kv, kv, heads)))
+    for x in (q, k, v):
+        x.copy_(normal(g, *x.shape, dtype=TYPES[mode]))
+    assert ops.window_attention(q, k, v, window=50, sinks=1, out=out) is out
+    assert torch.equal(out, ops.window_attention(*(x.contiguous() for x in (q, k, v)), window=50, sinks=1))
+    cache, f = ops.new_cache(1, kv, 30, dim, mode=mode), ops.rotation_frequencies(dim)
+    at, starts = torch.tensor([11], device="cuda"), starts_of([n])
+    want = ops.cache_append(*(x.contiguous() for x in (q, k, v)), *cache[:2], at, f, starts=starts)
+    held = [t.clone() for t in cache[:2]]
+    ops.cache_append(q, k, v, *cache[:2], at, f, starts=starts, out=q)
+    assert torch.equal(q, want) and all(torch.equal(t, h) for t, h in zip(cache[:2], held))
